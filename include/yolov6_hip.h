@@ -37,7 +37,8 @@ enum { Y6_OK = 0, Y6_EINVAL = -1, Y6_EHIP = -2, Y6_EUNSUPPORTED = -3, Y6_ENOMEM 
 enum { Y6_ACT_NONE = 0, Y6_ACT_RELU = 1, Y6_ACT_SILU = 2, Y6_ACT_HARDSWISH = 3 };
 
 /* dtype tags for boundary tensors */
-enum { Y6_F16 = 0, Y6_F32 = 1, Y6_U8 = 2 /* stem input only: uint8 pixels, read as imgs.half()/255 (core/evaler.py:121-123) */ };
+enum { Y6_F16 = 0, Y6_F32 = 1, Y6_U8 = 2 /* stem input only: uint8 pixels, read as imgs.half()/255 (core/evaler.py:121-123) */,
+       Y6_BF16 = 3 /* gradient lists and y6_linear_ce_* only */ };
 
 int y6_abi_version(void);
 /* sizeof of a public struct of this header by its name ("y6_conv_desc", ...), 0 if unknown: a hand-written mirror of these
@@ -803,6 +804,39 @@ int y6_loss_forward_backward(const y6_loss_grad_desc* d, void* stream);
 /* gradient only: d->fwd.out must hold the result of y6_loss_forward on the same operands */
 int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
 
+/* Softmax cross entropy of a linear classifier over many classes, without keeping the logits (no counterpart in the reference, whose
+ * classification losses are sigmoid; the semantics are F.cross_entropy(F.linear(x, weight, bias), target)'s):
+ *   z_nv = x_n . weight_v + bias_v;  lse_n = log sum_v exp z_nv
+ *   loss_n = lse_n - (1 - smoothing) z_n,target(n) - (smoothing / classes) sum_v z_nv, 0 where target(n) == ignore_index
+ *   reduction: every row, the sum, or the sum over max(1, labelled rows)
+ * backward: gradients of x [rows][width], weight [classes][width] and bias [classes], dense, in their type; each may be NULL.
+ * A label that is neither a class nor ignore_index makes the row's loss, and every gradient, NaN.  Rows with ignore_index are not
+ * read and get zeros.  x: rows x_pitch elements apart (0: all rows the same); weight: w_pitch >= width.  All in one type.
+ * lse [rows] (fp32): written by forward (may be NULL there) in units of log 2, read by backward with the same operands.
+ * workspace: 16-byte aligned, y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls. */
+enum { Y6_REDUCE_NONE = 0, Y6_REDUCE_SUM = 1, Y6_REDUCE_MEAN = 2 };
+typedef struct y6_linear_ce_desc {
+    const void* x;
+    const void* weight;
+    const void* bias;              /* or NULL */
+    const int64_t* target;         /* [rows] */
+    int64_t rows, x_pitch, w_pitch, ignore_index;
+    int32_t width, classes, dtype /* Y6_F16 | Y6_BF16 | Y6_F32 */, reduction;
+    float smoothing;
+    int32_t pad;
+    float* loss;                   /* [rows] or one value */
+    float* lse;
+    const float* grad_out;         /* backward: d / d loss, as many as loss */
+    void* dx;
+    void* dw;
+    void* dbias;
+    void* workspace;
+    size_t workspace_bytes;
+} y6_linear_ce_desc;
+size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int backward);
+int y6_linear_ce_forward(const y6_linear_ce_desc* d, void* stream);
+int y6_linear_ce_backward(const y6_linear_ce_desc* d, void* stream);
+
 /* SGD with (Nesterov) momentum over a flat fp32 arena, unscaling and overflow handling fused
  * (torch.optim.SGD as configured by yolov6/solver/build.py:10-30 + GradScaler.step/update, engine.py:258-266):
  *   y6_grad_finite_check  *found_inf = 1 if any gradient is inf/nan
@@ -820,6 +854,32 @@ int y6_sgd_step_grouped(float* param, const float* grad, float* momentum_buf, co
                         const int32_t* found_inf, void* stream);
 int y6_scaler_update(float* scale, int32_t* found_inf, int32_t* growth_tracker, float growth, float backoff, int interval,
                      void* stream);
+
+/* Global norm of many gradient tensors and their clipping (no counterpart in the reference, whose trainer does not clip; the
+ * semantics are torch.nn.utils.clip_grad_norm_'s):
+ *   norm = ||all elements||  (Y6_NORM_L2 | _L1 | _INF; sums in double, no atomics: same gradients, same bits)
+ *   c = min(1, max_norm / (norm + 1e-6));  every gradient *= c, one rounding to its type, nothing written when c is 1
+ * A NaN gradient gives a NaN norm and NaN gradients, an infinite one norm = inf and c = 0.  The list's arrays are HOST arrays read
+ * before the call returns; tensors are dense (any order of their elements), fp16 / bf16 / fp32 mixed, aligned to their elements.
+ * y6_grad_clip refuses lists whose tensors overlap.  norm: one device float.  workspace: y6_grad_norm_workspace_bytes(count). */
+enum { Y6_NORM_L2 = 0, Y6_NORM_L1 = 1, Y6_NORM_INF = 2 };
+typedef struct y6_grad_list {
+    void* const* grads_host;
+    const int64_t* numels_host;
+    const int32_t* dtypes_host;    /* Y6_F16 | Y6_BF16 | Y6_F32 */
+    int32_t count;
+    int32_t norm_type;
+} y6_grad_list;
+size_t y6_grad_norm_workspace_bytes(int count);
+int y6_grad_norm(const y6_grad_list* l, void* workspace, size_t workspace_bytes, float* norm, void* stream);
+int y6_grad_clip(const y6_grad_list* l, double max_norm, void* workspace, size_t workspace_bytes, float* norm, void* stream);
+/* y6_sgd_step_grouped with the gradients clipped inside the update (they are not written): norm = |grad_mul / *scale| * ||grad||,
+ * every gradient multiplied by min(1, max_norm / (norm + 1e-6)).  found_inf (NULL: none): set to 1 when a gradient is inf / nan -
+ * no y6_grad_finite_check needed - and then, or when it was set before, nothing is updated.  norm: one device float or NULL.
+ * param, grad, momentum_buf aligned to 16 bytes, group to 4.  workspace: y6_grad_norm_workspace_bytes(1). */
+int y6_sgd_step_clipped(float* param, const float* grad, float* momentum_buf, const uint8_t* group, size_t n, const float* lr3_host,
+                        const float* wd3_host, float momentum, int nesterov, int first_step, float grad_mul, const float* scale,
+                        int32_t* found_inf, double max_norm, void* workspace, size_t workspace_bytes, float* norm, void* stream);
 
 /* plan builders for the ops above */
 int y6_plan_add_bn_train_stats(y6_plan* p, const y6_bn_train_desc* d);

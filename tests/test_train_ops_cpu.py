@@ -1,0 +1,77 @@
+"""Refusals of the training operators that need no GPU: operands are checked before the library is called."""
+import math
+
+import pytest
+import torch
+
+from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+from yolov6_amd.solver import _is_dense, clip_grad_norm_, grad_norm
+
+
+def _operands(n=4, d=8, v=5, dtype=torch.float32):
+    return torch.zeros(n, d, dtype=dtype), torch.zeros(v, d, dtype=dtype), torch.zeros(n, dtype=torch.int64), torch.zeros(v, dtype=dtype)
+
+
+def test_linear_cross_entropy_refusals():
+    x, w, t, b = _operands()
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        linear_cross_entropy(x, w, t, b)
+    for bad, what in (((x.double(), w.double(), t, b.double()), "one type"), ((x.half(), w, t, b), "one type"), ((x, w, t, b.half()), "one type"),
+                      ((x, w, t.int(), b), "int64"), ((x[:, :7], w, t, b), "fit together"), ((x, w, t[:3], b), "fit together"),
+                      ((x, w, t, b[:4]), "fit together"), ((x, w[0], t, b), "fit together"), ((x, w[:0], t, b[:0]), "no class"),
+                      ((x[:, :0], w[:, :0], t, b), "no class")):
+        with pytest.raises(RuntimeError, match=what):
+            linear_cross_entropy(*bad)
+    with pytest.raises(RuntimeError, match="reduction"):
+        linear_cross_entropy(x, w, t, b, reduction="batchmean")
+    for e in (-0.1, 1.5, math.nan):
+        with pytest.raises(RuntimeError, match="label_smoothing"):
+            linear_cross_entropy(x, w, t, b, label_smoothing=e)
+
+
+def test_native_refusals(hip_lib):
+    """The C entry's own checks, before anything is launched."""
+    import ctypes as C
+    from yolov6_amd import _lib
+    d = _lib.LinearCeDesc()
+    d.x = d.weight = d.target = d.loss = d.lse = d.grad_out = d.dx = 4096
+    d.rows, d.width, d.classes, d.x_pitch, d.w_pitch, d.reduction = 4, 8, 5, 8, 8, 2
+    assert hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 0) > 0 and hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 1) > 0
+    d.workspace, d.workspace_bytes = 4096, 16
+    for call in (hip_lib.y6_linear_ce_forward, hip_lib.y6_linear_ce_backward):
+        assert call(C.byref(d), None) == -1 and b"workspace" in hip_lib.y6_last_error()
+    for field, value, what in (("dtype", 2, b"dtype"), ("rows", 0, b"rows"), ("classes", 0, b"classes"), ("width", 0, b"wide"), ("w_pitch", 7, b"pitch"),
+                               ("smoothing", 1.5, b"smoothing"), ("reduction", 5, b"reduction"), ("weight", 4097, b"aligned"), ("x", None, b"null")):
+        keep = getattr(d, field)
+        setattr(d, field, value)
+        assert hip_lib.y6_linear_ce_forward(C.byref(d), None) == -1 and what in hip_lib.y6_last_error(), field
+        assert hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 1) == 0
+        setattr(d, field, keep)
+    lst = _lib.GradList((C.c_void_p * 2)(4096, 4100), (C.c_int64 * 2)(8, 8), (C.c_int32 * 2)(1, 1), 2, 0)
+    assert hip_lib.y6_grad_clip(C.byref(lst), 1.0, 4096, 1 << 20, 4096, None) == -1 and b"share memory" in hip_lib.y6_last_error()
+    assert hip_lib.y6_grad_clip(C.byref(lst), -1.0, 4096, 1 << 20, 4096, None) == -1 and b"max_norm" in hip_lib.y6_last_error()
+    assert hip_lib.y6_grad_norm(C.byref(lst), 4096, 8, 4096, None) == -1 and b"workspace" in hip_lib.y6_last_error()
+    lst.norm_type = 7
+    assert hip_lib.y6_grad_norm(C.byref(lst), 4096, 1 << 20, 4096, None) == -1 and b"norm" in hip_lib.y6_last_error()
+
+
+def test_gradient_refusals():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        clip_grad_norm_([p], 1.0)
+    with pytest.raises(RuntimeError, match="no CPU fallback"):
+        grad_norm([p.grad])
+    with pytest.raises(RuntimeError, match="type"):
+        grad_norm([p.grad], 0.5)
+    with pytest.raises(RuntimeError, match="max_norm"):
+        clip_grad_norm_([p], -2.0)
+    with pytest.raises(RuntimeError, match="fp16, bf16 or fp32"):
+        grad_norm([p.grad.double()])
+    assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(4))], 1.0)) == 0.0
+
+
+def test_dense_layouts():
+    t = torch.zeros(4, 5, 6)
+    assert _is_dense(t) and _is_dense(t.permute(2, 0, 1)) and _is_dense(t[1:2].permute(0, 2, 1)) and _is_dense(torch.zeros(()))
+    assert not _is_dense(t[:, 1:]) and not _is_dense(t[:, :, 0]) and not _is_dense(torch.zeros(3, 1).expand(3, 4)) and not _is_dense(t[::2])

@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # Y6_LIB_PATH: developer override (e.g. a ceiling-probe build from tools/build_probe_libs.py); never a fallback
 LIB_PATH = os.environ.get("Y6_LIB_PATH") or os.path.join(_HERE, "lib", "libyolov6_hip.so")
 
-Y6_F16, Y6_F32, Y6_U8 = 0, 1, 2
+Y6_F16, Y6_F32, Y6_U8, Y6_BF16 = 0, 1, 2, 3
 ACT_NONE, ACT_RELU, ACT_SILU, ACT_HARDSWISH = 0, 1, 2, 3
 ACT_BY_NAME = {None: ACT_NONE, "relu": ACT_RELU, "silu": ACT_SILU, "hardswish": ACT_HARDSWISH}
 MAX_LEVELS = 4
@@ -221,6 +221,19 @@ class LossGradDesc(C.Structure):
     _fields_ = [("fwd", LossDesc), ("grad_scale", C.c_void_p), ("dpred_scores", C.c_void_p), ("dpred_distri", C.c_void_p)]
 
 
+class GradList(C.Structure):
+    _fields_ = [("grads", C.POINTER(C.c_void_p)), ("numels", C.POINTER(C.c_int64)), ("dtypes", C.POINTER(C.c_int32)), ("count", C.c_int32),
+                ("norm_type", C.c_int32)]
+
+
+class LinearCeDesc(C.Structure):
+    _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64),
+                ("x_pitch", C.c_int64), ("w_pitch", C.c_int64), ("ignore_index", C.c_int64), ("width", C.c_int32), ("classes", C.c_int32),
+                ("dtype", C.c_int32), ("reduction", C.c_int32), ("smoothing", C.c_float), ("pad", C.c_int32), ("loss", C.c_void_p),
+                ("lse", C.c_void_p), ("grad_out", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
 WG_3X3S1, WG_1X1, WG_3X3S2, WG_CONVT = 0, 1, 2, 3
 TOP_NAMES = {1: "bn_stats", 2: "bnact_fwd", 3: "bnact_bwd", 4: "wgrad_transpose", 5: "wgrad", 6: "pack", 7: "pool_bwd",
              8: "head_pack", 9: "head_unpack", 10: "s2d", 11: "bias_grad", 12: "fill", 13: "add", 14: "conv_i8", 15: "absmax", 16: "quantize",
@@ -237,6 +250,7 @@ STRUCTS = {
     "y6_bnact_bwd_desc": BnActBwdDesc, "y6_wgrad_t_desc": WgradTDesc, "y6_wgrad_desc": WgradDesc, "y6_wgrad_nhwc_desc": WgradNhwcDesc, "y6_wgrad_stem_desc": WgradStemDesc, "y6_wgrad_flat_geom": WgradFlatGeom,
     "y6_pack_job": PackJob, "y6_pack_batch_desc": PackBatchDesc, "y6_sppf_bwd_desc": SppfBwdDesc, "y6_dgrad_s2_desc": DgradS2Desc, "y6_sppf_q_desc": SppfQDesc, "y6_head_pack_desc": HeadPackDesc,
     "y6_head_ab_desc": HeadAbDesc, "y6_loss_grad_desc": LossGradDesc,
+    "y6_grad_list": GradList, "y6_linear_ce_desc": LinearCeDesc,
 }
 
 # symbol -> (restype, argtypes); also the list the CPU test checks the .so exports against
@@ -330,6 +344,15 @@ SIGNATURES = {
                               C.c_void_p, C.c_void_p, C.c_void_p]),
     "y6_sgd_step_grouped": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_float),
                                       C.c_float, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "y6_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc), C.c_int]),
+    "y6_linear_ce_forward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
+    "y6_linear_ce_backward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
+    "y6_grad_norm_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "y6_grad_norm": (C.c_int, [C.POINTER(GradList), C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "y6_grad_clip": (C.c_int, [C.POINTER(GradList), C.c_double, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
+    "y6_sgd_step_clipped": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_float),
+                                      C.c_float, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_double, C.c_void_p, C.c_size_t,
+                                      C.c_void_p, C.c_void_p]),
     "y6_scaler_update": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_float, C.c_float, C.c_int, C.c_void_p]),
     "y6_plan_add_bn_train_stats": (C.c_int, [C.c_void_p, C.POINTER(BnTrainDesc)]),
     "y6_plan_add_bn_train_stats_multi": (C.c_int, [C.c_void_p, C.POINTER(BnTrainMultiDesc)]),

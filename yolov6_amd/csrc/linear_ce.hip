@@ -1,0 +1,932 @@
+// linear_ce.hip - softmax cross entropy of a linear classifier, value and gradient, without keeping the logits.
+//
+//   z_nv = x_n . W_v + b_v          lse_n = log sum_v exp z_nv
+//   loss_n = lse_n - (1-e) z_n,t(n) - (e/V) sum_v z_nv               (label smoothing e; rows with ignore_index: 0)
+//   dz_nv = g_n (exp(z_nv - lse_n) - (1-e) [v = t(n)] - e/V)
+//   dx = dz W       dW = dz^T x      db = sum_n dz_n
+//
+// Four matrix products of one tiled kernel (gemm_kernel):
+//   forward     z = W x^T, tile by tile; the epilogue leaves a running maximum and a sum of exponentials per row and tile
+//   backward    for a piece of the vocabulary: z again, its epilogue turns it into dz (16 bits for 16-bit inputs: the operand the
+//               matrix instructions of the next two products take, one rounding), then dx += dz W[piece] and dW[piece] = dz^T x
+// so memory holds one piece of dz (kPieceBytes), never the logits.  Labelled rows are gathered first (`gather_kernel`): rows with
+// ignore_index cost nothing, and an infinity or a NaN in one of them reaches no gradient.
+//
+// No atomics: partial statistics and split products are joined in a fixed order, the same inputs give the same bits.
+#include "common.hpp"
+
+namespace {
+
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
+
+constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
+constexpr size_t kPieceBytes = (size_t)128 << 20;
+constexpr int kRowBytes = 128;             // bytes of the reduction a stage holds per row: 64 fp16 / bf16 or 32 fp32 values
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+// dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
+// adds nothing that fp16 gradients show.  bf16 and fp32 have the range.
+constexpr float kHalfScale = 16384.f;
+
+struct Half {
+    static constexpr int ES = 2, TYPE = Y6_F16;
+    static constexpr float kScale = kHalfScale;
+    typedef _Float16 S;
+    static __device__ __forceinline__ float get(S v) { return (float)v; }
+    static __device__ __forceinline__ S put(float v) { return (S)v; }
+};
+struct Brain {
+    static constexpr int ES = 2, TYPE = Y6_BF16;
+    static constexpr float kScale = 1.f;
+    typedef __bf16 S;
+    static __device__ __forceinline__ float get(S v) { return (float)v; }
+    static __device__ __forceinline__ S put(float v) { return (S)v; }
+};
+struct Single {
+    static constexpr int ES = 4, TYPE = Y6_F32;
+    static constexpr float kScale = 1.f;
+    typedef float S;
+    static __device__ __forceinline__ float get(S v) { return v; }
+    static __device__ __forceinline__ S put(float v) { return v; }
+};
+
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_logf(v); }
+
+// ------------------------------------------------------------------------------------------------------------- rows with a label
+// Block b takes rows [64 b, 64 b + 64): counts the labelled rows before them (N / 256 loads a thread; above kCountRows a kernel of its
+// own counts per block first), then copies its labelled rows to their places, each padded with zeros to a multiple of 16 bytes.
+constexpr int kGatherRows = 64;
+constexpr int kCountRows = 32768;
+
+struct GatherArgs {
+    const char* x;
+    long long pitch;               // bytes
+    const int64_t* target;
+    long long ignore;
+    int rows, width, classes;
+    int vec;                       // rows are multiples of 16 bytes at 16-byte addresses
+    const int* seg;                // labelled rows per block (above kCountRows), or null
+    char* xc;
+    long long cpitch;              // bytes
+    int* rowmap;                   // place -> row
+    int* label;                    // place -> label, -1: not a class
+    int* count;
+    // forward
+    float* loss_rows;              // 0 for rows without a label (reduction none), or null
+    // backward
+    const float* lse;              // by row
+    float* lsec;                   // by place
+    char* dx;                      // rows without a label: zeros
+};
+
+__device__ __forceinline__ int block_count(int mine, int* sh) {       // sum over the 256 threads
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) mine += __shfl_down(mine, d);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mine;
+    __syncthreads();
+    return sh[0] + sh[1] + sh[2] + sh[3];
+}
+
+__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg, int segs) {
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int r = s * kGatherRows + (threadIdx.x & 63);
+    const unsigned long long m = __ballot(r < rows && target[r < rows ? r : 0] != ignore);
+    if (s < segs && (threadIdx.x & 63) == 0) seg[s] = __popcll(m);
+}
+
+template <int ES>
+__global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
+    __shared__ int sh[4];
+    __shared__ int place[kGatherRows];
+    const int r0 = blockIdx.x * kGatherRows;
+    int before = 0;
+    if (a.seg) {
+        for (int i = threadIdx.x; i < (int)blockIdx.x; i += 256) before += a.seg[i];
+    } else {
+        for (int i = threadIdx.x; i < r0; i += 256) before += a.target[i] != a.ignore ? 1 : 0;
+    }
+    before = block_count(before, sh);
+    if (threadIdx.x < 64) {
+        const int r = r0 + threadIdx.x;
+        const long long t = r < a.rows ? a.target[r] : a.ignore;
+        const bool has = r < a.rows && t != a.ignore;
+        const unsigned long long m = __ballot(has);
+        const int p = before + __popcll(m & ((1ull << threadIdx.x) - 1));
+        place[threadIdx.x] = has ? p : -1;
+        if (has) {
+            a.rowmap[p] = r;
+            a.label[p] = t >= 0 && t < a.classes ? (int)t : -1;
+            if (a.lsec) a.lsec[p] = a.lse[r];
+        } else if (r < a.rows && a.loss_rows) {
+            a.loss_rows[r] = 0.f;
+        }
+        if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.count = before + __popcll(m);
+    }
+    __syncthreads();
+    const int rows = a.rows - r0 < kGatherRows ? a.rows - r0 : kGatherRows;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
+    for (int i = wave; i < rows; i += 4) {
+        const int p = place[i];
+        const char* const src = a.x + (long long)(r0 + i) * a.pitch;
+        if (p >= 0) {
+            char* const dst = a.xc + (long long)p * a.cpitch;
+            if (a.vec) {
+                for (int o = lane * 16; o < a.width * ES; o += 1024) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
+            } else {
+                for (int e = lane; e < a.cpitch / ES; e += 64)
+                    reinterpret_cast<U*>(dst)[e] = e < a.width ? reinterpret_cast<const U*>(src)[e] : (U)0;
+            }
+        } else if (a.dx) {
+            char* const dst = a.dx + (long long)(r0 + i) * a.width * ES;
+            for (int e = lane; e < a.width; e += 64) reinterpret_cast<U*>(dst)[e] = (U)0;
+        }
+    }
+}
+
+// rows padded with zeros to multiples of 16 bytes (a weight whose width or address the wide loads do not take)
+template <int ES>
+__global__ __launch_bounds__(256) void pad_kernel(const char* __restrict__ src, long long pitch, int rows, int width, char* __restrict__ dst,
+                                                  long long dpitch) {
+    typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    for (long long r = (long long)blockIdx.x * 4 + wave; r < rows; r += (long long)gridDim.x * 4) {
+        const U* const s = reinterpret_cast<const U*>(src + r * pitch);
+        U* const d = reinterpret_cast<U*>(dst + r * dpitch);
+        for (int e = lane; e < dpitch / ES; e += 64) d[e] = e < width ? s[e] : (U)0;
+    }
+}
+
+// --------------------------------------------------------------------------------------------------------------------- the product
+__device__ __forceinline__ i32x4_t make_rsrc(const void* base, unsigned bytes) {
+    const unsigned long long p = (unsigned long long)base;
+    i32x4_t r;
+    r[0] = (int)(unsigned)(p & 0xffffffffu);
+    r[1] = (int)(unsigned)((p >> 32) & 0xffffu);   // stride 0: raw buffer, byte offsets, range check against the byte count
+    r[2] = (int)bytes;
+    r[3] = 0x00020000;
+    return r;
+}
+// lane i: 16 bytes from rsrc.base + voff(lane) to lds_dst + 16 i; out of range: zeros.  The compiler does not count these requests;
+// the kernel waits for them itself (vmcnt) in front of the barrier that hands the stage over.
+__device__ __forceinline__ void dma16(const i32x4_t& rsrc, unsigned voff, unsigned lds_dst) {
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %3\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep)
+                 : "v"(voff), "s"(rsrc), "s"(__builtin_amdgcn_readfirstlane(lds_dst))
+                 : "memory");
+}
+__device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
+
+// One operand's tile of a stage: ROWS rows (of the result's m or n) by 128 bytes of the reduction.
+//   KC (reduction contiguous in memory): image [row][128 B], its 16-byte pieces permuted by piece ^ (row & 7): eight consecutive rows
+//      read the same piece from eight different bank groups
+//   else (rows of the reduction, m / n contiguous), 16-bit: image [32 columns][reduction 64][64 B], read by the transposing
+//      ds_read_b64_tr_b16; fp32: image [reduction 32][ROWS], read a value at a time
+template <class E, bool KC, int ROWS, int NW>
+struct Operand {
+    static constexpr int kBytes = ROWS * kRowBytes;
+    static constexpr int kInstr = kBytes / 1024;
+    static constexpr int kPer = kInstr / NW;
+    static constexpr int KS = kRowBytes / E::ES;         // values of the reduction per stage
+    static_assert(kInstr % NW == 0, "requests divide over the waves");
+
+    // requests of the stage that starts at value k0 of the reduction; rows r0.. of `extent`, reduction `depth` long
+    static __device__ __forceinline__ void issue(const char* base, long long pitch, int r0, int extent, int k0, int depth, unsigned lds, int wave, int lane) {
+        if (KC) {
+            const long long left = (long long)(extent - r0) * pitch;
+            const i32x4_t rs = make_rsrc(base + (long long)r0 * pitch, (unsigned)(left < kOob ? left : kOob));
+            const int kb = k0 * E::ES + (((lane & 7) ^ (lane >> 3)) << 4);
+            const bool in = kb < depth * E::ES;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int ins = wave * kPer + i;
+                const unsigned voff = (unsigned)(ins * 8 + (lane >> 3)) * (unsigned)pitch + (unsigned)kb;
+                dma16(rs, in ? voff : kOob, lds + ins * 1024);
+            }
+        } else {
+            const long long left = (long long)(depth - k0) * pitch;
+            const i32x4_t rs = make_rsrc(base + (long long)k0 * pitch, (unsigned)(left < kOob ? left : kOob));
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) {
+                const int ins = wave * kPer + i;
+                int k, col;
+                if (E::ES == 2) {
+                    k = (ins & 3) * 16 + (lane >> 2);
+                    col = (ins >> 2) * 32 + (lane & 3) * 8;
+                } else {
+                    const int b = ins * 1024 + lane * 16;
+                    k = b / (ROWS * 4);
+                    col = (b % (ROWS * 4)) / 4;
+                }
+                const unsigned voff = (unsigned)k * (unsigned)pitch + (unsigned)(r0 + col) * E::ES;
+                dma16(rs, r0 + col < extent ? voff : kOob, lds + ins * 1024);
+            }
+        }
+    }
+    // the 32 rows from row f: lane's 16 bytes of sub-step kk (four per stage).  16-bit: reduction values 16 kk + 8 (lane >> 5) + 0..7;
+    // fp32: 8 kk + 4 (lane >> 5) + 0..3
+    static __device__ __forceinline__ u32x4 frag(const char* img, int f, int kk, int lane) {
+        const int half = lane >> 5, l31 = lane & 31;
+        if (KC) {
+            const int r = f + l31;
+            return *reinterpret_cast<const u32x4*>(img + r * kRowBytes + (((kk * 2 + half) ^ (lane & 7)) << 4));
+        } else if (E::ES == 2) {
+            const char* const p = img + (f >> 5) * 4096 + (kk * 16 + half * 8 + ((lane & 15) >> 2)) * 64 + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 256));
+            typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+            const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
+            u32x4 r;
+            r[0] = l2[0], r[1] = l2[1], r[2] = h2[0], r[3] = h2[1];
+            return r;
+        } else {
+            u32x4 r;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(img + ((kk * 8 + half * 4 + i) * ROWS + f + l31) * 4);
+            return r;
+        }
+    }
+};
+
+template <class E>
+__device__ __forceinline__ f32x16_t mma(const u32x4& a, const u32x4& b, f32x16_t c) {
+    if constexpr (E::TYPE == Y6_F16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    } else if constexpr (E::TYPE == Y6_BF16) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
+        return c;
+    }
+}
+
+enum { EPI_STATS, EPI_DZ, EPI_STORE };
+enum { COUNT_NONE, COUNT_N, COUNT_K };
+
+struct GemmArgs {
+    const char *a, *b;
+    long long pa, pb;              // bytes between rows
+    int M, N, K;
+    const int* count;              // labelled rows: the extent that COUNT says
+    int tiles_m, tiles_n, splits;
+    // EPI_STATS, EPI_DZ: m = class, n = labelled row
+    const void* bias;
+    const int* label;
+    float *part_m, *part_s, *part_z, *zt;
+    long long np;                  // rows of the partial statistics' arrays
+    const float *lsec, *coef;      // log2 of the sum of exponentials; g_n / max |g| (null: 1)
+    float smooth, smooth_share;    // e, e / V
+    int class0;                    // first class of the piece
+    char* dz;
+    long long dz_pitch;            // bytes
+    // EPI_STORE: m = column, n = row of the output
+    float* part;                   // [split][N][part_pitch] or null: straight to out
+    long long part_pitch;          // elements
+    int add;                       // add to what the partial product holds
+    char* out;
+    long long out_pitch;           // elements
+    const int* rowmap;             // output row of row n, or null
+    const float *up, *gmax;        // the gradient's factor: *up [/ labelled rows], or *gmax
+    int mean, vec;
+};
+
+// what every gradient is multiplied by at the end: the upstream gradient (over the labelled rows for a mean), or the largest of the
+// rows' upstream gradients, and the inverse of dz's scale
+template <class E>
+__device__ __forceinline__ float grad_factor(const float* up, const float* gmax, int mean, const int* count) {
+    float f = gmax ? *gmax : *up;
+    if (mean) f = f / (float)(*count > 1 ? *count : 1);
+    return f * (1.f / E::kScale);
+}
+
+template <class E, bool VEC>
+__device__ __forceinline__ void store4(char* dst, const float (&v)[4], int left) {
+    typedef typename E::S S;
+    S* const p = reinterpret_cast<S*>(dst);
+    if (VEC && left >= 4) {
+        typedef S S4 __attribute__((ext_vector_type(4)));
+        S4 o;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[j] = E::put(v[j]);
+        *reinterpret_cast<S4*>(p) = o;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (j < left) p[j] = E::put(v[j]);
+    }
+}
+
+template <class E, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int EPI, int COUNT>
+__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM * WN) / 4) void gemm_kernel(const GemmArgs g) {
+    constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+    typedef Operand<E, AKC, BM, NW> OA;
+    typedef Operand<E, BKC, BN, NW> OB;
+    constexpr int kStage = OA::kBytes + OB::kBytes;
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wm = wave % WM, wn = wave / WM;
+    // Block b runs on XCD b % 8: each XCD takes one run of tiles, in groups of eight m-tiles by all n-tiles, so that the tiles it works
+    // on at one time share operand rows in its L2.
+    const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits;
+    const int per = (total + 7) >> 3;
+    const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    if ((int)(blockIdx.x >> 3) >= per || t >= total) return;
+    const int split = t / tiles, tt = t - split * tiles;
+    const int width = 8 * g.tiles_n, grp = tt / width, in = tt - grp * width;
+    const int gm = g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8;
+    const int tm = grp * 8 + in % gm, tn = in / gm;
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int N = COUNT == COUNT_N ? *g.count : g.N, K = COUNT == COUNT_K ? *g.count : g.K;
+    if (n0 >= N) return;
+    const int steps = (K + OA::KS - 1) / OA::KS;
+    const int s0 = (int)((long long)steps * split / g.splits), s1 = (int)((long long)steps * (split + 1) / g.splits);
+
+    f32x16_t acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+
+    const unsigned lds0 = lds_addr(smem);
+    auto issue = [&](int s) {
+        const unsigned st = lds0 + (unsigned)((s - s0) & 1) * kStage;
+        OA::issue(g.a, g.pa, m0, g.M, s * OA::KS, K, st, wave, lane);
+        OB::issue(g.b, g.pb, n0, N, s * OA::KS, K, st + OA::kBytes, wave, lane);
+    };
+    if (s0 < s1) issue(s0);
+    for (int s = s0; s < s1; ++s) {
+        // stage s has landed for every wave, and every wave has left stage s - 1, which the next requests overwrite
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (s + 1 < s1) issue(s + 1);
+        const char* const ia = smem + ((s - s0) & 1) * kStage;
+        const char* const ib = ia + OA::kBytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            u32x4 fa[FM], fb[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) fa[i] = OA::frag(ia, wm * (BM / WM) + i * 32, kk, lane);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) fb[j] = OB::frag(ib, wn * (BN / WN) + j * 32, kk, lane);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[i], fb[j], acc[i][j]);
+        }
+    }
+
+    // lane: row n = lane & 31 of a fragment; its 16 values are m = 8 (q >> 2) + 4 (lane >> 5) + (q & 3)
+    const int half = lane >> 5, l31 = lane & 31;
+    const int mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
+    typedef typename E::S S;
+    if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
+        if (g.bias) {
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
+                    const float b = m < g.M ? E::get(reinterpret_cast<const S*>(g.bias)[g.class0 + m]) : 0.f;
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
+                }
+        }
+    }
+    if constexpr (EPI == EPI_STATS) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = nw + j * 32 + l31;
+            const bool live = n < N;
+            float top = -INFINITY, zsum = 0.f;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) {
+                    const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
+                    if (m < g.M) zsum += acc[i][j][q];
+                    else acc[i][j][q] = -INFINITY;
+                    top = fmaxf(top, acc[i][j][q]);
+                }
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
+            const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) sum += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
+            sum += __shfl_xor(sum, 32);
+            zsum += __shfl_xor(zsum, 32);
+            if (live && half == 0) {
+                const long long o = (long long)(tm * WM + wm) * g.np + n;
+                g.part_m[o] = top == -INFINITY ? -INFINITY : m2;
+                g.part_s[o] = sum;
+                if (g.part_z) g.part_z[o] = zsum;
+            }
+            const int lab = live ? g.label[n] - mw : -1;
+            if (__ballot(lab >= 0 && lab < BM / WM)) {
+                float z = 0.f;
+                bool hit = false;
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if (lab == i * 32 + 8 * (q >> 2) + 4 * half + (q & 3)) {
+                            z = acc[i][j][q];
+                            hit = true;
+                        }
+                if (hit) g.zt[n] = z;
+            }
+        }
+    } else if constexpr (EPI == EPI_DZ) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = nw + j * 32 + l31;
+            if (n >= N) continue;
+            const float l2 = g.lsec[n];
+            const float c = (g.coef ? g.coef[n] : 1.f) * E::kScale;
+            const int lab = g.label[n] - g.class0;
+            char* const row = g.dz + (long long)n * g.dz_pitch;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {
+                    const int m = mw + i * 32 + 8 * gq + 4 * half;
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float d = exp2_fast(fmaf(acc[i][j][4 * gq + e], kLog2e, -l2)) - g.smooth_share;
+                        if (m + e == lab) d -= 1.f - g.smooth;
+                        v[e] = m + e < g.M ? d * c : 0.f;
+                    }
+                    // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
+                    if ((long long)m * E::ES < g.dz_pitch) store4<E, true>(row + (long long)m * E::ES, v, (int)(g.dz_pitch / E::ES) - m);
+                }
+        }
+    } else {
+        const float f = g.part ? 1.f : grad_factor<E>(g.up, g.gmax, g.mean, g.count);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = nw + j * 32 + l31;
+            if (n >= N) continue;
+            const long long row = !g.part && g.rowmap ? g.rowmap[n] : n;
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int gq = 0; gq < 4; ++gq) {
+                    const int m = mw + i * 32 + 8 * gq + 4 * half;
+                    if (m >= g.M) continue;
+                    if (g.part) {
+                        f32x4_t* const p = reinterpret_cast<f32x4_t*>(g.part + ((long long)split * g.N + n) * g.part_pitch + m);
+                        f32x4_t v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e];
+                        if (g.add) v += *p;
+                        *p = v;
+                    } else {
+                        float v[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e] * f;
+                        char* const dst = g.out + (row * g.out_pitch + m) * E::ES;
+                        if (g.vec) store4<E, true>(dst, v, g.M - m);
+                        else store4<E, false>(dst, v, g.M - m);
+                    }
+                }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------------------------- small kernels
+// 16 places x 16 slices of the tiles' statistics per block: lse and loss of each labelled row
+struct FinishArgs {
+    const float *part_m, *part_s, *part_z, *zt;
+    long long np;
+    int parts;
+    const int *rowmap, *label, *count;
+    float smooth, smooth_share;
+    float* lse;                    // by row: log2 of the sum of exponentials, or null
+    float* rows_out;               // by row (reduction none) or null
+    float* lossc;                  // by place
+};
+__global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
+    __shared__ float sm[16][17], ss[16][17], sz[16][17];
+    const int i = threadIdx.x & 15, sl = threadIdx.x >> 4;
+    const int n = blockIdx.x * 16 + i, N = *a.count;
+    float m = -INFINITY, s = 0.f, z = 0.f;
+    if (n < N) {
+        for (int p = sl; p < a.parts; p += 16) {
+            const float pm = a.part_m[(long long)p * a.np + n], ps = a.part_s[(long long)p * a.np + n];
+            if (a.part_z) z += a.part_z[(long long)p * a.np + n];
+            const float nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
+            s = s * exp2_fast(m - ref) + ps * exp2_fast(pm - ref);
+            m = nm;
+        }
+    }
+    sm[i][sl] = m, ss[i][sl] = s, sz[i][sl] = z;
+    __syncthreads();
+    if (sl != 0 || n >= N) return;
+    for (int k = 1; k < 16; ++k) m = fmaxf(m, sm[i][k]);
+    const float ref = m == -INFINITY ? 0.f : m;
+    s = 0.f, z = 0.f;
+    for (int k = 0; k < 16; ++k) {
+        s += ss[i][k] * exp2_fast(sm[i][k] - ref);
+        z += sz[i][k];
+    }
+    // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
+    float l2 = ref + log2_fast(s);
+    float loss = l2 * kLn2 - (1.f - a.smooth) * a.zt[n];
+    if (a.smooth > 0.f) loss -= a.smooth_share * z;
+    if (a.label[n] < 0) l2 = loss = NAN;       // a label that is no class
+    const int row = a.rowmap[n];
+    if (a.lse) a.lse[row] = l2;
+    if (a.rows_out) a.rows_out[row] = loss;
+    if (a.lossc) a.lossc[n] = loss;
+}
+
+__global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ lossc, const int* __restrict__ count, int mean, float* __restrict__ loss) {
+    __shared__ double sh[16];
+    const int N = *count;
+    double s = 0;
+    for (int i = threadIdx.x; i < N; i += 1024) s += (double)lossc[i];
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) s += __shfl_down(s, d);
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) s += sh[w];
+    *loss = (float)(mean ? s / (N > 1 ? N : 1) : s);
+}
+
+// reduction none: gmax = max |g| over the labelled rows, coef = g / gmax.  A gradient that is not finite makes all of them NaN.
+__global__ __launch_bounds__(1024) void coef_kernel(const float* __restrict__ up, const int* __restrict__ rowmap, const int* __restrict__ count,
+                                                    float* __restrict__ coef, float* __restrict__ gmax) {
+    __shared__ float sh[16];
+    const int N = *count;
+    float top = 0.f;
+    for (int i = threadIdx.x; i < N; i += 1024) {
+        const float v = fabsf(up[rowmap[i]]);
+        top = v > top || v != v ? v : top;
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) {
+        const float v = __shfl_xor(top, d);
+        top = v > top || v != v ? v : top;
+    }
+    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
+    __syncthreads();
+    top = sh[0];
+    for (int w = 1; w < 16; ++w) top = sh[w] > top || sh[w] != sh[w] ? sh[w] : top;
+    if (threadIdx.x == 0) *gmax = top;
+    for (int i = threadIdx.x; i < N; i += 1024) coef[i] = top > 0.f || top != top ? up[rowmap[i]] / top : 0.f;
+}
+
+// sum of the splits of a product, times the gradient's factor, rounded once
+struct JoinArgs {
+    const float* part;
+    long long part_pitch, part_rows;   // part: [split][part_rows][part_pitch]
+    int rows, width, splits;
+    char* out;
+    long long out_pitch;               // elements
+    const int *rowmap, *count;
+    int count_rows;                    // rows: *count
+    const float *up, *gmax;
+    int mean, vec;
+};
+template <class E>
+__global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
+    const int rows = a.count_rows ? *a.count : a.rows;
+    const float f = grad_factor<E>(a.up, a.gmax, a.mean, a.count);
+    const int q = (a.width + 3) >> 2;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * q; i += (long long)gridDim.x * 256) {
+        const int n = (int)(i / q), m = (int)(i - (long long)n * q) * 4;
+        f32x4_t s = *reinterpret_cast<const f32x4_t*>(a.part + (long long)n * a.part_pitch + m);
+        for (int k = 1; k < a.splits; ++k) s += *reinterpret_cast<const f32x4_t*>(a.part + ((long long)k * a.part_rows + n) * a.part_pitch + m);
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = s[e] * f;
+        const long long row = a.rowmap ? a.rowmap[n] : n;
+        char* const dst = a.out + (row * a.out_pitch + m) * E::ES;
+        if (a.vec) store4<E, true>(dst, v, a.width - m);
+        else store4<E, false>(dst, v, a.width - m);
+    }
+}
+
+// db of a piece: columns of dz summed over the labelled rows, blockIdx.y's share of them -> part[y][class]
+constexpr int kBiasRows = 32;          // shares at most
+template <class E>
+__global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__ dz, long long pitch, int classes, const int* __restrict__ count,
+                                                        float* __restrict__ part) {
+    __shared__ float sh[4][64];
+    const int N = *count, c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    const int r0 = (int)((long long)N * blockIdx.y / gridDim.y), r1 = (int)((long long)N * (blockIdx.y + 1) / gridDim.y);
+    float s = 0.f;
+    if (c < classes)
+        for (int r = r0 + w; r < r1; r += 4) s += E::get(*reinterpret_cast<const typename E::S*>(dz + (long long)r * pitch + (long long)c * E::ES));
+    sh[w][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (w == 0 && c < classes) part[(long long)blockIdx.y * classes + c] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+}
+template <class E>
+__global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
+                                                        const float* up, const float* gmax, int mean, const int* count) {
+    const int c = blockIdx.x * 256 + threadIdx.x;
+    if (c >= classes) return;
+    float s = 0.f;
+    for (int k = 0; k < shares; ++k) s += part[(long long)k * classes + c];
+    db[c] = E::put(s * grad_factor<E>(up, gmax, mean, count));
+}
+
+// ----------------------------------------------------------------------------------------------------------------------- host side
+int type_bytes(int t) { return t == Y6_F32 ? 4 : 2; }
+long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
+int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
+
+struct Layout {                        // offsets into the workspace
+    size_t xc, wc, rowmap, label, count, seg, part_m, part_s, part_z, zt, lossc;      // forward (seg, xc .. count: both)
+    size_t lsec, coef, gmax, dz, accx, accw, bpart;                                   // backward
+    size_t bytes;
+    long long cpitch, np;              // bytes; rows
+    int parts, piece, pieces, split_x, split_w, shares;
+    long long dz_pitch, px, pw;
+    bool pad_w;
+};
+
+constexpr int kTile = 128, kWavesM = 2;
+
+// how often a product of `tiles` tiles is cut along its reduction: until it fills the chip, eight steps to a share at least
+int splits_for(long long tiles, long long steps) {
+    long long s = 512 / (tiles > 0 ? tiles : 1);
+    if (s > steps / 8) s = steps / 8;
+    if (s > 32) s = 32;
+    return s < 1 ? 1 : (int)s;
+}
+
+Layout layout(const y6_linear_ce_desc* d, bool backward) {
+    Layout L = {};
+    const int es = type_bytes(d->dtype);
+    const long long n = d->rows, v = d->classes, w = d->width;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t o = at;
+        at += (bytes + 255) / 256 * 256;
+        return o;
+    };
+    L.cpitch = up_to(w * es, 16);
+    L.np = up_to(n, 64);
+    L.pad_w = (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
+    L.xc = take((size_t)n * L.cpitch);
+    L.wc = take(L.pad_w ? (size_t)v * L.cpitch : 0);
+    L.rowmap = take((size_t)n * 4);
+    L.label = take((size_t)n * 4);
+    L.count = take(4);
+    L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
+    if (!backward) {
+        L.parts = ceil_div(v, kTile) * kWavesM;
+        L.part_m = take((size_t)L.parts * L.np * 4);
+        L.part_s = take((size_t)L.parts * L.np * 4);
+        L.part_z = take(d->smoothing > 0.f ? (size_t)L.parts * L.np * 4 : 0);
+        L.zt = take((size_t)n * 4);
+        L.lossc = take((size_t)n * 4);
+    } else {
+        const int ks = kRowBytes / es;
+        long long piece = (long long)(kPieceBytes / ((size_t)n * es)) / kTile * kTile;
+        if (piece < kTile) piece = kTile;
+        if (piece > v) piece = v;
+        L.pieces = ceil_div(v, piece);
+        L.piece = (int)piece;
+        L.dz_pitch = up_to(piece * es, 16);
+        L.split_x = splits_for((long long)ceil_div(w, kTile) * ceil_div(n, kTile), ceil_div(piece, ks));
+        L.split_w = splits_for((long long)ceil_div(w, kTile) * ceil_div(piece, kTile), ceil_div(n, ks));
+        L.px = L.pw = up_to(w, 4);
+        L.shares = n < kBiasRows * 64 ? ceil_div(n, 64) : kBiasRows;
+        L.lsec = take((size_t)n * 4);
+        L.coef = take((size_t)n * 4);
+        L.gmax = take(4);
+        L.dz = take((size_t)n * L.dz_pitch);
+        L.accx = take(d->dx && (L.pieces > 1 || L.split_x > 1) ? (size_t)L.split_x * n * L.px * 4 : 0);
+        L.accw = take(d->dw && L.split_w > 1 ? (size_t)L.split_w * piece * L.pw * 4 : 0);
+        L.bpart = take(d->dbias ? (size_t)L.shares * piece * 4 : 0);
+    }
+    L.bytes = at;
+    return L;
+}
+
+int check_desc(const y6_linear_ce_desc* d, const char* what) {
+    Y6_REQUIRE(d, "%s: null argument", what);
+    Y6_REQUIRE(d->dtype == Y6_F16 || d->dtype == Y6_BF16 || d->dtype == Y6_F32, "%s: dtype %d (fp16, bf16 or fp32)", what, d->dtype);
+    Y6_REQUIRE(d->rows >= 1 && d->rows <= (1 << 30) && d->classes >= 1 && d->classes <= (1 << 30) && d->width >= 1 && d->width <= (1 << 20),
+               "%s: %lld rows x %d wide, %d classes", what, (long long)d->rows, d->width, d->classes);
+    Y6_REQUIRE(d->x && d->weight && d->target, "%s: null argument", what);
+    Y6_REQUIRE(d->x_pitch >= 0 && d->w_pitch >= d->width && d->w_pitch <= (1 << 21), "%s: pitches %lld, %lld", what, (long long)d->x_pitch, (long long)d->w_pitch);
+    Y6_REQUIRE(d->reduction == Y6_REDUCE_NONE || d->reduction == Y6_REDUCE_SUM || d->reduction == Y6_REDUCE_MEAN, "%s: reduction %d", what, d->reduction);
+    Y6_REQUIRE(d->smoothing >= 0.f && d->smoothing <= 1.f, "%s: label smoothing %g", what, (double)d->smoothing);
+    const uintptr_t es = type_bytes(d->dtype);
+    Y6_REQUIRE(((uintptr_t)d->x | (uintptr_t)d->weight | (uintptr_t)d->bias | (uintptr_t)d->dx | (uintptr_t)d->dw | (uintptr_t)d->dbias) % es == 0,
+               "%s: a tensor is not aligned to its elements", what);
+    return Y6_OK;
+}
+
+struct Run {
+    const y6_linear_ce_desc* d;
+    const Layout& L;
+    char* ws;
+    hipStream_t s;
+    template <class T>
+    T* at(size_t o) const { return reinterpret_cast<T*>(ws + o); }
+};
+
+template <class E>
+int launch_gather(const Run& r, bool backward) {
+    const y6_linear_ce_desc* d = r.d;
+    GatherArgs a = {};
+    a.x = (const char*)d->x, a.pitch = d->x_pitch * E::ES, a.target = d->target, a.ignore = d->ignore_index;
+    a.rows = (int)d->rows, a.width = d->width, a.classes = d->classes;
+    a.vec = (d->width * E::ES) % 16 == 0 && a.pitch % 16 == 0 && (uintptr_t)d->x % 16 == 0;
+    a.xc = r.at<char>(r.L.xc), a.cpitch = r.L.cpitch;
+    a.rowmap = r.at<int>(r.L.rowmap), a.label = r.at<int>(r.L.label), a.count = r.at<int>(r.L.count);
+    const int segs = ceil_div(d->rows, kGatherRows);
+    if (d->rows > kCountRows) {
+        a.seg = r.at<int>(r.L.seg);
+        hipLaunchKernelGGL(count_kernel, dim3(ceil_div(segs, 4)), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs);
+        Y6_LAUNCH_CHECK();
+    }
+    if (backward) {
+        a.lse = d->lse, a.lsec = r.at<float>(r.L.lsec);
+        a.dx = (char*)d->dx;
+    } else if (d->reduction == Y6_REDUCE_NONE) {
+        a.loss_rows = d->loss;
+    }
+    hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(256), 0, r.s, a);
+    Y6_LAUNCH_CHECK();
+    if (r.L.pad_w) {
+        const int blocks = ceil_div(d->classes, 4);
+        hipLaunchKernelGGL(pad_kernel<E::ES>, dim3(blocks < 4096 ? blocks : 4096), dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes,
+                           d->width, r.at<char>(r.L.wc), r.L.cpitch);
+        Y6_LAUNCH_CHECK();
+    }
+    return Y6_OK;
+}
+
+template <class E, bool AKC, bool BKC, int EPI, int COUNT>
+int launch_gemm(GemmArgs& g, hipStream_t s) {
+    constexpr int lds = 2 * (kTile + kTile) * kRowBytes;
+    g.tiles_m = ceil_div(g.M, kTile), g.tiles_n = ceil_div(g.N, kTile);
+    if (g.splits < 1) g.splits = 1;
+    const long long total = (long long)g.tiles_m * g.tiles_n * g.splits;
+    Y6_REQUIRE(total <= (1ll << 30), "linear_ce: %lld tiles", total);
+    hipLaunchKernelGGL((gemm_kernel<E, AKC, BKC, kTile, kTile, 2, 2, EPI, COUNT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, s, g);
+    Y6_LAUNCH_CHECK();
+    return Y6_OK;
+}
+
+#define Y6_TRY(expr)                     \
+    do {                                 \
+        const int _rc = (expr);          \
+        if (_rc != Y6_OK) return _rc;    \
+    } while (0)
+
+template <class E>
+int forward(const Run& r) {
+    const y6_linear_ce_desc* d = r.d;
+    const Layout& L = r.L;
+    Y6_TRY(launch_gather<E>(r, false));
+    GemmArgs g = {};
+    g.a = L.pad_w ? r.at<char>(L.wc) : (const char*)d->weight;
+    g.pa = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
+    g.b = r.at<char>(L.xc), g.pb = L.cpitch;
+    g.M = d->classes, g.N = (int)d->rows, g.K = d->width;
+    g.count = r.at<int>(L.count), g.label = r.at<int>(L.label), g.bias = d->bias;
+    g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
+    g.zt = r.at<float>(L.zt), g.np = L.np;
+    Y6_TRY((launch_gemm<E, true, true, EPI_STATS, COUNT_N>(g, r.s)));
+    FinishArgs f = {};
+    f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.zt = g.zt, f.np = L.np, f.parts = L.parts;
+    f.rowmap = r.at<int>(L.rowmap), f.label = g.label, f.count = g.count;
+    f.smooth = d->smoothing, f.smooth_share = d->smoothing / d->classes;
+    f.lse = d->lse;
+    if (d->reduction == Y6_REDUCE_NONE) f.rows_out = d->loss;
+    else f.lossc = r.at<float>(L.lossc);
+    hipLaunchKernelGGL(finish_kernel, dim3(ceil_div(d->rows, 16)), dim3(256), 0, r.s, f);
+    Y6_LAUNCH_CHECK();
+    if (d->reduction != Y6_REDUCE_NONE) {
+        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, f.lossc, f.count, d->reduction == Y6_REDUCE_MEAN ? 1 : 0, d->loss);
+        Y6_LAUNCH_CHECK();
+    }
+    return Y6_OK;
+}
+
+template <class E>
+int backward(const Run& r) {
+    const y6_linear_ce_desc* d = r.d;
+    const Layout& L = r.L;
+    Y6_TRY(launch_gather<E>(r, true));
+    const int* const count = r.at<int>(L.count);
+    const int* const rowmap = r.at<int>(L.rowmap);
+    const float *gmax = nullptr, *coef = nullptr;
+    if (d->reduction == Y6_REDUCE_NONE) {
+        hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, r.s, d->grad_out, rowmap, count, r.at<float>(L.coef), r.at<float>(L.gmax));
+        Y6_LAUNCH_CHECK();
+        gmax = r.at<float>(L.gmax), coef = r.at<float>(L.coef);
+    }
+    const int mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
+    const char* const w = L.pad_w ? r.at<char>(L.wc) : (const char*)d->weight;
+    const long long wp = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
+    char* const dz = r.at<char>(L.dz);
+    const bool accx = L.pieces > 1 || L.split_x > 1;
+    for (int p = 0; p < L.pieces; ++p) {
+        const int v0 = p * L.piece, vn = d->classes - v0 < L.piece ? d->classes - v0 : L.piece;
+        GemmArgs g = {};
+        g.a = w + v0 * wp, g.pa = wp, g.b = r.at<char>(L.xc), g.pb = L.cpitch;
+        g.M = vn, g.N = (int)d->rows, g.K = d->width, g.count = count;
+        g.label = r.at<int>(L.label), g.bias = d->bias, g.class0 = v0;
+        g.lsec = r.at<float>(L.lsec), g.coef = coef;
+        g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
+        g.dz = dz, g.dz_pitch = up_to((long long)vn * E::ES, 16);
+        Y6_TRY((launch_gemm<E, true, true, EPI_DZ, COUNT_N>(g, r.s)));
+        if (d->dbias) {
+            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 64), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count, r.at<float>(L.bpart));
+            Y6_LAUNCH_CHECK();
+            hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), L.shares, vn,
+                               (typename E::S*)d->dbias + v0, d->grad_out, gmax, mean, count);
+            Y6_LAUNCH_CHECK();
+        }
+        if (d->dx) {
+            GemmArgs x = {};
+            x.a = w + v0 * wp, x.pa = wp, x.b = dz, x.pb = g.dz_pitch;
+            x.M = d->width, x.N = (int)d->rows, x.K = vn, x.count = count, x.splits = L.split_x;
+            x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
+            if (accx) {
+                x.part = r.at<float>(L.accx), x.part_pitch = L.px, x.add = p > 0;
+            } else {
+                x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = rowmap;
+                x.vec = (d->width * E::ES) % (4 * E::ES) == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
+            }
+            Y6_TRY((launch_gemm<E, false, true, EPI_STORE, COUNT_N>(x, r.s)));
+        }
+        if (d->dw) {
+            GemmArgs x = {};
+            x.a = r.at<char>(L.xc), x.pa = L.cpitch, x.b = dz, x.pb = g.dz_pitch;
+            x.M = d->width, x.N = vn, x.K = (int)d->rows, x.count = count, x.splits = L.split_w;
+            x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
+            char* const dw = (char*)d->dw + (long long)v0 * d->width * E::ES;
+            const int vec = d->width % 4 == 0 && (uintptr_t)d->dw % (4 * E::ES) == 0;
+            if (L.split_w > 1) x.part = r.at<float>(L.accw), x.part_pitch = L.pw;
+            else x.out = dw, x.out_pitch = d->width, x.vec = vec;
+            Y6_TRY((launch_gemm<E, false, false, EPI_STORE, COUNT_K>(x, r.s)));
+            if (L.split_w > 1) {
+                JoinArgs j = {};
+                j.part = x.part, j.part_pitch = L.pw, j.part_rows = vn, j.rows = vn, j.width = d->width, j.splits = L.split_w;
+                j.out = dw, j.out_pitch = d->width, j.count = count, j.up = d->grad_out, j.gmax = gmax, j.mean = mean, j.vec = vec;
+                const long long need = ((long long)vn * ((d->width + 3) / 4) + 255) / 256;
+                hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, r.s, j);
+                Y6_LAUNCH_CHECK();
+            }
+        }
+    }
+    if (d->dx && accx) {
+        JoinArgs j = {};
+        j.part = r.at<float>(L.accx), j.part_pitch = L.px, j.part_rows = d->rows, j.rows = (int)d->rows, j.width = d->width, j.splits = L.split_x;
+        j.out = (char*)d->dx, j.out_pitch = d->width, j.rowmap = rowmap, j.count = count, j.count_rows = 1;
+        j.up = d->grad_out, j.gmax = gmax, j.mean = mean;
+        j.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
+        const long long need = (d->rows * ((d->width + 3) / 4) + 255) / 256;
+        hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, r.s, j);
+        Y6_LAUNCH_CHECK();
+    }
+    return Y6_OK;
+}
+
+}  // namespace
+
+// ====================================================================== C ABI
+extern "C" size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int backward_pass) {
+    if (check_desc(d, "linear_ce_workspace_bytes") != Y6_OK) return 0;
+    return layout(d, backward_pass != 0).bytes;
+}
+
+extern "C" int y6_linear_ce_forward(const y6_linear_ce_desc* d, void* stream) {
+    Y6_CLEAR_STALE_ERROR();
+    Y6_TRY(check_desc(d, "linear_ce_forward"));
+    Y6_REQUIRE(d->loss && d->workspace, "linear_ce_forward: null argument");
+    const Layout L = layout(d, false);
+    Y6_REQUIRE(d->workspace_bytes >= L.bytes && (uintptr_t)d->workspace % 16 == 0, "linear_ce_forward: workspace of %zu bytes, %zu needed", d->workspace_bytes, L.bytes);
+    const Run r = {d, L, (char*)d->workspace, (hipStream_t)stream};
+    return d->dtype == Y6_F16 ? forward<Half>(r) : d->dtype == Y6_BF16 ? forward<Brain>(r) : forward<Single>(r);
+}
+
+extern "C" int y6_linear_ce_backward(const y6_linear_ce_desc* d, void* stream) {
+    Y6_CLEAR_STALE_ERROR();
+    Y6_TRY(check_desc(d, "linear_ce_backward"));
+    Y6_REQUIRE(d->lse && d->grad_out && d->workspace, "linear_ce_backward: null argument");
+    if (!d->dx && !d->dw && !d->dbias) return Y6_OK;
+    const Layout L = layout(d, true);
+    Y6_REQUIRE(d->workspace_bytes >= L.bytes && (uintptr_t)d->workspace % 16 == 0, "linear_ce_backward: workspace of %zu bytes, %zu needed", d->workspace_bytes, L.bytes);
+    const Run r = {d, L, (char*)d->workspace, (hipStream_t)stream};
+    return d->dtype == Y6_F16 ? backward<Half>(r) : d->dtype == Y6_BF16 ? backward<Brain>(r) : backward<Single>(r);
+}

@@ -61,7 +61,9 @@ extern "C" size_t y6_abi_sizeof(const char* name) {
         {"y6_sppf_q_desc", sizeof(y6_sppf_q_desc)},
         {"y6_head_pack_desc", sizeof(y6_head_pack_desc)},
         {"y6_head_ab_desc", sizeof(y6_head_ab_desc)},
-        {"y6_loss_grad_desc", sizeof(y6_loss_grad_desc)}};
+        {"y6_loss_grad_desc", sizeof(y6_loss_grad_desc)},
+        {"y6_grad_list", sizeof(y6_grad_list)},
+        {"y6_linear_ce_desc", sizeof(y6_linear_ce_desc)}};
     if (!name) return 0;
     for (const auto& e : kTab)
         if (strcmp(e.n, name) == 0) return e.s;

@@ -6,6 +6,9 @@
                   (core/engine.py:258-266 scaler.step / scaler.update)
     LossScaler    the dynamic loss scale of torch.cuda.amp.GradScaler kept ON DEVICE (no host sync per step)
     ArenaEMA      ModelEMA.update (yolov6/utils/ema.py:27-37) as one lerp over the arena + the BatchNorm buffers
+    clip_grad_norm_, grad_norm
+                  the global norm of any list of gradients and their clipping (torch.nn.utils.clip_grad_norm_'s semantics; the
+                  reference's trainer does not clip); `FusedSGD.step(max_norm=...)` clips inside the update
 The reference's own `torch.optim.SGD` / `GradScaler` also work on the arena-backed parameters (their `.grad`s are arena
 views); these classes are the fast path the benchmark uses.
 """
@@ -30,6 +33,94 @@ def param_groups(model):
         elif hasattr(v, 'weight') and isinstance(v.weight, nn.Parameter):
             g_w.append(v.weight)
     return g_bnw, g_w, g_b
+
+
+_NORMS = {2.0: 0, 1.0: 1, math.inf: 2}
+_GRAD_TYPES = {torch.float16: _lib.Y6_F16, torch.bfloat16: _lib.Y6_BF16, torch.float32: _lib.Y6_F32}
+
+
+def _is_dense(t):
+    """Whether t's elements fill one run of memory, each place once, in whatever order."""
+    if t.is_contiguous():
+        return True
+    run = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != run:
+            return False
+        run *= size
+    return True
+
+
+def _norm_code(norm_type):
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise RuntimeError(f"yolov6_amd: gradient norm of type {norm_type!r} (1, 2 and inf are there)")
+    return code
+
+
+def _grad_list(grads, norm):
+    """The native call's view of `grads` and the tensors that have to outlive it."""
+    device = grads[0].device
+    for g in grads:
+        if g.layout != torch.strided or g.dtype not in _GRAD_TYPES:
+            raise RuntimeError(f"yolov6_amd: gradients must be dense fp16, bf16 or fp32 tensors (got {g.dtype}, {g.layout})")
+        if g.device != device:
+            raise RuntimeError(f"yolov6_amd: gradients on {device} and {g.device}: one norm is taken on one device")
+    _lib.require_gpu_tensor(grads[0], "gradients")
+    n = len(grads)
+    keep = ((C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads]),
+            (C.c_int32 * n)(*[_GRAD_TYPES[g.dtype] for g in grads]))
+    return _lib.GradList(*keep, n, norm), keep
+
+
+def _call_on(grads, norm, call):
+    """call(lib, list, workspace, bytes, norm, stream) for dense `grads`; the norm as a device scalar."""
+    lst, keep = _grad_list(grads, norm)
+    with torch.cuda.device(grads[0].device):
+        lib = _lib.load()
+        ws = torch.empty(lib.y6_grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8, device=grads[0].device)
+        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
+        call(lib, C.byref(lst), C.c_void_p(ws.data_ptr()), ws.numel(), C.c_void_p(out.data_ptr()), _lib.current_stream_ptr())
+    return out
+
+
+@torch.no_grad()
+def grad_norm(grads, norm_type=2.0):
+    """The norm (2, 1 or inf) of all elements of the tensors `grads` together, as an fp32 scalar on their device (no host
+    synchronisation).  Sums are doubles in a fixed order: the same gradients give the same bits.  NaN if any element is NaN."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    code = _norm_code(norm_type)
+    if not grads:
+        return torch.tensor(0.0)
+    grads = [g if _is_dense(g) else g.contiguous() for g in grads]
+    return _call_on(grads, code, lambda lib, *a: _lib.check(lib.y6_grad_norm(*a), "grad_norm"))
+
+
+@torch.no_grad()
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
+    """Scale the gradients of `parameters` (a tensor or an iterable; those without `.grad` are left out, one that comes twice
+    counts once) in place by min(1, max_norm / (norm + 1e-6)), norm = grad_norm of all of them; returns the norm before clipping.
+    The semantics of torch.nn.utils.clip_grad_norm_, in two launches whatever the number of tensors up to 160, without a host
+    synchronisation unless `error_if_nonfinite` asks for the check (then nothing has been scaled when it raises).  Under a
+    LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
+    code = _norm_code(norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise RuntimeError(f"yolov6_amd: max_norm {max_norm} is negative or not a number")
+    if not grads:
+        return torch.tensor(0.0)
+    if any(g.requires_grad for g in grads):
+        raise RuntimeError("yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place")
+    if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
+        raise RuntimeError(f"yolov6_amd: the norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
+    dense = [g if _is_dense(g) else g.contiguous() for g in grads]
+    norm = _call_on(dense, code, lambda lib, lst, *a: _lib.check(lib.y6_grad_clip(lst, max_norm, *a), "grad_clip"))
+    for g, d in zip(grads, dense):
+        if d is not g:
+            g.copy_(d)
+    return norm
 
 
 class LossScaler:
@@ -71,15 +162,29 @@ class FusedSGD:
     def zero_grad(self):
         self.arena.zero_grad()
 
-    def step(self, scaler: LossScaler = None, grad_mul: float = 1.0):
+    def step(self, scaler: LossScaler = None, grad_mul: float = 1.0, max_norm: float = None):
+        """One update.  `max_norm`: clip the gradients (unscaled, times grad_mul) to that global 2-norm first - over the whole arena,
+        so over every trainable parameter - inside the update: `.grad` keeps its values; returns the norm before clipping, an fp32
+        device scalar.  With a GradReducer every rank holds the reduced gradients, so all take the same factor."""
         lib = _lib.load()
         a = self.arena
         s = _lib.current_stream_ptr()
         scale = found = None
         if scaler is not None and scaler.enabled:
             scale, found = C.c_void_p(scaler.scale.data_ptr()), C.c_void_p(scaler.found_inf.data_ptr())
-            _lib.check(lib.y6_grad_finite_check(C.c_void_p(a.grad.data_ptr()), a.numel, found, s), "grad_finite_check")
         lr3, wd3 = (C.c_float * 3)(*self.lr), (C.c_float * 3)(*self.wd)
+        if max_norm is not None:
+            ws = torch.empty(lib.y6_grad_norm_workspace_bytes(1), dtype=torch.uint8, device=a.data.device)
+            norm = torch.empty((), dtype=torch.float32, device=a.data.device)
+            _lib.check(lib.y6_sgd_step_clipped(C.c_void_p(a.data.data_ptr()), C.c_void_p(a.grad.data_ptr()), C.c_void_p(self.buf.data_ptr()),
+                                               C.c_void_p(self.group.data_ptr()), a.numel, lr3, wd3, self.momentum, int(self.nesterov),
+                                               int(self.steps == 0), float(grad_mul), scale, found, float(max_norm), C.c_void_p(ws.data_ptr()),
+                                               ws.numel(), C.c_void_p(norm.data_ptr()), s), "sgd_step_clipped")
+            self.steps += 1
+            bump_native_generation()
+            return norm
+        if found is not None:
+            _lib.check(lib.y6_grad_finite_check(C.c_void_p(a.grad.data_ptr()), a.numel, found, s), "grad_finite_check")
         _lib.check(lib.y6_sgd_step_grouped(C.c_void_p(a.data.data_ptr()), C.c_void_p(a.grad.data_ptr()), C.c_void_p(self.buf.data_ptr()),
                                            C.c_void_p(self.group.data_ptr()), a.numel, lr3, wd3, self.momentum, int(self.nesterov),
                                            int(self.steps == 0), float(grad_mul), scale, found, s), "sgd_step_grouped")
