@@ -13,6 +13,8 @@
 // ignore_index cost nothing, and an infinity or a NaN in one of them reaches no gradient.
 //
 // No atomics: partial statistics and split products are joined in a fixed order, the same inputs give the same bits.
+#include <atomic>
+
 #include "common.hpp"
 
 namespace {
@@ -24,7 +26,7 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
 constexpr size_t kPieceBytes = (size_t)128 << 20;
-constexpr int kRowBytes = 128;             // bytes of the reduction a stage holds per row: 64 fp16 / bf16 or 32 fp32 values
+constexpr int kRowBytes = 128;             // bytes of the reduction of a step, for the splits' count: 64 fp16 / bf16 or 32 fp32 values
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
 // adds nothing that fp16 gradients show.  bf16 and fp32 have the range.
@@ -56,10 +58,11 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_logf(v); }
 
 // ------------------------------------------------------------------------------------------------------------- rows with a label
-// Block b takes rows [64 b, 64 b + 64): counts the labelled rows before them (N / 256 loads a thread; above kCountRows a kernel of its
-// own counts per block first), then copies its labelled rows to their places, each padded with zeros to a multiple of 16 bytes.
-constexpr int kGatherRows = 64;
-constexpr int kCountRows = 32768;
+// Block b takes rows [16 b, 16 b + 16): counts the labelled rows before them (at most kCountRows / 256 loads a thread; with more rows a
+// kernel of its own counts per block first), then copies its labelled rows to their places, each padded with zeros to a multiple of
+// 16 bytes.  Four rows a wave: 4096 x 1024 bf16 are 256 blocks.
+constexpr int kGatherRows = 16;
+constexpr int kCountRows = 2048;
 
 struct GatherArgs {
     const char* x;
@@ -91,10 +94,9 @@ __device__ __forceinline__ int block_count(int mine, int* sh) {       // sum ove
 }
 
 __global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg, int segs) {
-    const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int r = s * kGatherRows + (threadIdx.x & 63);
+    const int r = blockIdx.x * 256 + threadIdx.x, s = r / kGatherRows;
     const unsigned long long m = __ballot(r < rows && target[r < rows ? r : 0] != ignore);
-    if (s < segs && (threadIdx.x & 63) == 0) seg[s] = __popcll(m);
+    if (s < segs && r % kGatherRows == 0) seg[s] = __popcll((m >> (threadIdx.x & 63)) & ((1ull << kGatherRows) - 1));
 }
 
 template <int ES>
@@ -111,16 +113,17 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
     before = block_count(before, sh);
     if (threadIdx.x < 64) {
         const int r = r0 + threadIdx.x;
-        const long long t = r < a.rows ? a.target[r] : a.ignore;
-        const bool has = r < a.rows && t != a.ignore;
+        const bool mine = threadIdx.x < kGatherRows && r < a.rows;
+        const long long t = mine ? a.target[r] : a.ignore;
+        const bool has = mine && t != a.ignore;
         const unsigned long long m = __ballot(has);
         const int p = before + __popcll(m & ((1ull << threadIdx.x) - 1));
-        place[threadIdx.x] = has ? p : -1;
+        if (threadIdx.x < kGatherRows) place[threadIdx.x] = has ? p : -1;
         if (has) {
             a.rowmap[p] = r;
             a.label[p] = t >= 0 && t < a.classes ? (int)t : -1;
             if (a.lsec) a.lsec[p] = a.lse[r];
-        } else if (r < a.rows && a.loss_rows) {
+        } else if (mine && a.loss_rows) {
             a.loss_rows[r] = 0.f;
         }
         if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) *a.count = before + __popcll(m);
@@ -181,30 +184,35 @@ __device__ __forceinline__ void dma16(const i32x4_t& rsrc, unsigned voff, unsign
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
 
-// One operand's tile of a stage: ROWS rows (of the result's m or n) by 128 bytes of the reduction.
-//   KC (reduction contiguous in memory): image [row][128 B], its 16-byte pieces permuted by piece ^ (row & 7): eight consecutive rows
-//      read the same piece from eight different bank groups
-//   else (rows of the reduction, m / n contiguous), 16-bit: image [32 columns][reduction 64][64 B], read by the transposing
-//      ds_read_b64_tr_b16; fp32: image [reduction 32][ROWS], read a value at a time
-template <class E, bool KC, int ROWS, int NW>
+// One operand's tile of a stage: ROWS rows (of the result's m or n) by KB bytes (128 or 64) of the reduction.
+//   KC (reduction contiguous in memory): image [row][KB], its 16-byte pieces permuted so that eight consecutive rows read the same
+//      piece from eight different bank groups
+//   else (rows of the reduction, m / n contiguous), 16-bit: image [32 columns][reduction KB / 2][64 B], read by the transposing
+//      ds_read_b64_tr_b16; fp32: image [reduction KB / 4][ROWS], read a value at a time
+template <class E, bool KC, int ROWS, int NW, int KB>
 struct Operand {
-    static constexpr int kBytes = ROWS * kRowBytes;
+    static constexpr int kBytes = ROWS * KB;
     static constexpr int kInstr = kBytes / 1024;
     static constexpr int kPer = kInstr / NW;
-    static constexpr int KS = kRowBytes / E::ES;         // values of the reduction per stage
+    static constexpr int KS = KB / E::ES;                // values of the reduction per stage
     static_assert(kInstr % NW == 0, "requests divide over the waves");
+    static_assert(KB == 128 || KB == 64, "eight or four pieces a row");
+
+    static __device__ __forceinline__ int permuted(int row, int piece) { return KB == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3); }
 
     // requests of the stage that starts at value k0 of the reduction; rows r0.. of `extent`, reduction `depth` long
     static __device__ __forceinline__ void issue(const char* base, long long pitch, int r0, int extent, int k0, int depth, unsigned lds, int wave, int lane) {
         if (KC) {
+            constexpr int RPI = 1024 / KB;               // rows per request
             const long long left = (long long)(extent - r0) * pitch;
             const i32x4_t rs = make_rsrc(base + (long long)r0 * pitch, (unsigned)(left < kOob ? left : kOob));
-            const int kb = k0 * E::ES + (((lane & 7) ^ (lane >> 3)) << 4);
+            const int lr = lane / (KB / 16);
+            const int kb = k0 * E::ES + (permuted(lr, lane & (KB / 16 - 1)) << 4);
             const bool in = kb < depth * E::ES;
 #pragma unroll
             for (int i = 0; i < kPer; ++i) {
                 const int ins = wave * kPer + i;
-                const unsigned voff = (unsigned)(ins * 8 + (lane >> 3)) * (unsigned)pitch + (unsigned)kb;
+                const unsigned voff = (unsigned)(ins * RPI + lr) * (unsigned)pitch + (unsigned)kb;
                 dma16(rs, in ? voff : kOob, lds + ins * 1024);
             }
         } else {
@@ -215,8 +223,9 @@ struct Operand {
                 const int ins = wave * kPer + i;
                 int k, col;
                 if (E::ES == 2) {
-                    k = (ins & 3) * 16 + (lane >> 2);
-                    col = (ins >> 2) * 32 + (lane & 3) * 8;
+                    constexpr int IPC = KB / 32;         // requests per 32 columns
+                    k = (ins % IPC) * 16 + (lane >> 2);
+                    col = (ins / IPC) * 32 + (lane & 3) * 8;
                 } else {
                     const int b = ins * 1024 + lane * 16;
                     k = b / (ROWS * 4);
@@ -227,15 +236,14 @@ struct Operand {
             }
         }
     }
-    // the 32 rows from row f: lane's 16 bytes of sub-step kk (four per stage).  16-bit: reduction values 16 kk + 8 (lane >> 5) + 0..7;
-    // fp32: 8 kk + 4 (lane >> 5) + 0..3
+    // the 32 rows from row f: lane's 16 bytes of sub-step kk (KB / 32 per stage).  16-bit: reduction values 16 kk + 8 (lane >> 5) +
+    // 0..7; fp32: 8 kk + 4 (lane >> 5) + 0..3
     static __device__ __forceinline__ u32x4 frag(const char* img, int f, int kk, int lane) {
         const int half = lane >> 5, l31 = lane & 31;
         if (KC) {
-            const int r = f + l31;
-            return *reinterpret_cast<const u32x4*>(img + r * kRowBytes + (((kk * 2 + half) ^ (lane & 7)) << 4));
+            return *reinterpret_cast<const u32x4*>(img + (f + l31) * KB + (permuted(l31, kk * 2 + half) << 4));
         } else if (E::ES == 2) {
-            const char* const p = img + (f >> 5) * 4096 + (kk * 16 + half * 8 + ((lane & 15) >> 2)) * 64 + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+            const char* const p = img + (f >> 5) * (KB * 32) + (kk * 16 + half * 8 + ((lane & 15) >> 2)) * 64 + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
             const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
             const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 256));
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
@@ -304,6 +312,16 @@ __device__ __forceinline__ float grad_factor(const float* up, const float* gmax,
     return f * (1.f / E::kScale);
 }
 
+template <class E>
+__device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
+    typedef typename E::S S4 __attribute__((ext_vector_type(4)));
+    S4 o;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = E::put(v[j]);
+    uint2 r;
+    __builtin_memcpy(&r, &o, sizeof(r));
+    return r;
+}
 template <class E, bool VEC>
 __device__ __forceinline__ void store4(char* dst, const float (&v)[4], int left) {
     typedef typename E::S S;
@@ -321,21 +339,34 @@ __device__ __forceinline__ void store4(char* dst, const float (&v)[4], int left)
     }
 }
 
-template <class E, bool AKC, bool BKC, int BM, int BN, int WM, int WN, int EPI, int COUNT>
-__global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM * WN) / 4) void gemm_kernel(const GemmArgs g) {
+// Tile of a block: BM x BN of the result over WM x WN waves, KB bytes of the reduction per stage, STAGES stages, BPC blocks per CU.
+template <int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_, int BPC_>
+struct Tile {
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_, BPC = BPC_, NW = WM_ * WN_;
+    static constexpr int kLds = STAGES_ * (BM_ + BN_) * KB_;
+    static_assert(kLds * BPC_ <= 160 * 1024, "LDS of a CU");
+};
+
+template <int N>
+__device__ __forceinline__ void wait_requests() {       // all but the newest N requests of this wave have landed
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+// One block's tile of a product; `bid` of `8 * ceil(tiles / 8)` blocks.  Block b runs on XCD b % 8: each XCD takes one run of tiles, in
+// groups of eight m-tiles by all n-tiles, so that the tiles it works on at one time share operand rows in its L2.
+template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+__device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char* smem) {
+    constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN;
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
-    typedef Operand<E, AKC, BM, NW> OA;
-    typedef Operand<E, BKC, BN, NW> OB;
+    typedef Operand<E, AKC, BM, NW, T::KB> OA;
+    typedef Operand<E, BKC, BN, NW, T::KB> OB;
     constexpr int kStage = OA::kBytes + OB::kBytes;
-    extern __shared__ __attribute__((aligned(16))) char smem[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave % WM, wn = wave / WM;
-    // Block b runs on XCD b % 8: each XCD takes one run of tiles, in groups of eight m-tiles by all n-tiles, so that the tiles it works
-    // on at one time share operand rows in its L2.
     const int tiles = g.tiles_m * g.tiles_n, total = tiles * g.splits;
     const int per = (total + 7) >> 3;
-    const int t = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-    if ((int)(blockIdx.x >> 3) >= per || t >= total) return;
+    const int t = (bid & 7) * per + (bid >> 3);
+    if ((int)(bid >> 3) >= per || t >= total) return;
     const int split = t / tiles, tt = t - split * tiles;
     const int width = 8 * g.tiles_n, grp = tt / width, in = tt - grp * width;
     const int gm = g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8;
@@ -355,20 +386,27 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM *
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
 
     const unsigned lds0 = lds_addr(smem);
+    unsigned st_in = 0, st_out = 0;                      // stage the next requests fill, stage the next products read
     auto issue = [&](int s) {
-        const unsigned st = lds0 + (unsigned)((s - s0) & 1) * kStage;
+        const unsigned st = lds0 + st_in;
         OA::issue(g.a, g.pa, m0, g.M, s * OA::KS, K, st, wave, lane);
         OB::issue(g.b, g.pb, n0, N, s * OA::KS, K, st + OA::kBytes, wave, lane);
+        st_in = st_in + kStage == T::STAGES * kStage ? 0 : st_in + kStage;
     };
-    if (s0 < s1) issue(s0);
-    for (int s = s0; s < s1; ++s) {
-        // stage s has landed for every wave, and every wave has left stage s - 1, which the next requests overwrite
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < s1) issue(s + 1);
-        const char* const ia = smem + ((s - s0) & 1) * kStage;
-        const char* const ib = ia + OA::kBytes;
+    constexpr int kAhead = T::STAGES - 1;
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) {
+    for (int i = 0; i < kAhead; ++i)
+        if (s0 + i < s1) issue(s0 + i);
+    for (int s = s0; s < s1; ++s) {
+        // stage s has landed for every wave, and every wave has left the stage of s - 1, which the next requests overwrite
+        if (kAhead > 1 && s + kAhead <= s1) wait_requests<(kAhead - 1) * (OA::kPer + OB::kPer)>();
+        else wait_requests<0>();
+        if (s + kAhead < s1) issue(s + kAhead);
+        const char* const ia = smem + st_out;
+        const char* const ib = ia + OA::kBytes;
+        st_out = st_out + kStage == T::STAGES * kStage ? 0 : st_out + kStage;
+#pragma unroll
+        for (int kk = 0; kk < T::KB / 32; ++kk) {
             u32x4 fa[FM], fb[FN];
 #pragma unroll
             for (int i = 0; i < FM; ++i) fa[i] = OA::frag(ia, wm * (BM / WM) + i * 32, kk, lane);
@@ -385,14 +423,16 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM *
     const int half = lane >> 5, l31 = lane & 31;
     const int mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
     typedef typename E::S S;
+    const bool whole = mw + BM / WM <= g.M;              // every class of this wave's tile is one
     if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
         if (g.bias) {
+            const S* const bias = reinterpret_cast<const S*>(g.bias) + g.class0;
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
                 for (int q = 0; q < 16; ++q) {
                     const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
-                    const float b = m < g.M ? E::get(reinterpret_cast<const S*>(g.bias)[g.class0 + m]) : 0.f;
+                    const float b = E::get(bias[m < g.M ? m : g.M - 1]);
 #pragma unroll
                     for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
                 }
@@ -403,44 +443,57 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM *
         for (int j = 0; j < FN; ++j) {
             const int n = nw + j * 32 + l31;
             const bool live = n < N;
-            float top = -INFINITY, zsum = 0.f;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                    const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
-                    if (m < g.M) zsum += acc[i][j][q];
-                    else acc[i][j][q] = -INFINITY;
-                    top = fmaxf(top, acc[i][j][q]);
-                }
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
-            const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
-            float sum = 0.f;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int q = 0; q < 16; ++q) sum += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
-            sum += __shfl_xor(sum, 32);
-            zsum += __shfl_xor(zsum, 32);
-            if (live && half == 0) {
-                const long long o = (long long)(tm * WM + wm) * g.np + n;
-                g.part_m[o] = top == -INFINITY ? -INFINITY : m2;
-                g.part_s[o] = sum;
-                if (g.part_z) g.part_z[o] = zsum;
-            }
-            const int lab = live ? g.label[n] - mw : -1;
-            if (__ballot(lab >= 0 && lab < BM / WM)) {
-                float z = 0.f;
-                bool hit = false;
+            const long long o = (long long)(tm * WM + wm) * g.np + n;
+            const int left = g.M - mw - 4 * half;        // classes of this lane's 4-runs: 32 i + 8 (q >> 2) + (q & 3) < left
+            if (g.part_z) {
+                float zsum = 0.f;
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int q = 0; q < 16; ++q)
-                        if (lab == i * 32 + 8 * (q >> 2) + 4 * half + (q & 3)) {
-                            z = acc[i][j][q];
-                            hit = true;
-                        }
+                        if (whole || i * 32 + 8 * (q >> 2) + (q & 3) < left) zsum += acc[i][j][q];
+                zsum += __shfl_xor(zsum, 32);
+                if (live && half == 0) g.part_z[o] = zsum;
+            }
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q)
+                        if (i * 32 + 8 * (q >> 2) + (q & 3) >= left) acc[i][j][q] = -INFINITY;
+            }
+            float top = acc[0][j][0];
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
+            top = fmaxf(top, __shfl_xor(top, 32));
+            // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
+            const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
+            float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            all += __shfl_xor(all, 32);
+            if (live && half == 0) {
+                g.part_m[o] = top == -INFINITY ? -INFINITY : m2;
+                g.part_s[o] = all;
+            }
+            const int lab = live ? g.label[n] - mw : -1;
+            if (__ballot(lab >= 0 && lab < BM / WM)) {   // a label of these rows lies in this tile: few do
+                const int mine = lab - 4 * half;
+                float z = 0.f;
+                int hit = 0;
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) {
+                        const bool is = mine == i * 32 + 8 * (q >> 2) + (q & 3);
+                        z = is ? acc[i][j][q] : z;
+                        hit = is ? 1 : hit;
+                    }
                 if (hit) g.zt[n] = z;
             }
         }
@@ -451,22 +504,42 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM *
             if (n >= N) continue;
             const float l2 = g.lsec[n];
             const float c = (g.coef ? g.coef[n] : 1.f) * E::kScale;
-            const int lab = g.label[n] - g.class0;
-            char* const row = g.dz + (long long)n * g.dz_pitch;
+            const int lab = g.label[n] - g.class0 - mw - 4 * half;
+            char* const row = g.dz + (long long)n * g.dz_pitch + (long long)(mw + 4 * half) * E::ES;
+            const int left = g.M - mw - 4 * half;
+            const int room = (int)(g.dz_pitch / E::ES) - mw - 4 * half;
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int gq = 0; gq < 4; ++gq) {
-                    const int m = mw + i * 32 + 8 * gq + 4 * half;
-                    float v[4];
+                for (int gp = 0; gp < 2; ++gp) {
+                    float v[2][4];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float d = exp2_fast(fmaf(acc[i][j][4 * gq + e], kLog2e, -l2)) - g.smooth_share;
-                        if (m + e == lab) d -= 1.f - g.smooth;
-                        v[e] = m + e < g.M ? d * c : 0.f;
+                    for (int k = 0; k < 2; ++k)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int m = i * 32 + 16 * gp + 8 * k + e;
+                            float d = exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + e], kLog2e, -l2)) - g.smooth_share;
+                            d -= m == lab ? 1.f - g.smooth : 0.f;
+                            v[k][e] = d * c;
+                        }
+                    if (whole && E::ES == 2) {
+                        // the half-waves trade runs of four classes: each lane then holds eight in a row, one 16-byte store
+                        const uint2 a = pack4<E>(v[0]), b = pack4<E>(v[1]);
+                        const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
+                        const auto y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+                        *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * E::ES) = make_uint4(x[0], y[0], x[1], y[1]);
+                        continue;
                     }
-                    // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
-                    if ((long long)m * E::ES < g.dz_pitch) store4<E, true>(row + (long long)m * E::ES, v, (int)(g.dz_pitch / E::ES) - m);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const int m = i * 32 + 16 * gp + 8 * k;
+                        if (m >= room) continue;
+                        // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (m + e >= left) v[k][e] = 0.f;
+                        store4<E, true>(row + m * E::ES, v[k], room - m);
+                    }
                 }
         }
     } else {
@@ -502,25 +575,42 @@ __global__ __launch_bounds__(WM * WN * 64, (BM * BN > 128 * 128 ? 1 : 2) * (WM *
     }
 }
 
+template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+__global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void gemm_kernel(const GemmArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    gemm_tile<E, AKC, BKC, T, EPI, COUNT>(g, blockIdx.x, smem);
+}
+// dx and dW of a piece in one launch: neither has tiles enough to fill the chip evenly, together they do (way_of_grads)
+template <class E, class T>
+__global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void grads_kernel(const GemmArgs x, const GemmArgs w, unsigned xblocks, int x_first) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    const unsigned wblocks = gridDim.x - xblocks;
+    const bool is_x = x_first ? blockIdx.x < xblocks : blockIdx.x >= wblocks;
+    if (is_x) gemm_tile<E, false, true, T, EPI_STORE, COUNT_N>(x, x_first ? blockIdx.x : blockIdx.x - wblocks, smem);
+    else gemm_tile<E, false, false, T, EPI_STORE, COUNT_K>(w, x_first ? blockIdx.x - xblocks : blockIdx.x, smem);
+}
+
 // ------------------------------------------------------------------------------------------------------------------- small kernels
-// 16 places x 16 slices of the tiles' statistics per block: lse and loss of each labelled row
+// lse and loss of each labelled row: `places` rows (a power of two) x 1024 / places slices of the tiles' statistics per block - 32 rows
+// read whole 128-byte lines, few rows are cut into more slices
 struct FinishArgs {
     const float *part_m, *part_s, *part_z, *zt;
     long long np;
-    int parts;
+    int parts, places;
     const int *rowmap, *label, *count;
     float smooth, smooth_share;
     float* lse;                    // by row: log2 of the sum of exponentials, or null
     float* rows_out;               // by row (reduction none) or null
     float* lossc;                  // by place
 };
-__global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
-    __shared__ float sm[16][17], ss[16][17], sz[16][17];
-    const int i = threadIdx.x & 15, sl = threadIdx.x >> 4;
-    const int n = blockIdx.x * 16 + i, N = *a.count;
+__global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
+    __shared__ float sm[1024], ss[1024], sz[1024];
+    const int i = threadIdx.x & (a.places - 1), sl = threadIdx.x / a.places;
+    int slices = 1024 / a.places;
+    const int n = blockIdx.x * a.places + i, N = *a.count;
     float m = -INFINITY, s = 0.f, z = 0.f;
     if (n < N) {
-        for (int p = sl; p < a.parts; p += 16) {
+        for (int p = sl; p < a.parts; p += slices) {
             const float pm = a.part_m[(long long)p * a.np + n], ps = a.part_s[(long long)p * a.np + n];
             if (a.part_z) z += a.part_z[(long long)p * a.np + n];
             const float nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
@@ -528,18 +618,21 @@ __global__ __launch_bounds__(256) void finish_kernel(const FinishArgs a) {
             m = nm;
         }
     }
-    sm[i][sl] = m, ss[i][sl] = s, sz[i][sl] = z;
-    __syncthreads();
-    if (sl != 0 || n >= N) return;
-    for (int k = 1; k < 16; ++k) m = fmaxf(m, sm[i][k]);
-    const float ref = m == -INFINITY ? 0.f : m;
-    s = 0.f, z = 0.f;
-    for (int k = 0; k < 16; ++k) {
-        s += ss[i][k] * exp2_fast(sm[i][k] - ref);
-        z += sz[i][k];
+    sm[threadIdx.x] = m, ss[threadIdx.x] = s, sz[threadIdx.x] = z;
+    for (; slices > 1; slices >>= 1) {
+        __syncthreads();
+        if (sl < slices / 2) {
+            const int o = threadIdx.x + slices / 2 * a.places;
+            const float pm = sm[o], nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
+            s = s * exp2_fast(m - ref) + ss[o] * exp2_fast(pm - ref);
+            z += sz[o];
+            m = nm;
+            sm[threadIdx.x] = m, ss[threadIdx.x] = s, sz[threadIdx.x] = z;
+        }
     }
+    if (sl != 0 || n >= N) return;
     // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
-    float l2 = ref + log2_fast(s);
+    float l2 = (m == -INFINITY ? 0.f : m) + log2_fast(s);
     float loss = l2 * kLn2 - (1.f - a.smooth) * a.zt[n];
     if (a.smooth > 0.f) loss -= a.smooth_share * z;
     if (a.label[n] < 0) l2 = loss = NAN;       // a label that is no class
@@ -617,20 +710,38 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
     }
 }
 
-// db of a piece: columns of dz summed over the labelled rows, blockIdx.y's share of them -> part[y][class]
-constexpr int kBiasRows = 32;          // shares at most
+// db of a piece: columns of dz summed over the labelled rows, blockIdx.y's share of them -> part[y][class].  A thread takes 16 bytes of
+// a row, 32 threads 512 bytes, eight rows at a time.
+constexpr int kBiasRows = 64;          // shares at most
 template <class E>
 __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__ dz, long long pitch, int classes, const int* __restrict__ count,
                                                         float* __restrict__ part) {
-    __shared__ float sh[4][64];
-    const int N = *count, c = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+    constexpr int V = 16 / E::ES;
+    __shared__ float sh[8][32 * V + 1];
+    const int N = *count, c = (blockIdx.x * 32 + (threadIdx.x & 31)) * V, w = threadIdx.x >> 5;
     const int r0 = (int)((long long)N * blockIdx.y / gridDim.y), r1 = (int)((long long)N * (blockIdx.y + 1) / gridDim.y);
-    float s = 0.f;
-    if (c < classes)
-        for (int r = r0 + w; r < r1; r += 4) s += E::get(*reinterpret_cast<const typename E::S*>(dz + (long long)r * pitch + (long long)c * E::ES));
-    sh[w][threadIdx.x & 63] = s;
+    float s[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) s[e] = 0.f;
+    if (c < classes) {                 // (rows are padded to 16 bytes)
+#pragma unroll 4
+        for (int r = r0 + w; r < r1; r += 8) {
+            typedef typename E::S SV __attribute__((ext_vector_type(V)));
+            const SV v = *reinterpret_cast<const SV*>(dz + (long long)r * pitch + (long long)c * E::ES);
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += E::get(v[e]);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) sh[w][(threadIdx.x & 31) * V + e] = s[e];
     __syncthreads();
-    if (w == 0 && c < classes) part[(long long)blockIdx.y * classes + c] = sh[0][threadIdx.x] + sh[1][threadIdx.x] + sh[2][threadIdx.x] + sh[3][threadIdx.x];
+    for (int i = threadIdx.x; i < 32 * V; i += 256) {
+        const int col = blockIdx.x * 32 * V + i;
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += sh[k][i];
+        if (col < classes) part[(long long)blockIdx.y * classes + col] = t;
+    }
 }
 template <class E>
 __global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
@@ -647,29 +758,87 @@ int type_bytes(int t) { return t == Y6_F32 ? 4 : 2; }
 long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
+// ---- tiles.  kBig: eight waves of 128 x 64 (dx, dW) - 8192 x 8192 x 2048 bf16 at 1.20 PFLOP/s, 128 x 128 tiles reach 1.04 - one
+// block per CU.  kMid: four waves of 64 x 64, two blocks per CU: 2.5 times the blocks for what kBig leaves unfilled.  kSmall: 64 x 64 with
+// three stages in flight: 64 rows x 1000 classes x 512 in 6.0 us against kMid's 9.1, one row x 32000 classes x 1024 in 12.4 against 15.2.
+typedef Tile<256, 256, 2, 4, 128, 2, 1> BigScores;     // stats, dz: a lane's row has 64 classes per fragment column (2 x 4: 1.04, 4 x 2: 0.99 PFLOP/s)
+typedef Tile<256, 256, 4, 2, 128, 2, 1> BigGrads;      // dx, dW (4 x 2: 1.20, 2 x 4: 1.15 PFLOP/s)
+typedef Tile<128, 128, 2, 2, 128, 2, 2> Mid;
+typedef Tile<64, 64, 2, 2, 128, 4, 2> Small;
+enum { kBig, kMid, kSmall, kTiles };
+constexpr int kSide[kTiles] = {256, 128, 64};
+constexpr int kSlots[kTiles] = {256, 512, 512};
+constexpr int kWavesM[kTiles] = {BigScores::WM, Mid::WM, Small::WM};
+// microseconds of one 128-byte step of a block, alone on its CU and beside another, and of its first loads and its epilogue (measured,
+// bf16; fp32 steps hold half the values at a sixteenth of the rate)
+constexpr double kStepAlone[2][kTiles] = {{1.9, 0.75, 0.38}, {1e9, 2.0, 0.6}};
+constexpr double kStepFull[2][kTiles] = {{1.9, 1.06, 0.45}, {1e9, 3.9, 1.0}};
+constexpr double kEnds[kTiles] = {7.0, 4.0, 2.0};
+constexpr double kBytesPerUs = 4e6;
+
+double block_us(int tile, bool fp32, long long steps, long long blocks) {
+    return (blocks <= 256 ? kStepAlone : kStepFull)[fp32][tile] * steps + kEnds[tile];
+}
+// the tile for M x N x `steps` without splits: the one whose rounds of blocks take least
+int way_of_scores(bool fp32, long long m, long long n, long long steps) {
+    int best = kMid;
+    double least = 1e300;
+    for (int t = fp32 ? kMid : kBig; t < kTiles; ++t) {
+        const long long blocks = (long long)ceil_div(m, kSide[t]) * ceil_div(n, kSide[t]);
+        const double us = ceil_div(blocks, kSlots[t]) * block_us(t, fp32, steps, blocks);
+        if (us < least) least = us, best = t;
+    }
+    return best;
+}
+struct GradWay {
+    int tile, split_x, split_w;
+};
+// Tile and splits of a piece's dx (width x rows, reduction `classes`) and dW (width x classes, reduction `rows`) in one launch: the long
+// blocks go first, the short ones fill up behind them; splits cost the traffic of their partial products.
+GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long width, long long classes, int pieces) {
+    const int ks = fp32 ? 32 : 64;
+    const long long kx = ceil_div(classes, ks), kw = ceil_div(rows, ks);
+    GradWay best = {kMid, 1, 1};
+    double least = 1e300;
+    for (int t = fp32 ? kMid : kBig; t < kTiles; ++t)
+        for (int sx = 1; sx <= (dx ? 32 : 1) && (sx == 1 || kx / sx >= 4); sx *= 2)
+            for (int sw = 1; sw <= (dw ? 32 : 1) && (sw == 1 || kw / sw >= 4); sw *= 2) {
+                const long long wide = ceil_div(width, kSide[t]);
+                const long long bx = dx ? wide * ceil_div(rows, kSide[t]) * sx : 0, bw = dw ? wide * ceil_div(classes, kSide[t]) * sw : 0;
+                double ux = block_us(t, fp32, ceil_div(kx, sx), bx + bw), uw = block_us(t, fp32, ceil_div(kw, sw), bx + bw);
+                long long nl = bx, ns = bw;
+                if (uw > ux) {
+                    const double u = ux;
+                    ux = uw, uw = u, nl = bw, ns = bx;
+                }
+                const long long p = kSlots[t], q = nl / p, r = nl % p;
+                double us;
+                const long long fill = r ? (p - r) * (long long)(ux / uw) : 0;
+                if (ns <= fill) us = (q + (r ? 1 : 0)) * ux;
+                else us = (q + (r ? 1 : 0)) * ux + ceil_div(ns - fill, p) * uw;
+                if (dx && (sx > 1 || pieces > 1)) us += (pieces > 1 ? 2.0 : 1.0) * rows * width * 4 * sx / kBytesPerUs;
+                if (dx && sx > 1 && pieces == 1) us += 4 + 1.0 * rows * width * 4 * sx / kBytesPerUs;
+                if (dw && sw > 1) us += 4 + 2.0 * classes * width * 4 * sw / kBytesPerUs;
+                if (us < least) least = us, best = {t, sx, sw};
+            }
+    return best;
+}
+
 struct Layout {                        // offsets into the workspace
     size_t xc, wc, rowmap, label, count, seg, part_m, part_s, part_z, zt, lossc;      // forward (seg, xc .. count: both)
     size_t lsec, coef, gmax, dz, accx, accw, bpart;                                   // backward
     size_t bytes;
     long long cpitch, np;              // bytes; rows
-    int parts, piece, pieces, split_x, split_w, shares;
-    long long dz_pitch, px, pw;
+    int scores, parts, piece, pieces, shares;
+    GradWay grads;
+    long long px, pw;
     bool pad_w;
 };
-
-constexpr int kTile = 128, kWavesM = 2;
-
-// how often a product of `tiles` tiles is cut along its reduction: until it fills the chip, eight steps to a share at least
-int splits_for(long long tiles, long long steps) {
-    long long s = 512 / (tiles > 0 ? tiles : 1);
-    if (s > steps / 8) s = steps / 8;
-    if (s > 32) s = 32;
-    return s < 1 ? 1 : (int)s;
-}
 
 Layout layout(const y6_linear_ce_desc* d, bool backward) {
     Layout L = {};
     const int es = type_bytes(d->dtype);
+    const bool fp32 = d->dtype == Y6_F32;
     const long long n = d->rows, v = d->classes, w = d->width;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -686,31 +855,32 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.label = take((size_t)n * 4);
     L.count = take(4);
     L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
+    const long long steps = ceil_div(w * es, kRowBytes);
     if (!backward) {
-        L.parts = ceil_div(v, kTile) * kWavesM;
+        L.scores = way_of_scores(fp32, v, n, steps);
+        L.parts = ceil_div(v, kSide[L.scores]) * kWavesM[L.scores];
         L.part_m = take((size_t)L.parts * L.np * 4);
         L.part_s = take((size_t)L.parts * L.np * 4);
         L.part_z = take(d->smoothing > 0.f ? (size_t)L.parts * L.np * 4 : 0);
         L.zt = take((size_t)n * 4);
         L.lossc = take((size_t)n * 4);
     } else {
-        const int ks = kRowBytes / es;
-        long long piece = (long long)(kPieceBytes / ((size_t)n * es)) / kTile * kTile;
-        if (piece < kTile) piece = kTile;
+        // pieces of equal size, whole tiles, of about kPieceBytes of dz
+        const long long pieces = (long long)(((size_t)n * v * es + kPieceBytes - 1) / kPieceBytes);
+        long long piece = up_to((v + pieces - 1) / pieces, 256);
         if (piece > v) piece = v;
         L.pieces = ceil_div(v, piece);
         L.piece = (int)piece;
-        L.dz_pitch = up_to(piece * es, 16);
-        L.split_x = splits_for((long long)ceil_div(w, kTile) * ceil_div(n, kTile), ceil_div(piece, ks));
-        L.split_w = splits_for((long long)ceil_div(w, kTile) * ceil_div(piece, kTile), ceil_div(n, ks));
+        L.scores = way_of_scores(fp32, piece, n, steps);
+        L.grads = way_of_grads(fp32, d->dx != nullptr, d->dw != nullptr, n, w, piece, L.pieces);
         L.px = L.pw = up_to(w, 4);
-        L.shares = n < kBiasRows * 64 ? ceil_div(n, 64) : kBiasRows;
+        L.shares = n < kBiasRows * 32 ? ceil_div(n, 32) : kBiasRows;
         L.lsec = take((size_t)n * 4);
         L.coef = take((size_t)n * 4);
         L.gmax = take(4);
-        L.dz = take((size_t)n * L.dz_pitch);
-        L.accx = take(d->dx && (L.pieces > 1 || L.split_x > 1) ? (size_t)L.split_x * n * L.px * 4 : 0);
-        L.accw = take(d->dw && L.split_w > 1 ? (size_t)L.split_w * piece * L.pw * 4 : 0);
+        L.dz = take((size_t)n * up_to(piece * es, 16));
+        L.accx = take(d->dx && (L.pieces > 1 || L.grads.split_x > 1) ? (size_t)L.grads.split_x * n * L.px * 4 : 0);
+        L.accw = take(d->dw && L.grads.split_w > 1 ? (size_t)L.grads.split_w * piece * L.pw * 4 : 0);
         L.bpart = take(d->dbias ? (size_t)L.shares * piece * 4 : 0);
     }
     L.bytes = at;
@@ -753,7 +923,7 @@ int launch_gather(const Run& r, bool backward) {
     const int segs = ceil_div(d->rows, kGatherRows);
     if (d->rows > kCountRows) {
         a.seg = r.at<int>(r.L.seg);
-        hipLaunchKernelGGL(count_kernel, dim3(ceil_div(segs, 4)), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs);
+        hipLaunchKernelGGL(count_kernel, dim3(ceil_div(d->rows, 256)), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs);
         Y6_LAUNCH_CHECK();
     }
     if (backward) {
@@ -773,16 +943,68 @@ int launch_gather(const Run& r, bool backward) {
     return Y6_OK;
 }
 
-template <class E, bool AKC, bool BKC, int EPI, int COUNT>
-int launch_gemm(GemmArgs& g, hipStream_t s) {
-    constexpr int lds = 2 * (kTile + kTile) * kRowBytes;
-    g.tiles_m = ceil_div(g.M, kTile), g.tiles_n = ceil_div(g.N, kTile);
+// (raising a kernel's LDS limit is idempotent: threads that get here together all do it)
+int raise_lds(const void* kern, int lds, std::atomic<unsigned long long>& raised) {
+    if (lds <= 64 * 1024) return Y6_OK;
+    int dev = 0;
+    Y6_HIP(hipGetDevice(&dev));
+    if (dev >= 64 || !(raised.load(std::memory_order_acquire) >> dev & 1)) {
+        Y6_HIP(hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, lds));
+        if (dev < 64) raised.fetch_or(1ull << dev, std::memory_order_release);
+    }
+    return Y6_OK;
+}
+template <class T>
+int set_tiles(GemmArgs& g, unsigned* blocks) {
+    g.tiles_m = ceil_div(g.M, T::BM), g.tiles_n = ceil_div(g.N, T::BN);
     if (g.splits < 1) g.splits = 1;
     const long long total = (long long)g.tiles_m * g.tiles_n * g.splits;
     Y6_REQUIRE(total <= (1ll << 30), "linear_ce: %lld tiles", total);
-    hipLaunchKernelGGL((gemm_kernel<E, AKC, BKC, kTile, kTile, 2, 2, EPI, COUNT>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(256), lds, s, g);
+    *blocks = (unsigned)((total + 7) / 8 * 8);
+    return Y6_OK;
+}
+template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+int launch_tile(GemmArgs& g, hipStream_t s) {
+    static std::atomic<unsigned long long> raised{0};
+    auto* const kern = gemm_kernel<E, AKC, BKC, T, EPI, COUNT>;
+    unsigned blocks = 0;
+    int rc = set_tiles<T>(g, &blocks);
+    if (rc == Y6_OK) rc = raise_lds((const void*)kern, T::kLds, raised);
+    if (rc != Y6_OK) return rc;
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(T::NW * 64), T::kLds, s, g);
     Y6_LAUNCH_CHECK();
     return Y6_OK;
+}
+template <class E, int EPI>
+int launch_scores(int tile, GemmArgs& g, hipStream_t s) {
+    if (tile == kSmall) return launch_tile<E, true, true, Small, EPI, COUNT_N>(g, s);
+    if constexpr (E::ES == 2) {
+        if (tile == kBig) return launch_tile<E, true, true, BigScores, EPI, COUNT_N>(g, s);
+    }
+    return launch_tile<E, true, true, Mid, EPI, COUNT_N>(g, s);
+}
+template <class E, class T>
+int launch_grads_tile(GemmArgs* x, GemmArgs* w, hipStream_t s) {
+    if (!w) return launch_tile<E, false, true, T, EPI_STORE, COUNT_N>(*x, s);
+    if (!x) return launch_tile<E, false, false, T, EPI_STORE, COUNT_K>(*w, s);
+    static std::atomic<unsigned long long> raised{0};
+    auto* const kern = grads_kernel<E, T>;
+    unsigned bx = 0, bw = 0;
+    int rc = set_tiles<T>(*x, &bx);
+    if (rc == Y6_OK) rc = set_tiles<T>(*w, &bw);
+    if (rc == Y6_OK) rc = raise_lds((const void*)kern, T::kLds, raised);
+    if (rc != Y6_OK) return rc;
+    hipLaunchKernelGGL(kern, dim3(bx + bw), dim3(T::NW * 64), T::kLds, s, *x, *w, bx, x->K / x->splits >= w->K / w->splits ? 1 : 0);
+    Y6_LAUNCH_CHECK();
+    return Y6_OK;
+}
+template <class E>
+int launch_grads(int tile, GemmArgs* x, GemmArgs* w, hipStream_t s) {
+    if (tile == kSmall) return launch_grads_tile<E, Small>(x, w, s);
+    if constexpr (E::ES == 2) {
+        if (tile == kBig) return launch_grads_tile<E, BigGrads>(x, w, s);
+    }
+    return launch_grads_tile<E, Mid>(x, w, s);
 }
 
 #define Y6_TRY(expr)                     \
@@ -804,15 +1026,16 @@ int forward(const Run& r) {
     g.count = r.at<int>(L.count), g.label = r.at<int>(L.label), g.bias = d->bias;
     g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
     g.zt = r.at<float>(L.zt), g.np = L.np;
-    Y6_TRY((launch_gemm<E, true, true, EPI_STATS, COUNT_N>(g, r.s)));
+    Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
     FinishArgs f = {};
     f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.zt = g.zt, f.np = L.np, f.parts = L.parts;
+    f.places = d->rows >= 1024 ? 32 : d->rows >= 64 ? 8 : 1;
     f.rowmap = r.at<int>(L.rowmap), f.label = g.label, f.count = g.count;
     f.smooth = d->smoothing, f.smooth_share = d->smoothing / d->classes;
     f.lse = d->lse;
     if (d->reduction == Y6_REDUCE_NONE) f.rows_out = d->loss;
     else f.lossc = r.at<float>(L.lossc);
-    hipLaunchKernelGGL(finish_kernel, dim3(ceil_div(d->rows, 16)), dim3(256), 0, r.s, f);
+    hipLaunchKernelGGL(finish_kernel, dim3(ceil_div(d->rows, f.places)), dim3(1024), 0, r.s, f);
     Y6_LAUNCH_CHECK();
     if (d->reduction != Y6_REDUCE_NONE) {
         hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, f.lossc, f.count, d->reduction == Y6_REDUCE_MEAN ? 1 : 0, d->loss);
@@ -838,7 +1061,8 @@ int backward(const Run& r) {
     const char* const w = L.pad_w ? r.at<char>(L.wc) : (const char*)d->weight;
     const long long wp = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
     char* const dz = r.at<char>(L.dz);
-    const bool accx = L.pieces > 1 || L.split_x > 1;
+    const bool accx = L.pieces > 1 || L.grads.split_x > 1;
+    const int split_x = L.grads.split_x, split_w = L.grads.split_w;
     for (int p = 0; p < L.pieces; ++p) {
         const int v0 = p * L.piece, vn = d->classes - v0 < L.piece ? d->classes - v0 : L.piece;
         GemmArgs g = {};
@@ -848,50 +1072,44 @@ int backward(const Run& r) {
         g.lsec = r.at<float>(L.lsec), g.coef = coef;
         g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
         g.dz = dz, g.dz_pitch = up_to((long long)vn * E::ES, 16);
-        Y6_TRY((launch_gemm<E, true, true, EPI_DZ, COUNT_N>(g, r.s)));
+        Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
         if (d->dbias) {
-            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 64), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count, r.at<float>(L.bpart));
+            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 32 * (16 / E::ES)), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count, r.at<float>(L.bpart));
             Y6_LAUNCH_CHECK();
             hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), L.shares, vn,
                                (typename E::S*)d->dbias + v0, d->grad_out, gmax, mean, count);
             Y6_LAUNCH_CHECK();
         }
-        if (d->dx) {
-            GemmArgs x = {};
-            x.a = w + v0 * wp, x.pa = wp, x.b = dz, x.pb = g.dz_pitch;
-            x.M = d->width, x.N = (int)d->rows, x.K = vn, x.count = count, x.splits = L.split_x;
-            x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
-            if (accx) {
-                x.part = r.at<float>(L.accx), x.part_pitch = L.px, x.add = p > 0;
-            } else {
-                x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = rowmap;
-                x.vec = (d->width * E::ES) % (4 * E::ES) == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
-            }
-            Y6_TRY((launch_gemm<E, false, true, EPI_STORE, COUNT_N>(x, r.s)));
+        GemmArgs x = {}, y = {};
+        x.a = w + v0 * wp, x.pa = wp, x.b = dz, x.pb = g.dz_pitch;
+        x.M = d->width, x.N = (int)d->rows, x.K = vn, x.count = count, x.splits = split_x;
+        x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
+        if (accx) {
+            x.part = r.at<float>(L.accx), x.part_pitch = L.px, x.add = p > 0;
+        } else {
+            x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = rowmap;
+            x.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
         }
-        if (d->dw) {
-            GemmArgs x = {};
-            x.a = r.at<char>(L.xc), x.pa = L.cpitch, x.b = dz, x.pb = g.dz_pitch;
-            x.M = d->width, x.N = vn, x.K = (int)d->rows, x.count = count, x.splits = L.split_w;
-            x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
-            char* const dw = (char*)d->dw + (long long)v0 * d->width * E::ES;
-            const int vec = d->width % 4 == 0 && (uintptr_t)d->dw % (4 * E::ES) == 0;
-            if (L.split_w > 1) x.part = r.at<float>(L.accw), x.part_pitch = L.pw;
-            else x.out = dw, x.out_pitch = d->width, x.vec = vec;
-            Y6_TRY((launch_gemm<E, false, false, EPI_STORE, COUNT_K>(x, r.s)));
-            if (L.split_w > 1) {
-                JoinArgs j = {};
-                j.part = x.part, j.part_pitch = L.pw, j.part_rows = vn, j.rows = vn, j.width = d->width, j.splits = L.split_w;
-                j.out = dw, j.out_pitch = d->width, j.count = count, j.up = d->grad_out, j.gmax = gmax, j.mean = mean, j.vec = vec;
-                const long long need = ((long long)vn * ((d->width + 3) / 4) + 255) / 256;
-                hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, r.s, j);
-                Y6_LAUNCH_CHECK();
-            }
+        y.a = r.at<char>(L.xc), y.pa = L.cpitch, y.b = dz, y.pb = g.dz_pitch;
+        y.M = d->width, y.N = vn, y.K = (int)d->rows, y.count = count, y.splits = split_w;
+        y.up = d->grad_out, y.gmax = gmax, y.mean = mean;
+        char* const dw = (char*)d->dw + (long long)v0 * d->width * E::ES;
+        const int vec = d->width % 4 == 0 && (uintptr_t)d->dw % (4 * E::ES) == 0;
+        if (split_w > 1) y.part = r.at<float>(L.accw), y.part_pitch = L.pw;
+        else y.out = dw, y.out_pitch = d->width, y.vec = vec;
+        if (d->dx || d->dw) Y6_TRY(launch_grads<E>(L.grads.tile, d->dx ? &x : nullptr, d->dw ? &y : nullptr, r.s));
+        if (d->dw && split_w > 1) {
+            JoinArgs j = {};
+            j.part = y.part, j.part_pitch = L.pw, j.part_rows = vn, j.rows = vn, j.width = d->width, j.splits = split_w;
+            j.out = dw, j.out_pitch = d->width, j.count = count, j.up = d->grad_out, j.gmax = gmax, j.mean = mean, j.vec = vec;
+            const long long need = ((long long)vn * ((d->width + 3) / 4) + 255) / 256;
+            hipLaunchKernelGGL(join_kernel<E>, dim3((unsigned)(need < 4096 ? need : 4096)), dim3(256), 0, r.s, j);
+            Y6_LAUNCH_CHECK();
         }
     }
     if (d->dx && accx) {
         JoinArgs j = {};
-        j.part = r.at<float>(L.accx), j.part_pitch = L.px, j.part_rows = d->rows, j.rows = (int)d->rows, j.width = d->width, j.splits = L.split_x;
+        j.part = r.at<float>(L.accx), j.part_pitch = L.px, j.part_rows = d->rows, j.rows = (int)d->rows, j.width = d->width, j.splits = split_x;
         j.out = (char*)d->dx, j.out_pitch = d->width, j.rowmap = rowmap, j.count = count, j.count_rows = 1;
         j.up = d->grad_out, j.gmax = gmax, j.mean = mean;
         j.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
