@@ -5,6 +5,8 @@ Tolerances.  u = torch.finfo(dtype).eps / 2, products exact, fp32 accumulation.
              width * 2^-24 * sum |x w| <= width * 2^-24 * |x| |w| (worst order), lse and the rest by a few 2^-24 of the largest logit
   gradients  dz is rounded once (u |dz|), the result once (u), both accumulated in fp32.  Norm-wise over a whole gradient:
              |d dx| <= u | |dz| |W| | + u |dx|, so each is held to (|dz| |W|) u + u |dx| + the logits' error, elementwise.
+             A probability below fp32's smallest normal number, 2^-126, may be flushed to zero by the exponential and the products
+             (hardware exp2; 1e-38 of a gradient): 2^-126 of the other operand's magnitudes, doubled.
 """
 import math
 
@@ -56,7 +58,7 @@ def _oracle(x, w, b, t, up, smoothing=0.0, reduction="mean", ignore=-100):
 
 def _logit_error(x, w, b):
     e = x.shape[1] * 2.0 ** -24 * float(x.double().norm(dim=1).max()) * float(w.double().norm(dim=1).max())
-    top = float(x.double().norm(dim=1).max()) * float(w.double().norm(dim=1).max()) + (0 if b is None else float(b.abs().max()))
+    top = float(x.double().norm(dim=1).max()) * float(w.double().norm(dim=1).max()) + (0 if b is None else float(b[b.abs() < 1e30].abs().max()))
     return e + 8 * 2.0 ** -24 * (top + math.log(w.shape[0]) + 1)
 
 
@@ -78,7 +80,8 @@ def _check(x, w, b, t, smoothing=0.0, reduction="mean", up=None, ignore=-100):
     # fp32 products accumulate `length` terms: length * 2^-24 of the sum of magnitudes
     for got, leaf, ex, sp, so, length in zip(grads, leaves, exact, spread, soft, (w.shape[0], x.shape[0], x.shape[0])):
         assert got.dtype == leaf.dtype and got.shape == leaf.shape
-        slack = u * sp + u * ex.abs() + 2 * err * so + length * 2.0 ** -24 * sp + 2 ** -20 * so * 2 + tiny
+        flush = 2.0 ** -125 * (length * float(max(x.double().nan_to_num().abs().max(), w.double().abs().max(), 1.0)) * float(up.abs().max()) + 1)
+        slack = u * sp + u * ex.abs() + 2 * err * so + length * 2.0 ** -24 * sp + 2 ** -20 * so * 2 + tiny + flush
         over = (got.double() - ex).abs() - slack * 1.01
         assert bool((over <= 0).all()), (tuple(leaf.shape), float(over.max()), float(ex.abs().max()))
     return loss, grads
@@ -106,3 +109,258 @@ def test_options(dtype, reduction, smoothing, bias):
         up = torch.linspace(-2, 3, 150, device=DEV)
         up[::7] = 0
     _check(x, w, b, t, smoothing, reduction, up)
+
+
+# (rows, width, classes): every tile size, several pieces of the vocabulary (over 128 MB of dz), splits of both gradient products
+LARGE = [(2100, 72, 33000), (4097, 40, 20011), (1100, 1032, 2057), (20000, 64, 81), (40, 136, 70001), (3000, 512, 4100)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,v", LARGE)
+def test_pieces_tiles_and_splits(n, d, v, dtype):
+    x, w, b, t = _inputs(n, d, v, dtype, True, seed=v)
+    _check(x, w, b, t, smoothing=0.1, up=torch.tensor(16.0 * n if dtype == torch.float16 else 1.0, device=DEV))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [24, 25])
+def test_views(dtype, d):
+    """Rows of a wider buffer (at odd addresses), columns of a transposed one, one row for all, more than two dimensions."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(90, 80, 70, dtype, True, seed=d)
+    for cut in (x[:, 3:3 + d], x[::2, 1:1 + d], x.t()[:d].t(), x[:1, 5:5 + d].expand(30, d)):
+        for wcut in (w[:, 7:7 + d], w.t()[:d].t(), w[:1, :d].expand(70, d)):
+            _check(cut, wcut, b, t[:cut.shape[0]], reduction="sum")
+    flat = x[:, :d].contiguous()
+    cube = flat.view(3, 5, 6, d).requires_grad_()
+    loss = linear_cross_entropy(cube, w[:, :d], t.view(3, 5, 6), b, reduction="none")
+    assert loss.shape == (3, 5, 6)
+    (g,) = torch.autograd.grad(loss.sum(), cube)
+    _, grads = _check(flat, w[:, :d], b, t, reduction="none")
+    assert torch.equal(g.view(90, d), grads[0])
+    one = linear_cross_entropy(flat[0], w[:, :d], t[0], b, reduction="none")
+    assert one.shape == () and torch.equal(one, loss.view(-1)[0].detach())
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_rows_without_a_label(dtype):
+    """They are not read: what is in them reaches nothing; all rows without one: loss 0, gradients 0."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(200, 48, 90, dtype, True, seed=1, ignored=0.4)
+    _, clean = _check(x, w, b, t)
+    x[t == -100] = math.nan
+    x[0 if int(t[0]) == -100 else int((t == -100).nonzero()[0]), 0] = math.inf
+    leaves = [o.detach().requires_grad_() for o in (x, w, b)]
+    loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    grads = torch.autograd.grad(loss, leaves)
+    assert bool(torch.isfinite(loss)) and all(torch.equal(a, c) for a, c in zip(grads, clean))
+    none = torch.full_like(t, 7)
+    for reduction in ("mean", "sum", "none"):
+        loss = linear_cross_entropy(leaves[0], leaves[1], none, leaves[2], ignore_index=7, reduction=reduction)
+        grads = torch.autograd.grad(loss.sum(), leaves)
+        assert int(loss.count_nonzero()) == 0 and all(int(g.count_nonzero()) == 0 for g in grads)
+    empty = leaves[0][:0]
+    loss = linear_cross_entropy(empty, leaves[1], t[:0], leaves[2])
+    grads = torch.autograd.grad(loss, leaves)
+    assert float(loss) == 0.0 and all(int(g.count_nonzero()) == 0 for g in grads)
+    assert linear_cross_entropy(empty, leaves[1], t[:0], leaves[2], reduction="none").shape == (0,)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_what_is_not_finite(dtype):
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(70, 32, 300, dtype, True, seed=2, ignored=0.0)
+    # classes switched off by a bias of -infinity (whole tiles of them among others): finite everywhere
+    off = b.clone()
+    off[64:200] = -math.inf
+    off[t.unique()] = 0.0
+    _check(x, w, off, t)
+    lowest = b.clone()
+    lowest[64:200] = torch.finfo(dtype).min
+    lowest[t.unique()] = 0.0
+    _check(x, w, lowest, t)
+    # a label whose class is switched off: infinite loss, as torch
+    off[t[3]] = -math.inf
+    rows = linear_cross_entropy(x, w, t, off, reduction="none")
+    want = torch.nn.functional.cross_entropy(x.float() @ w.float().t() + off.float(), t, reduction="none")
+    assert torch.equal(rows.isinf(), want.isinf()) and torch.equal(rows.isnan(), want.isnan()) and bool(rows[3].isinf())
+    # every class off: NaN, as torch;  a NaN feature: its row alone
+    assert bool(linear_cross_entropy(x, w, t, torch.full_like(b, -math.inf), reduction="none").isnan().all())
+    bad = x.clone()
+    bad[5, 7] = math.nan
+    rows = linear_cross_entropy(bad, w, t, b, reduction="none")
+    assert bool(rows[5].isnan()) and int(rows.isnan().sum()) == 1
+    # a label that is no class: NaN there, and in the gradients
+    for wrong in (300, -1, 1 << 40):
+        tt = t.clone()
+        tt[9] = wrong
+        xg = x.detach().requires_grad_()
+        rows = linear_cross_entropy(xg, w, tt, b, reduction="none")
+        assert bool(rows[9].isnan()) and int(rows.isnan().sum()) == 1
+        (g,) = torch.autograd.grad(linear_cross_entropy(xg, w, tt, b), xg)
+        assert bool(g[9].isnan().all())
+    # large logits: exp of nothing overflows
+    _check(x * 30, w * 30, b, t, reduction="sum")
+
+
+@pytest.mark.parametrize("want", [(0,), (1,), (2,), (0, 1), (1, 2), (0, 2)])
+def test_gradients_that_are_asked_for(want):
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    ops = _inputs(130, 64, 257, torch.bfloat16, True, seed=4)
+    _, every = _check(*ops)
+    leaves = [o.detach().requires_grad_(k in want) for k, o in enumerate(ops[:3])]
+    loss = linear_cross_entropy(leaves[0], leaves[1], ops[3], leaves[2])
+    got = torch.autograd.grad(loss, [leaves[k] for k in want], retain_graph=True)
+    again = torch.autograd.grad(loss, [leaves[k] for k in want])
+    for k, g, a in zip(want, got, again):
+        # (fewer gradients may be cut into other tiles: the same sums in another order)
+        assert torch.equal(g, a) and float((g.double() - every[k].double()).abs().max()) <= 2.0 ** -7 * float(every[k].abs().max())
+
+
+def test_gradient_by_differences():
+    """Central differences of the double-precision loss at bf16-rounded points are not exact here, so of the fp32 kernel's own loss: an
+    fp32 sum of 24 rows is off by 1e-6 of its 60 or so, over a step of 2^-5 by 2e-3 at most."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(24, 16, 40, torch.float32, True, seed=6)
+    leaves = [o.detach().requires_grad_() for o in (x, w, b)]
+    grads = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="sum", label_smoothing=0.1), leaves)
+    g = torch.Generator().manual_seed(1)
+    for k in range(3):
+        way = torch.randn(leaves[k].shape, generator=g).to(DEV)
+        way /= way.norm()
+        ends = []
+        for h in (2.0 ** -5, -2.0 ** -5):
+            moved = [o.detach() + (h * way if i == k else 0) for i, o in enumerate(leaves)]
+            ends.append(float(linear_cross_entropy(moved[0], moved[1], t, moved[2], reduction="sum", label_smoothing=0.1)))
+        # third derivatives along a unit direction are at most of the order of the logits' cubes: h^2 / 6 of it is within 1e-2
+        assert abs((ends[0] - ends[1]) / 2.0 ** -4 - float((grads[k] * way).sum())) <= 2e-3 + 1e-2
+
+
+def test_same_inputs_same_bits():
+    ops = _inputs(1500, 200, 5003, torch.bfloat16, True, seed=8)
+    first = _check(*ops)
+    for _ in range(2):
+        again = _check(*ops)
+        assert torch.equal(first[0], again[0]) and all(torch.equal(a, c) for a, c in zip(first[1], again[1]))
+
+
+def test_once_differentiable():
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(10, 16, 12, torch.float32, True)
+    x.requires_grad_()
+    (g,) = torch.autograd.grad(linear_cross_entropy(x, w, t, b), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        g.sum().backward()
+
+
+def test_autocast_and_the_torch_op():
+    import yolov6_amd.torch_ops  # noqa: F401
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    x, w, b, t = _inputs(100, 40, 333, torch.float32, True, seed=9)
+    leaves = [o.detach().requires_grad_() for o in (x, w, b)]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2])
+    grads = torch.autograd.grad(loss, leaves)
+    low = [o.bfloat16() for o in (x, w, b)]
+    want, wgrads = _check(*low, t)
+    assert torch.equal(loss, want) and all(g.dtype == torch.float32 and torch.equal(g, c.float()) for g, c in zip(grads, wgrads))
+    for reduction in ("mean", "none"):
+        want, wgrads = _check(*low, t, reduction=reduction)
+        leaves = [o.detach().requires_grad_() for o in low]
+        loss, _ = torch.ops.yolov6_hip.linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], -100, 0.0, reduction)
+        grads = torch.autograd.grad(loss.sum(), leaves)
+        assert torch.equal(loss, want) and all(torch.equal(g, c) for g, c in zip(grads, wgrads))
+    loss, _ = torch.ops.yolov6_hip.linear_cross_entropy(low[0].requires_grad_(), low[1], t, None, -100, 0.0, "mean")
+    assert torch.autograd.grad(loss, low[0])[0].shape == low[0].shape
+
+
+def test_another_stream_and_graphs():
+    """A side stream; then two captured steps whose replays alternate with eager ones on new inputs."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+
+    def step(ops):
+        leaves = [o.detach().requires_grad_() for o in ops[:3]]
+        loss = linear_cross_entropy(leaves[0], leaves[1], ops[3], leaves[2], label_smoothing=0.1)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves)]
+
+    sets = [_inputs(300, 72, 1001, torch.bfloat16, True, seed=20), _inputs(64, 512, 130, torch.bfloat16, True, seed=21)]
+    eager = [step(o) for o in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = [step(o) for o in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for e, o in zip(eager, other) for a, c in zip(e, o))
+    graphs, outs = [], []
+    for o in sets:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(step(o))
+        graphs.append(g)
+    for turn in range(3):
+        for k, o in enumerate(sets):
+            fresh = _inputs(o[0].shape[0], o[0].shape[1], o[1].shape[0], torch.bfloat16, True, seed=30 + turn)
+            for a, c in zip(o, fresh):
+                a.copy_(c)
+        for g in graphs:
+            g.replay()
+        for k, o in enumerate(sets):
+            want = step(o)
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, c) for a, c in zip(outs[k], want)), (turn, k)
+
+
+def test_a_training_run_of_all_of_them():
+    """Backbone features -> linear_cross_entropy under autocast and a loss scale -> clipped FusedSGD step, against torch's operators in double
+    precision on the rounded operands: the first step's gradients and update; then the loop runs, skips an overflow and goes on."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    from yolov6_amd.solver import FusedSGD, LossScaler, clip_grad_norm_, grad_norm
+    from yolov6_amd.train_engine import ParamArena
+    torch.manual_seed(0)
+    model = torch.nn.Sequential(torch.nn.Linear(32, 64), torch.nn.ReLU(), torch.nn.Linear(64, 500)).to(DEV)
+    ref = [p.detach().double().requires_grad_() for p in model.parameters()]
+    arena = ParamArena(model)
+    opt, scaler = FusedSGD(model, arena, lr=0.1, weight_decay=0.0), LossScaler(DEV, init_scale=1024.0)
+    x, t = torch.randn(96, 32, device=DEV), torch.randint(0, 500, (96,), device=DEV)
+    t[::5] = -100
+    head = model[2]
+
+    def step():
+        opt.zero_grad()
+        feats = torch.relu(model[0](x))
+        with torch.autocast("cuda", dtype=torch.float16):
+            loss = linear_cross_entropy(feats, head.weight, t, head.bias, label_smoothing=0.1)
+        scaler.scale_loss(loss).backward()
+        return loss.detach()
+
+    loss = step()
+    h = torch.relu(x.double() @ ref[0].t() + ref[1])
+    want = torch.nn.functional.cross_entropy(h.half().double() @ ref[2].half().double().t() + ref[3].half().double(), t, label_smoothing=0.1)
+    # (through the straight rounding of h and the head, the gradients are those of the unrounded graph up to fp16: 2^-11 a factor)
+    full = torch.nn.functional.cross_entropy(h @ ref[2].t() + ref[3], t, label_smoothing=0.1)
+    full.backward()
+    assert abs(float(loss) - float(want)) <= 1e-5 * float(want)
+    total = float(grad_norm([p.grad for p in model.parameters()])) / 1024
+    exact = float(torch.cat([r.grad.reshape(-1) for r in ref]).norm())
+    assert abs(total - exact) <= 8 * 2.0 ** -11 * exact
+    norm = opt.step(scaler, max_norm=0.5 * exact)
+    assert abs(float(norm) - total) <= 2.0 ** -20 * total
+    scaler.update()
+    for p, r in zip(model.parameters(), ref):
+        moved = -0.1 * (1 + 0.937) * 0.5 * r.grad
+        assert float((p.detach().double() - r.detach() - moved).norm()) <= 8 * 2.0 ** -11 * float(moved.norm()) + 2.0 ** -22 * float(r.detach().norm())
+    for _ in range(3):
+        step()
+        clip_grad_norm_(model.parameters(), 1.0)
+        opt.step(scaler, max_norm=1.0)
+        scaler.update()
+    before = arena.data.clone()
+    step()
+    arena.grad[3] = math.inf
+    opt.step(scaler, max_norm=1.0)
+    scaler.update()
+    assert torch.equal(before, arena.data) and float(scaler.scale) == 512.0
+    step()
+    opt.step(scaler, max_norm=1.0)
+    assert not torch.equal(before, arena.data) and bool(torch.isfinite(arena.data).all())

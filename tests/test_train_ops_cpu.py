@@ -5,14 +5,14 @@ import pytest
 import torch
 
 from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
-from yolov6_amd.solver import _is_dense, clip_grad_norm_, grad_norm
+from yolov6_amd.solver import clip_grad_norm_, grad_norm
 
 
 def _operands(n=4, d=8, v=5, dtype=torch.float32):
     return torch.zeros(n, d, dtype=dtype), torch.zeros(v, d, dtype=dtype), torch.zeros(n, dtype=torch.int64), torch.zeros(v, dtype=dtype)
 
 
-def test_linear_cross_entropy_refusals():
+def test_linear_cross_entropy_refusals(hip_lib):
     x, w, t, b = _operands()
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         linear_cross_entropy(x, w, t, b)
@@ -55,7 +55,7 @@ def test_native_refusals(hip_lib):
     assert hip_lib.y6_grad_norm(C.byref(lst), 4096, 1 << 20, 4096, None) == -1 and b"norm" in hip_lib.y6_last_error()
 
 
-def test_gradient_refusals():
+def test_gradient_refusals(hip_lib):
     p = torch.nn.Parameter(torch.zeros(4))
     p.grad = torch.zeros(4)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
@@ -70,8 +70,3 @@ def test_gradient_refusals():
         grad_norm([p.grad.double()])
     assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(4))], 1.0)) == 0.0
 
-
-def test_dense_layouts():
-    t = torch.zeros(4, 5, 6)
-    assert _is_dense(t) and _is_dense(t.permute(2, 0, 1)) and _is_dense(t[1:2].permute(0, 2, 1)) and _is_dense(torch.zeros(()))
-    assert not _is_dense(t[:, 1:]) and not _is_dense(t[:, :, 0]) and not _is_dense(torch.zeros(3, 1).expand(3, 4)) and not _is_dense(t[::2])

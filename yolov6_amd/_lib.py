@@ -408,6 +408,26 @@ SIGNATURES = {
 }
 
 _lib = None
+_torch_host = None
+TORCH_HOST_PATH = os.path.join(_HERE, "lib", "_y6_torch.so")
+
+
+def torch_host():
+    """The extension of csrc/torch_host.cpp (loaded once), calling the library that load() returns; RuntimeError if it has not been built."""
+    global _torch_host
+    if _torch_host is None:
+        lib = load()
+        if not os.path.exists(TORCH_HOST_PATH):
+            raise RuntimeError(f"yolov6_amd: {TORCH_HOST_PATH} is missing - build it with `python yolov6_amd/csrc/build.py`")
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("_y6_torch", TORCH_HOST_PATH)
+        ext = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(ext)
+        ext.bind([C.cast(getattr(lib, n), C.c_void_p).value for n in (
+            "y6_last_error", "y6_linear_ce_workspace_bytes", "y6_linear_ce_forward", "y6_linear_ce_backward", "y6_grad_norm_workspace_bytes",
+            "y6_grad_norm", "y6_grad_clip")])
+        _torch_host = ext
+    return _torch_host
 
 
 def load():

@@ -19,6 +19,7 @@ ROOT = os.path.dirname(os.path.dirname(HERE))
 OUT_DIR = os.path.join(os.path.dirname(HERE), "lib")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(OUT_DIR, "libyolov6_hip.so")
+TORCH_HOST = os.path.join(OUT_DIR, "_y6_torch.so")     # host code against torch's C++ API (csrc/torch_host.cpp); no kernels
 
 COMMON = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
           "-Wno-unused-variable", "-I" + os.path.join(ROOT, "include")]
@@ -82,6 +83,32 @@ def compile_one(cc, src, flags, force):
     return obj, True
 
 
+def build_torch_host(force=False, verbose=True):
+    """The Python extension of csrc/torch_host.cpp, with g++: host code only."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+    flags = ["-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    include = [sysconfig.get_paths()["include"], os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include")] + cpp_extension.include_paths()
+    libs = os.path.join(os.path.dirname(torch.__file__), "lib")
+    mark = os.path.join(OBJ_DIR, "_y6_torch.tag")
+    tag = digest(["torch_host.cpp", os.path.join(ROOT, "include", "yolov6_hip.h")], [flags, torch.__version__])
+    if not force and os.path.exists(TORCH_HOST) and os.path.exists(mark) and open(mark).read() == tag:
+        return TORCH_HOST
+    cmd = (["g++"] + flags + [a for i in dict.fromkeys(include) for a in ("-isystem", i)] +
+           [os.path.join(HERE, "torch_host.cpp"), "-o", TORCH_HOST, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"])
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed for torch_host.cpp:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    with open(mark, "w") as f:
+        f.write(tag)
+    if verbose:
+        print(f"[build] linked {TORCH_HOST}")
+    return TORCH_HOST
+
+
 def build(force=False, jobs=None, verbose=True):
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(OUT_DIR, exist_ok=True)
@@ -103,6 +130,7 @@ def build(force=False, jobs=None, verbose=True):
             raise RuntimeError(f"link failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
         if verbose:
             print(f"[build] linked {LIB}")
+    build_torch_host(force, verbose)
     # drop stale objects
     keep = set(objs)
     for f in os.listdir(OBJ_DIR):

@@ -36,19 +36,6 @@ def param_groups(model):
 
 
 _NORMS = {2.0: 0, 1.0: 1, math.inf: 2}
-_GRAD_TYPES = {torch.float16: _lib.Y6_F16, torch.bfloat16: _lib.Y6_BF16, torch.float32: _lib.Y6_F32}
-
-
-def _is_dense(t):
-    """Whether t's elements fill one run of memory, each place once, in whatever order."""
-    if t.is_contiguous():
-        return True
-    run = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != run:
-            return False
-        run *= size
-    return True
 
 
 def _norm_code(norm_type):
@@ -58,69 +45,25 @@ def _norm_code(norm_type):
     return code
 
 
-def _grad_list(grads, norm):
-    """The native call's view of `grads` and the tensors that have to outlive it."""
-    device = grads[0].device
-    for g in grads:
-        if g.layout != torch.strided or g.dtype not in _GRAD_TYPES:
-            raise RuntimeError(f"yolov6_amd: gradients must be dense fp16, bf16 or fp32 tensors (got {g.dtype}, {g.layout})")
-        if g.device != device:
-            raise RuntimeError(f"yolov6_amd: gradients on {device} and {g.device}: one norm is taken on one device")
-    _lib.require_gpu_tensor(grads[0], "gradients")
-    n = len(grads)
-    keep = ((C.c_void_p * n)(*[g.data_ptr() for g in grads]), (C.c_int64 * n)(*[g.numel() for g in grads]),
-            (C.c_int32 * n)(*[_GRAD_TYPES[g.dtype] for g in grads]))
-    return _lib.GradList(*keep, n, norm), keep
-
-
-def _call_on(grads, norm, call):
-    """call(lib, list, workspace, bytes, norm, stream) for dense `grads`; the norm as a device scalar."""
-    lst, keep = _grad_list(grads, norm)
-    with torch.cuda.device(grads[0].device):
-        lib = _lib.load()
-        ws = torch.empty(lib.y6_grad_norm_workspace_bytes(len(grads)), dtype=torch.uint8, device=grads[0].device)
-        out = torch.empty((), dtype=torch.float32, device=grads[0].device)
-        call(lib, C.byref(lst), C.c_void_p(ws.data_ptr()), ws.numel(), C.c_void_p(out.data_ptr()), _lib.current_stream_ptr())
-    return out
-
-
-@torch.no_grad()
 def grad_norm(grads, norm_type=2.0):
     """The norm (2, 1 or inf) of all elements of the tensors `grads` together, as an fp32 scalar on their device (no host
-    synchronisation).  Sums are doubles in a fixed order: the same gradients give the same bits.  NaN if any element is NaN."""
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-    code = _norm_code(norm_type)
-    if not grads:
-        return torch.tensor(0.0)
-    grads = [g if _is_dense(g) else g.contiguous() for g in grads]
-    return _call_on(grads, code, lambda lib, *a: _lib.check(lib.y6_grad_norm(*a), "grad_norm"))
+    synchronisation).  Sums are doubles in a fixed order: the same gradients give the same bits.  NaN if any element is NaN.  Any
+    strided layout; views with gaps are copied first."""
+    grads = [grads] if isinstance(grads, torch.Tensor) else grads
+    return _lib.torch_host().grad_norm(grads, _norm_code(norm_type))
 
 
-@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scale the gradients of `parameters` (a tensor or an iterable; those without `.grad` are left out, one that comes twice
     counts once) in place by min(1, max_norm / (norm + 1e-6)), norm = grad_norm of all of them; returns the norm before clipping.
-    The semantics of torch.nn.utils.clip_grad_norm_, in two launches whatever the number of tensors up to 160, without a host
-    synchronisation unless `error_if_nonfinite` asks for the check (then nothing has been scaled when it raises).  Under a
-    LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
+    The semantics of torch.nn.utils.clip_grad_norm_, in two launches for up to 160 tensors, without a host synchronisation unless
+    `error_if_nonfinite` asks for the check (then nothing has been scaled when it raises).  Gradients that share memory are
+    refused.  Under a LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
-    grads = [p.grad for p in {id(p): p for p in parameters}.values() if p.grad is not None]
-    code = _norm_code(norm_type)
-    max_norm = float(max_norm)
+    code, max_norm = _norm_code(norm_type), float(max_norm)
     if not max_norm >= 0:
         raise RuntimeError(f"yolov6_amd: max_norm {max_norm} is negative or not a number")
-    if not grads:
-        return torch.tensor(0.0)
-    if any(g.requires_grad for g in grads):
-        raise RuntimeError("yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place")
-    if error_if_nonfinite and not bool(torch.isfinite(grad_norm(grads, norm_type))):
-        raise RuntimeError(f"yolov6_amd: the norm of order {norm_type} of the gradients is not finite, so they cannot be clipped")
-    dense = [g if _is_dense(g) else g.contiguous() for g in grads]
-    norm = _call_on(dense, code, lambda lib, lst, *a: _lib.check(lib.y6_grad_clip(lst, max_norm, *a), "grad_clip"))
-    for g, d in zip(grads, dense):
-        if d is not g:
-            g.copy_(d)
-    return norm
+    return _lib.torch_host().clip_grad_norm(parameters, max_norm, code, bool(error_if_nonfinite))
 
 
 class LossScaler:

@@ -5,6 +5,7 @@
     labels, boxes, scores, fg = torch.ops.yolov6_hip.tal_assign(pd_scores, pd_bboxes, anc_points, gt_labels, gt_bboxes, mask_gt,
                                                                  13, 1.0, 6.0, 1e-9)
     y = torch.ops.yolov6_hip.conv2d_bias_act(x_nchw, weight, bias, "relu", 1)
+    loss, _ = torch.ops.yolov6_hip.linear_cross_entropy(features, weight, target, bias, -100, 0.0, "mean")      # differentiable
 
 Each op is a dispatcher-visible custom op (schema, CUDA-only implementation, fake / meta kernel for shape inference), so
 `torch.compile` traces THROUGH callers of them (they stay opaque calls into libyolov6_hip.so), `torch.ops.yolov6_hip.*` works from
@@ -23,7 +24,7 @@ import torch
 from torch import Tensor
 
 NAMESPACE = "yolov6_hip"
-__all__ = ["nms_batched", "tal_assign", "atss_assign", "conv2d_bias_act"]
+__all__ = ["nms_batched", "tal_assign", "atss_assign", "conv2d_bias_act", "linear_cross_entropy"]
 
 
 @torch.library.custom_op(f"{NAMESPACE}::nms_batched", mutates_args=(), device_types="cuda")
@@ -101,3 +102,44 @@ def _(x, weight, bias, act, stride):
     k = weight.shape[-1]
     Ho, Wo = (H + 2 * (k // 2) - k) // stride + 1, (W + 2 * (k // 2) - k) // stride + 1
     return x.new_empty((B, weight.shape[0], Ho, Wo))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy", mutates_args=(), device_types="cuda")
+def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], ignore_index: int, label_smoothing: float,
+                         reduction: str) -> Tuple[Tensor, Tensor]:
+    """(loss, log2 of each row's sum of exponentials [rows]; the latter for the backward only): models/losses/loss_ce.py with a schema."""
+    from . import _lib
+    return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction)
+
+
+@linear_cross_entropy.register_fake
+def _(features, weight, target, bias, ignore_index, label_smoothing, reduction):
+    return (features.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32),
+            features.new_empty((target.numel(),), dtype=torch.float32))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy_backward", mutates_args=(), device_types="cuda")
+def linear_cross_entropy_backward(grad: Tensor, features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], lse: Tensor,
+                                  ignore_index: int, label_smoothing: float, reduction: str) -> Tuple[Tensor, Tensor, Tensor]:
+    from . import _lib
+    return _lib.torch_host().linear_cross_entropy_backward(grad, features, weight, target, bias, lse, ignore_index, label_smoothing, reduction)
+
+
+@linear_cross_entropy_backward.register_fake
+def _(grad, features, weight, target, bias, lse, ignore_index, label_smoothing, reduction):
+    return (features.new_empty(features.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else (weight.shape[0],)))
+
+
+def _ce_setup(ctx, inputs, output):
+    features, weight, target, bias, *ctx.options = inputs
+    ctx.mark_non_differentiable(output[1])
+    ctx.save_for_backward(features, weight, target, bias, output[1])
+
+
+def _ce_grad(ctx, grad, _):
+    features, weight, target, bias, lse = ctx.saved_tensors
+    dx, dw, db = torch.ops.yolov6_hip.linear_cross_entropy_backward(grad, features, weight, target, bias, lse, *ctx.options)
+    return dx, dw, None, None if bias is None else db, None, None, None
+
+
+linear_cross_entropy.register_autograd(_ce_grad, setup_context=_ce_setup)
