@@ -812,8 +812,9 @@ int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
  * backward: gradients of x [rows][width], weight [classes][width] and bias [classes], dense, in their type; each may be NULL.
  * A label that is neither a class nor ignore_index makes the row's loss, and every gradient, NaN.  Rows with ignore_index are not
  * read and get zeros.  x: rows x_pitch elements apart (0: all rows the same); weight: w_pitch >= width.  All in one type.
- * lse [rows] (fp32): written by forward (may be NULL there) in units of log 2, read by backward with the same operands.
- * workspace: 16-byte aligned, y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls. */
+ * saved: y6_linear_ce_saved_bytes(d) that forward writes (the labelled rows gathered, their statistics; a weight of an unaligned
+ * width padded) and backward reads, with the same operands; NULL for a forward that no backward follows.
+ * workspace: y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls.  Both 16-byte aligned. */
 enum { Y6_REDUCE_NONE = 0, Y6_REDUCE_SUM = 1, Y6_REDUCE_MEAN = 2 };
 typedef struct y6_linear_ce_desc {
     const void* x;
@@ -825,7 +826,8 @@ typedef struct y6_linear_ce_desc {
     float smoothing;
     int32_t pad;
     float* loss;                   /* [rows] or one value */
-    float* lse;
+    void* saved;
+    size_t saved_bytes;
     const float* grad_out;         /* backward: d / d loss, as many as loss */
     void* dx;
     void* dw;
@@ -833,6 +835,7 @@ typedef struct y6_linear_ce_desc {
     void* workspace;
     size_t workspace_bytes;
 } y6_linear_ce_desc;
+size_t y6_linear_ce_saved_bytes(const y6_linear_ce_desc* d);
 size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int backward);
 int y6_linear_ce_forward(const y6_linear_ce_desc* d, void* stream);
 int y6_linear_ce_backward(const y6_linear_ce_desc* d, void* stream);

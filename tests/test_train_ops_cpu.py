@@ -34,10 +34,12 @@ def test_native_refusals(hip_lib):
     import ctypes as C
     from yolov6_amd import _lib
     d = _lib.LinearCeDesc()
-    d.x = d.weight = d.target = d.loss = d.lse = d.grad_out = d.dx = 4096
+    d.x = d.weight = d.target = d.loss = d.grad_out = d.dx = 4096
     d.rows, d.width, d.classes, d.x_pitch, d.w_pitch, d.reduction = 4, 8, 5, 8, 8, 2
     assert hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 0) > 0 and hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 1) > 0
     d.workspace, d.workspace_bytes = 4096, 16
+    assert hip_lib.y6_linear_ce_backward(C.byref(d), None) == -1 and b"null" in hip_lib.y6_last_error()
+    d.saved, d.saved_bytes = 4096, 1 << 20
     for call in (hip_lib.y6_linear_ce_forward, hip_lib.y6_linear_ce_backward):
         assert call(C.byref(d), None) == -1 and b"workspace" in hip_lib.y6_last_error()
     for field, value, what in (("dtype", 2, b"dtype"), ("rows", 0, b"rows"), ("classes", 0, b"classes"), ("width", 0, b"wide"), ("w_pitch", 7, b"pitch"),
@@ -47,6 +49,9 @@ def test_native_refusals(hip_lib):
         assert hip_lib.y6_linear_ce_forward(C.byref(d), None) == -1 and what in hip_lib.y6_last_error(), field
         assert hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 1) == 0
         setattr(d, field, keep)
+    d.workspace_bytes, d.saved_bytes = 1 << 20, 16
+    for call in (hip_lib.y6_linear_ce_forward, hip_lib.y6_linear_ce_backward):
+        assert call(C.byref(d), None) == -1 and b"saved" in hip_lib.y6_last_error()
     lst = _lib.GradList((C.c_void_p * 2)(4096, 4100), (C.c_int64 * 2)(8, 8), (C.c_int32 * 2)(1, 1), 2, 0)
     assert hip_lib.y6_grad_clip(C.byref(lst), 1.0, 4096, 1 << 20, 4096, None) == -1 and b"share memory" in hip_lib.y6_last_error()
     assert hip_lib.y6_grad_clip(C.byref(lst), -1.0, 4096, 1 << 20, 4096, None) == -1 and b"max_norm" in hip_lib.y6_last_error()

@@ -230,7 +230,7 @@ class LinearCeDesc(C.Structure):
     _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64),
                 ("x_pitch", C.c_int64), ("w_pitch", C.c_int64), ("ignore_index", C.c_int64), ("width", C.c_int32), ("classes", C.c_int32),
                 ("dtype", C.c_int32), ("reduction", C.c_int32), ("smoothing", C.c_float), ("pad", C.c_int32), ("loss", C.c_void_p),
-                ("lse", C.c_void_p), ("grad_out", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+                ("saved", C.c_void_p), ("saved_bytes", C.c_size_t), ("grad_out", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
@@ -344,6 +344,7 @@ SIGNATURES = {
                               C.c_void_p, C.c_void_p, C.c_void_p]),
     "y6_sgd_step_grouped": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_float),
                                       C.c_float, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "y6_linear_ce_saved_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc)]),
     "y6_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc), C.c_int]),
     "y6_linear_ce_forward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
     "y6_linear_ce_backward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
@@ -424,7 +425,7 @@ def torch_host():
         ext = importlib.util.module_from_spec(spec)
         spec.loader.exec_module(ext)
         ext.bind([C.cast(getattr(lib, n), C.c_void_p).value for n in (
-            "y6_last_error", "y6_linear_ce_workspace_bytes", "y6_linear_ce_forward", "y6_linear_ce_backward", "y6_grad_norm_workspace_bytes",
+            "y6_last_error", "y6_linear_ce_saved_bytes", "y6_linear_ce_workspace_bytes", "y6_linear_ce_forward", "y6_linear_ce_backward", "y6_grad_norm_workspace_bytes",
             "y6_grad_norm", "y6_grad_clip")])
         _torch_host = ext
     return _torch_host

@@ -14,6 +14,7 @@
 //
 // No atomics: partial statistics and split products are joined in a fixed order, the same inputs give the same bits.
 #include <atomic>
+#include <type_traits>
 
 #include "common.hpp"
 
@@ -75,14 +76,10 @@ struct GatherArgs {
     char* xc;
     long long cpitch;              // bytes
     int* rowmap;                   // place -> row
+    int* place;                    // row -> place, -1: no label
     int* label;                    // place -> label, -1: not a class
     int* count;
-    // forward
     float* loss_rows;              // 0 for rows without a label (reduction none), or null
-    // backward
-    const float* lse;              // by row
-    float* lsec;                   // by place
-    char* dx;                      // rows without a label: zeros
 };
 
 __device__ __forceinline__ int block_count(int mine, int* sh) {       // sum over the 256 threads
@@ -119,10 +116,10 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
         const unsigned long long m = __ballot(has);
         const int p = before + __popcll(m & ((1ull << threadIdx.x) - 1));
         if (threadIdx.x < kGatherRows) place[threadIdx.x] = has ? p : -1;
+        if (mine) a.place[r] = has ? p : -1;
         if (has) {
             a.rowmap[p] = r;
             a.label[p] = t >= 0 && t < a.classes ? (int)t : -1;
-            if (a.lsec) a.lsec[p] = a.lse[r];
         } else if (mine && a.loss_rows) {
             a.loss_rows[r] = 0.f;
         }
@@ -143,9 +140,6 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
                 for (int e = lane; e < a.cpitch / ES; e += 64)
                     reinterpret_cast<U*>(dst)[e] = e < a.width ? reinterpret_cast<const U*>(src)[e] : (U)0;
             }
-        } else if (a.dx) {
-            char* const dst = a.dx + (long long)(r0 + i) * a.width * ES;
-            for (int e = lane; e < a.width; e += 64) reinterpret_cast<U*>(dst)[e] = (U)0;
         }
     }
 }
@@ -273,7 +267,7 @@ __device__ __forceinline__ f32x16_t mma(const u32x4& a, const u32x4& b, f32x16_t
     }
 }
 
-enum { EPI_STATS, EPI_DZ, EPI_STORE };
+enum { EPI_STATS, EPI_DZ };
 enum { COUNT_NONE, COUNT_N, COUNT_K };
 
 struct GemmArgs {
@@ -292,13 +286,13 @@ struct GemmArgs {
     int class0;                    // first class of the piece
     char* dz;
     long long dz_pitch;            // bytes
-    // EPI_STORE: m = column, n = row of the output
+    // products into a gradient: m = column, n = row of the output
     float* part;                   // [split][N][part_pitch] or null: straight to out
     long long part_pitch;          // elements
     int add;                       // add to what the partial product holds
     char* out;
     long long out_pitch;           // elements
-    const int* rowmap;             // output row of row n, or null
+    const int *rowmap, *place;     // output row of row n, or null; rows of the output that no row n has get zeros
     const float *up, *gmax;        // the gradient's factor: *up [/ labelled rows], or *gmax
     int mean, vec;
 };
@@ -354,7 +348,7 @@ __device__ __forceinline__ void wait_requests() {       // all but the newest N 
 
 // One block's tile of a product; `bid` of `8 * ceil(tiles / 8)` blocks.  Block b runs on XCD b % 8: each XCD takes one run of tiles, in
 // groups of eight m-tiles by all n-tiles, so that the tiles it works on at one time share operand rows in its L2.
-template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+template <class E, bool AKC, bool BKC, class T, int COUNT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char* smem) {
     constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN;
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
@@ -373,6 +367,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char*
     const int tm = grp * 8 + in % gm, tn = in / gm;
     const int m0 = tm * BM, n0 = tn * BN;
     const int N = COUNT == COUNT_N ? *g.count : g.N, K = COUNT == COUNT_K ? *g.count : g.K;
+    if (COUNT == COUNT_N && !g.part && N < g.N) {        // dx of rows n0.. without a label: zeros
+        const int wide = g.M - m0 < BM ? g.M - m0 : BM;
+        for (int r = n0 + wave; r < n0 + BN && r < g.N; r += NW)
+            if (g.place[r] < 0)
+                for (int c = lane; c < wide; c += 64) reinterpret_cast<typename E::S*>(g.out)[(long long)r * g.out_pitch + m0 + c] = E::put(0.f);
+    }
     if (n0 >= N) return;
     const int steps = (K + OA::KS - 1) / OA::KS;
     const int s0 = (int)((long long)steps * split / g.splits), s1 = (int)((long long)steps * (split + 1) / g.splits);
@@ -422,163 +422,290 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char*
     // lane: row n = lane & 31 of a fragment; its 16 values are m = 8 (q >> 2) + 4 (lane >> 5) + (q & 3)
     const int half = lane >> 5, l31 = lane & 31;
     const int mw = m0 + wm * (BM / WM), nw = n0 + wn * (BN / WN);
-    typedef typename E::S S;
-    const bool whole = mw + BM / WM <= g.M;              // every class of this wave's tile is one
-    if constexpr (EPI == EPI_STATS || EPI == EPI_DZ) {
-        if (g.bias) {
-            const S* const bias = reinterpret_cast<const S*>(g.bias) + g.class0;
+    const float f = g.part ? 1.f : grad_factor<E>(g.up, g.gmax, g.mean, g.count);
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < FN; ++j) {
+        const int n = nw + j * 32 + l31;
+        if (n >= N) continue;
+        const long long row = !g.part && g.rowmap ? g.rowmap[n] : n;
 #pragma unroll
-                for (int q = 0; q < 16; ++q) {
-                    const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
-                    const float b = E::get(bias[m < g.M ? m : g.M - 1]);
+        for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
+            for (int gq = 0; gq < 4; ++gq) {
+                const int m = mw + i * 32 + 8 * gq + 4 * half;
+                if (m >= g.M) continue;
+                if (g.part) {
+                    f32x4_t* const p = reinterpret_cast<f32x4_t*>(g.part + ((long long)split * g.N + n) * g.part_pitch + m);
+                    f32x4_t v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e];
+                    if (g.add) v += *p;
+                    *p = v;
+                } else {
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e] * f;
+                    char* const dst = g.out + (row * g.out_pitch + m) * E::ES;
+                    if (g.vec) store4<E, true>(dst, v, g.M - m);
+                    else store4<E, false>(dst, v, g.M - m);
                 }
-        }
+            }
     }
-    if constexpr (EPI == EPI_STATS) {
+}
+
+// The arguments once more, loaded where the epilogue uses them: taken from the parameter itself they stay in registers through the loop
+// over the steps, and two dozen of them spill.
+__device__ __forceinline__ GemmArgs args_again() {
+    unsigned long long v = (unsigned long long)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(v));
+    const __attribute__((address_space(4))) unsigned* const src = reinterpret_cast<const __attribute__((address_space(4))) unsigned*>(v);
+    static_assert(sizeof(GemmArgs) % 4 == 0, "copied by dwords");
+    GemmArgs r;
+    unsigned* const dst = reinterpret_cast<unsigned*>(&r);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = nw + j * 32 + l31;
-            const bool live = n < N;
-            const long long o = (long long)(tm * WM + wm) * g.np + n;
-            const int left = g.M - mw - 4 * half;        // classes of this lane's 4-runs: 32 i + 8 (q >> 2) + (q & 3) < left
-            if (g.part_z) {
-                float zsum = 0.f;
+    for (unsigned i = 0; i < sizeof(GemmArgs) / 4; ++i) dst[i] = src[i];
+    return r;
+}
+
+// The scores' product: z = W x^T tile by tile, with the statistics (EPI_STATS) or dz (EPI_DZ) as its epilogue; m = class, n = labelled row.
+// A tile's reduction is short (the features' width: 16 steps at 1024), so what lies around it counts.  For dz a block stays and walks
+// its tiles as one sequence of steps, the first loads of the next tile in flight while the last step of this one is multiplied and its
+// dz stored: 16384 x 4096 x 1024 in 151 instead of 164 us.  (Keeping dz in registers to store it during the next tile spills, 203 us.)  The
+// statistics have little to store, and in the loop their masks spill: there a block takes one tile.
+template <class E, class T, int EPI>
+__global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(const GemmArgs g) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN;
+    constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
+    typedef Operand<E, true, BM, NW, T::KB> OA;
+    typedef Operand<E, true, BN, NW, T::KB> OB;
+    constexpr int kStage = OA::kBytes + OB::kBytes;
+    constexpr bool kPack = EPI == EPI_DZ && E::ES == 2;
+    constexpr bool kStay = EPI == EPI_DZ;
+    typedef typename E::S S;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int wm = wave % WM, wn = wave / WM;
+    const int half = lane >> 5, l31 = lane & 31;
+    const int N = *g.count, K = g.K;
+    // (XCDs and groups of tiles: gemm_tile)
+    const int total = g.tiles_m * g.tiles_n, per = (total + 7) >> 3;
+    const int base = (blockIdx.x & 7) * per, stride = gridDim.x >> 3;
+    const int end = base + per < total ? base + per : total;
+    const int width = 8 * g.tiles_n;
+    auto place = [&](int t, int& tm, int& tn) {
+        const int grp = t / width, in = t - grp * width;
+        const int gm = g.tiles_m - grp * 8 < 8 ? g.tiles_m - grp * 8 : 8;
+        tn = in / gm;
+        tm = grp * 8 + in - tn * gm;
+    };
+    auto next = [&](int t, int& tm, int& tn) {            // the block's first tile from t on that has rows; `end`: none
+        for (; t < end; t += stride) {
+            place(t, tm, tn);
+            if (tn * BN < N) return t;
+        }
+        return end;
+    };
+    const int steps = (K + OA::KS - 1) / OA::KS;
+    const unsigned lds0 = lds_addr(smem);
+    unsigned st_in = 0, st_out = 0;
+    int ptm = 0, ptn = 0, pt = next(base + (int)(blockIdx.x >> 3), ptm, ptn), ps = 0, ahead = 0;
+    int tm = ptm, tn = ptn, t = pt;
+    if (t >= end) return;
+    auto issue = [&]() {                                  // requests of the sequence's next step, if there is one
+        if (pt >= end) return;
+        const unsigned st = lds0 + st_in;
+        OA::issue(g.a, g.pa, ptm * BM, g.M, ps * OA::KS, K, st, wave, lane);
+        OB::issue(g.b, g.pb, ptn * BN, N, ps * OA::KS, K, st + OA::kBytes, wave, lane);
+        st_in = st_in + kStage == T::STAGES * kStage ? 0 : st_in + kStage;
+        ++ahead;
+        if (++ps == steps) {
+            ps = 0;
+            pt = kStay ? next(pt + stride, ptm, ptn) : end;
+        }
+    };
+    constexpr int kAhead = T::STAGES - 1;
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) issue();
+
+    while (t < end) {
+        f32x16_t acc[FM][FN];
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+        for (int s = 0; s < steps; ++s) {
+            // this step's stage has landed for every wave, and every wave has left the stage before, which the next requests overwrite
+            // (stores in between only make the count stricter)
+            if (kAhead > 1 && ahead == kAhead) wait_requests<(kAhead - 1) * (OA::kPer + OB::kPer)>();
+            else wait_requests<0>();
+            --ahead;
+            issue();
+            const char* const ia = smem + st_out;
+            const char* const ib = ia + OA::kBytes;
+            st_out = st_out + kStage == T::STAGES * kStage ? 0 : st_out + kStage;
+#pragma unroll
+            for (int kk = 0; kk < T::KB / 32; ++kk) {
+                u32x4 fa[FM], fb[FN];
+#pragma unroll
+                for (int i = 0; i < FM; ++i) fa[i] = OA::frag(ia, wm * (BM / WM) + i * 32, kk, lane);
+#pragma unroll
+                for (int j = 0; j < FN; ++j) fb[j] = OB::frag(ib, wn * (BN / WN) + j * 32, kk, lane);
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        if (whole || i * 32 + 8 * (q >> 2) + (q & 3) < left) zsum += acc[i][j][q];
-                zsum += __shfl_xor(zsum, 32);
-                if (live && half == 0) g.part_z[o] = zsum;
+                    for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[i], fb[j], acc[i][j]);
             }
-            if (!whole) {
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        if (i * 32 + 8 * (q >> 2) + (q & 3) >= left) acc[i][j][q] = -INFINITY;
-            }
-            float top = acc[0][j][0];
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
-            top = fmaxf(top, __shfl_xor(top, 32));
-            // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
-            const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
-            float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            all += __shfl_xor(all, 32);
-            if (live && half == 0) {
-                g.part_m[o] = top == -INFINITY ? -INFINITY : m2;
-                g.part_s[o] = all;
-            }
-            const int lab = live ? g.label[n] - mw : -1;
-            if (__ballot(lab >= 0 && lab < BM / WM)) {   // a label of these rows lies in this tile: few do
-                const int mine = lab - 4 * half;
-                float z = 0.f;
-                int hit = 0;
+        }
+        const GemmArgs e = args_again();
+        // lane: row n = lane & 31 of a fragment; its 16 values are m = 8 (q >> 2) + 4 (lane >> 5) + (q & 3)
+        const int mw = tm * BM + wm * (BM / WM), nw = tn * BN + wn * (BN / WN);
+        const bool whole = mw + BM / WM <= e.M;              // every class of this wave's tile is one
+        {
+            if (e.bias) {
+                const S* const bias = reinterpret_cast<const S*>(e.bias) + e.class0;
 #pragma unroll
                 for (int i = 0; i < FM; ++i)
 #pragma unroll
                     for (int q = 0; q < 16; ++q) {
-                        const bool is = mine == i * 32 + 8 * (q >> 2) + (q & 3);
-                        z = is ? acc[i][j][q] : z;
-                        hit = is ? 1 : hit;
+                        const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
+                        const float b = E::get(bias[m < e.M ? m : e.M - 1]);
+#pragma unroll
+                        for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
                     }
-                if (hit) g.zt[n] = z;
             }
         }
-    } else if constexpr (EPI == EPI_DZ) {
+        if constexpr (EPI == EPI_STATS) {
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = nw + j * 32 + l31;
-            if (n >= N) continue;
-            const float l2 = g.lsec[n];
-            const float c = (g.coef ? g.coef[n] : 1.f) * E::kScale;
-            const int lab = g.label[n] - g.class0 - mw - 4 * half;
-            char* const row = g.dz + (long long)n * g.dz_pitch + (long long)(mw + 4 * half) * E::ES;
-            const int left = g.M - mw - 4 * half;
-            const int room = (int)(g.dz_pitch / E::ES) - mw - 4 * half;
+            for (int j = 0; j < FN; ++j) {
+                const int n = nw + j * 32 + l31;
+                const bool live = n < N;
+                const long long o = (long long)(tm * WM + wm) * e.np + n;
+                int left = e.M - mw - 4 * half;              // classes of this lane's 4-runs: 32 i + 8 (q >> 2) + (q & 3) < left
+                if (e.part_z) {
+                    float zsum = 0.f;
 #pragma unroll
-            for (int i = 0; i < FM; ++i)
+                    for (int i = 0; i < FM; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int gp = 0; gp < 2; ++gp) {
-                    float v[2][4];
+                        for (int q = 0; q < 16; ++q)
+                            if (whole || i * 32 + 8 * (q >> 2) + (q & 3) < left) zsum += acc[i][j][q];
+                    }
+                    zsum += __shfl_xor(zsum, 32);
+                    if (live && half == 0) e.part_z[o] = zsum;
+                }
+                if (!whole) {
+                    asm volatile("" : "+v"(left));           // (or the compiler forms all masks of all columns ahead, and they spill)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                    for (int i = 0; i < FM; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int m = i * 32 + 16 * gp + 8 * k + e;
-                            float d = exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + e], kLog2e, -l2)) - g.smooth_share;
-                            d -= m == lab ? 1.f - g.smooth : 0.f;
-                            v[k][e] = d * c;
+                        for (int q = 0; q < 16; ++q)
+                            if (i * 32 + 8 * (q >> 2) + (q & 3) >= left) acc[i][j][q] = -INFINITY;
+                    }
+                }
+                float top = acc[0][j][0];
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
+                top = fmaxf(top, __shfl_xor(top, 32));
+                // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
+                const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
+                float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                all += __shfl_xor(all, 32);
+                if (live && half == 0) {
+                    e.part_m[o] = top == -INFINITY ? -INFINITY : m2;
+                    e.part_s[o] = all;
+                }
+                const int lab = live ? e.label[n] - mw : -1;
+                if (__ballot(lab >= 0 && lab < BM / WM)) {   // a label of these rows lies in this tile: few do
+                    int mine = lab - 4 * half;
+                    asm volatile("" : "+v"(mine));
+                    float z = 0.f;
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);   // (or all the comparisons come first, and their masks spill)
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) z = mine == i * 32 + 8 * (q >> 2) + (q & 3) ? acc[i][j][q] : z;
+                    }
+                    if (mine >= 0 && mine < BM / WM && (mine & 4) == 0) e.zt[n] = z;
+                }
+            }
+        } else if constexpr (EPI == EPI_DZ) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+                const int n = nw + j * 32 + l31;
+                const bool live = n < N;
+                const int nl = live ? n : N - 1;
+                const float l2 = e.lsec[nl];
+                const float c = (e.coef ? e.coef[nl] : 1.f) * E::kScale;
+                const float share = -e.smooth_share * c, hit = (1.f - e.smooth) * c;
+                const int lab = e.label[nl] - e.class0 - mw - 4 * half;
+                char* const row = e.dz + (long long)n * e.dz_pitch + (long long)(mw + 4 * half) * E::ES;
+                const int left = e.M - mw - 4 * half;
+                const int room = (int)(e.dz_pitch / E::ES) - mw - 4 * half;
+                auto emit = [&](auto labelled, auto inside) {
+                    int at = lab, to = left, end16 = room;
+                    asm volatile("" : "+v"(at), "+v"(to), "+v"(end16));   // (or the compiler forms every mask ahead of the branches, and they spill)
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int gp = 0; gp < 2; ++gp) {
+                            if (labelled.value) __builtin_amdgcn_sched_barrier(0);
+                            float v[2][4];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int c4 = 0; c4 < 4; ++c4) {
+                                    const int m = i * 32 + 16 * gp + 8 * k + c4;
+                                    float d = fmaf(exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + c4], kLog2e, -l2)), c, share);
+                                    if (labelled.value) d -= m == at ? hit : 0.f;
+                                    v[k][c4] = d;
+                                }
+                            if (inside.value && kPack) {
+                                // the half-waves trade runs of four classes: each lane then holds eight in a row, one 16-byte store
+                                const uint2 a = pack4<E>(v[0]), b = pack4<E>(v[1]);
+                                const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
+                                const auto y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
+                                if (live) *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * E::ES) = make_uint4(x[0], y[0], x[1], y[1]);
+                                continue;
+                            }
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const int m = i * 32 + 16 * gp + 8 * k;
+                                __builtin_amdgcn_sched_barrier(0);
+                                if (!live || m >= end16) continue;
+                                // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
+                                if (!inside.value) {
+#pragma unroll
+                                    for (int c4 = 0; c4 < 4; ++c4)
+                                        if (m + c4 >= to) v[k][c4] = 0.f;
+                                }
+                                store4<E, true>(row + m * E::ES, v[k], end16 - m);
+                            }
                         }
-                    if (whole && E::ES == 2) {
-                        // the half-waves trade runs of four classes: each lane then holds eight in a row, one 16-byte store
-                        const uint2 a = pack4<E>(v[0]), b = pack4<E>(v[1]);
-                        const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
-                        const auto y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
-                        *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * E::ES) = make_uint4(x[0], y[0], x[1], y[1]);
-                        continue;
-                    }
-#pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const int m = i * 32 + 16 * gp + 8 * k;
-                        if (m >= room) continue;
-                        // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            if (m + e >= left) v[k][e] = 0.f;
-                        store4<E, true>(row + m * E::ES, v[k], room - m);
-                    }
-                }
+                };
+                if (!whole) emit(std::true_type{}, std::false_type{});
+                else if (__ballot(lab >= -4 && lab < BM / WM)) emit(std::true_type{}, std::true_type{});   // a label of these rows lies in this tile: few do
+                else emit(std::false_type{}, std::true_type{});
+            }
         }
-    } else {
-        const float f = g.part ? 1.f : grad_factor<E>(g.up, g.gmax, g.mean, g.count);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) {
-            const int n = nw + j * 32 + l31;
-            if (n >= N) continue;
-            const long long row = !g.part && g.rowmap ? g.rowmap[n] : n;
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int gq = 0; gq < 4; ++gq) {
-                    const int m = mw + i * 32 + 8 * gq + 4 * half;
-                    if (m >= g.M) continue;
-                    if (g.part) {
-                        f32x4_t* const p = reinterpret_cast<f32x4_t*>(g.part + ((long long)split * g.N + n) * g.part_pitch + m);
-                        f32x4_t v;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e];
-                        if (g.add) v += *p;
-                        *p = v;
-                    } else {
-                        float v[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * gq + e] * f;
-                        char* const dst = g.out + (row * g.out_pitch + m) * E::ES;
-                        if (g.vec) store4<E, true>(dst, v, g.M - m);
-                        else store4<E, false>(dst, v, g.M - m);
-                    }
-                }
-        }
+        if (!kStay) break;
+        t = next(t + stride, tm, tn);
     }
 }
 
-template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+template <class E, bool AKC, bool BKC, class T, int COUNT>
 __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void gemm_kernel(const GemmArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
-    gemm_tile<E, AKC, BKC, T, EPI, COUNT>(g, blockIdx.x, smem);
+    gemm_tile<E, AKC, BKC, T, COUNT>(g, blockIdx.x, smem);
 }
 // dx and dW of a piece in one launch: neither has tiles enough to fill the chip evenly, together they do (way_of_grads)
 template <class E, class T>
@@ -586,8 +713,8 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void grads_kernel(c
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const unsigned wblocks = gridDim.x - xblocks;
     const bool is_x = x_first ? blockIdx.x < xblocks : blockIdx.x >= wblocks;
-    if (is_x) gemm_tile<E, false, true, T, EPI_STORE, COUNT_N>(x, x_first ? blockIdx.x : blockIdx.x - wblocks, smem);
-    else gemm_tile<E, false, false, T, EPI_STORE, COUNT_K>(w, x_first ? blockIdx.x - xblocks : blockIdx.x, smem);
+    if (is_x) gemm_tile<E, false, true, T, COUNT_N>(x, x_first ? blockIdx.x : blockIdx.x - wblocks, smem);
+    else gemm_tile<E, false, false, T, COUNT_K>(w, x_first ? blockIdx.x - xblocks : blockIdx.x, smem);
 }
 
 // ------------------------------------------------------------------------------------------------------------------- small kernels
@@ -599,9 +726,11 @@ struct FinishArgs {
     int parts, places;
     const int *rowmap, *label, *count;
     float smooth, smooth_share;
-    float* lse;                    // by row: log2 of the sum of exponentials, or null
+    float* lsec;                   // by place: log2 of the sum of exponentials
     float* rows_out;               // by row (reduction none) or null
-    float* lossc;                  // by place
+    float* lossc;                  // by place, unless this is the only block
+    float* loss;                   // the only block: the sum, or the mean
+    int mean;
 };
 __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     __shared__ float sm[1024], ss[1024], sz[1024];
@@ -630,16 +759,25 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
             sm[threadIdx.x] = m, ss[threadIdx.x] = s, sz[threadIdx.x] = z;
         }
     }
-    if (sl != 0 || n >= N) return;
-    // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
-    float l2 = (m == -INFINITY ? 0.f : m) + log2_fast(s);
-    float loss = l2 * kLn2 - (1.f - a.smooth) * a.zt[n];
-    if (a.smooth > 0.f) loss -= a.smooth_share * z;
-    if (a.label[n] < 0) l2 = loss = NAN;       // a label that is no class
-    const int row = a.rowmap[n];
-    if (a.lse) a.lse[row] = l2;
-    if (a.rows_out) a.rows_out[row] = loss;
-    if (a.lossc) a.lossc[n] = loss;
+    __syncthreads();
+    float loss = 0.f;
+    if (sl == 0 && n < N) {
+        // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
+        float l2 = (m == -INFINITY ? 0.f : m) + log2_fast(s);
+        loss = l2 * kLn2 - (1.f - a.smooth) * a.zt[n];
+        if (a.smooth > 0.f) loss -= a.smooth_share * z;
+        if (a.label[n] < 0) l2 = loss = NAN;   // a label that is no class
+        a.lsec[n] = l2;
+        if (a.rows_out) a.rows_out[a.rowmap[n]] = loss;
+        if (a.lossc) a.lossc[n] = loss;
+    }
+    if (!a.loss) return;
+    sm[threadIdx.x] = loss;
+    __syncthreads();
+    if (threadIdx.x) return;
+    double all = 0;
+    for (int k = 0; k < a.places; ++k) all += (double)sm[k];
+    *a.loss = (float)(a.mean ? all / (N > 1 ? N : 1) : all);
 }
 
 __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict__ lossc, const int* __restrict__ count, int mean, float* __restrict__ loss) {
@@ -686,25 +824,27 @@ struct JoinArgs {
     int rows, width, splits;
     char* out;
     long long out_pitch;               // elements
-    const int *rowmap, *count;
-    int count_rows;                    // rows: *count
+    const int *place, *count;          // dx: row -> row of part, -1: zeros; or null
     const float *up, *gmax;
     int mean, vec;
 };
 template <class E>
 __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
-    const int rows = a.count_rows ? *a.count : a.rows;
     const float f = grad_factor<E>(a.up, a.gmax, a.mean, a.count);
     const int q = (a.width + 3) >> 2;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * q; i += (long long)gridDim.x * 256) {
-        const int n = (int)(i / q), m = (int)(i - (long long)n * q) * 4;
-        f32x4_t s = *reinterpret_cast<const f32x4_t*>(a.part + (long long)n * a.part_pitch + m);
-        for (int k = 1; k < a.splits; ++k) s += *reinterpret_cast<const f32x4_t*>(a.part + ((long long)k * a.part_rows + n) * a.part_pitch + m);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)a.rows * q; i += (long long)gridDim.x * 256) {
+        const int row = (int)(i / q), m = (int)(i - (long long)row * q) * 4;
+        const int n = a.place ? a.place[row] : row;
+        f32x4_t s = {0.f, 0.f, 0.f, 0.f};
+        if (n >= 0) {
+            const float* const p = a.part + (long long)n * a.part_pitch + m;
+#pragma unroll 8
+            for (int k = 0; k < a.splits; ++k) s += *reinterpret_cast<const f32x4_t*>(p + (long long)k * a.part_rows * a.part_pitch);
+        }
         float v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = s[e] * f;
-        const long long row = a.rowmap ? a.rowmap[n] : n;
-        char* const dst = a.out + (row * a.out_pitch + m) * E::ES;
+        for (int e = 0; e < 4; ++e) v[e] = n >= 0 ? s[e] * f : 0.f;
+        char* const dst = a.out + ((long long)row * a.out_pitch + m) * E::ES;
         if (a.vec) store4<E, true>(dst, v, a.width - m);
         else store4<E, false>(dst, v, a.width - m);
     }
@@ -715,7 +855,8 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
 constexpr int kBiasRows = 64;          // shares at most
 template <class E>
 __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__ dz, long long pitch, int classes, const int* __restrict__ count,
-                                                        float* __restrict__ part) {
+                                                        float* __restrict__ part, typename E::S* __restrict__ db, const float* up, const float* gmax,
+                                                        int mean) {
     constexpr int V = 16 / E::ES;
     __shared__ float sh[8][32 * V + 1];
     const int N = *count, c = (blockIdx.x * 32 + (threadIdx.x & 31)) * V, w = threadIdx.x >> 5;
@@ -740,7 +881,9 @@ __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__
         float t = 0.f;
 #pragma unroll
         for (int k = 0; k < 8; ++k) t += sh[k][i];
-        if (col < classes) part[(long long)blockIdx.y * classes + col] = t;
+        if (col >= classes) continue;
+        if (db) db[col] = E::put(t * grad_factor<E>(up, gmax, mean, count));       // the only share
+        else part[(long long)blockIdx.y * classes + col] = t;
     }
 }
 template <class E>
@@ -749,6 +892,7 @@ __global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict_
     const int c = blockIdx.x * 256 + threadIdx.x;
     if (c >= classes) return;
     float s = 0.f;
+#pragma unroll 16
     for (int k = 0; k < shares; ++k) s += part[(long long)k * classes + c];
     db[c] = E::put(s * grad_factor<E>(up, gmax, mean, count));
 }
@@ -758,22 +902,22 @@ int type_bytes(int t) { return t == Y6_F32 ? 4 : 2; }
 long long up_to(long long v, long long m) { return (v + m - 1) / m * m; }
 int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
-// ---- tiles.  kBig: eight waves of 128 x 64 (dx, dW) - 8192 x 8192 x 2048 bf16 at 1.20 PFLOP/s, 128 x 128 tiles reach 1.04 - one
-// block per CU.  kMid: four waves of 64 x 64, two blocks per CU: 2.5 times the blocks for what kBig leaves unfilled.  kSmall: 64 x 64 with
-// three stages in flight: 64 rows x 1000 classes x 512 in 6.0 us against kMid's 9.1, one row x 32000 classes x 1024 in 12.4 against 15.2.
-typedef Tile<256, 256, 2, 4, 128, 2, 1> BigScores;     // stats, dz: a lane's row has 64 classes per fragment column (2 x 4: 1.04, 4 x 2: 0.99 PFLOP/s)
-typedef Tile<256, 256, 4, 2, 128, 2, 1> BigGrads;      // dx, dW (4 x 2: 1.20, 2 x 4: 1.15 PFLOP/s)
-typedef Tile<128, 128, 2, 2, 128, 2, 2> Mid;
+// ---- tiles.  kBig: 256 x 256, eight waves, one block per CU.  kMid: 128 x 128, four waves, two blocks per CU: a quarter of the tile for
+// what kBig leaves unfilled, and its epilogue hides behind the other block.  kSmall: 64 x 64 with three stages in flight: 64 rows x 1000 classes x
+// 512 in 6.0 us against kMid's 9.1, one row x 32000 classes x 1024 in 12.1 against 14.8.
+typedef Tile<256, 256, 2, 4, 128, 2, 1> BigScores;     // waves 2 x 4: a lane's row has 128 classes (32000 x 4096 x 1024 statistics 262 us, 4 x 2: 300)
+typedef Tile<256, 256, 4, 2, 128, 2, 1> BigGrads;      // dx, dW: 4 x 2: 1.20 PFLOP/s, 2 x 4: 1.15 (8192 x 8192 x 2048)
+typedef Tile<128, 128, 2, 2, 128, 2, 2> Mid;           // dx, dW 1.04 PFLOP/s; the same statistics 280 us
 typedef Tile<64, 64, 2, 2, 128, 4, 2> Small;
 enum { kBig, kMid, kSmall, kTiles };
 constexpr int kSide[kTiles] = {256, 128, 64};
 constexpr int kSlots[kTiles] = {256, 512, 512};
 constexpr int kWavesM[kTiles] = {BigScores::WM, Mid::WM, Small::WM};
 // microseconds of one 128-byte step of a block, alone on its CU and beside another, and of its first loads and its epilogue (measured,
-// bf16; fp32 steps hold half the values at a sixteenth of the rate)
-constexpr double kStepAlone[2][kTiles] = {{1.9, 0.75, 0.38}, {1e9, 2.0, 0.6}};
-constexpr double kStepFull[2][kTiles] = {{1.9, 1.06, 0.45}, {1e9, 3.9, 1.0}};
-constexpr double kEnds[kTiles] = {7.0, 4.0, 2.0};
+// bf16; fp32 steps hold half the values at a sixteenth of the rate, and kBig is no faster than kMid there)
+constexpr double kStepAlone[2][kTiles] = {{1.85, 0.75, 0.38}, {1e9, 2.0, 0.6}};
+constexpr double kStepFull[2][kTiles] = {{1.85, 1.05, 0.5}, {1e9, 3.9, 1.0}};
+constexpr double kEnds[kTiles] = {4.0, 2.0, 1.5};
 constexpr double kBytesPerUs = 4e6;
 
 double block_us(int tile, bool fp32, long long steps, long long blocks) {
@@ -824,12 +968,13 @@ GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long widt
     return best;
 }
 
-struct Layout {                        // offsets into the workspace
-    size_t xc, wc, rowmap, label, count, seg, part_m, part_s, part_z, zt, lossc;      // forward (seg, xc .. count: both)
-    size_t lsec, coef, gmax, dz, accx, accw, bpart;                                   // backward
+struct Layout {
+    size_t xc, wc, rowmap, place, label, count, lsec, kept;                           // what the backward takes over from the forward
+    size_t seg, part_m, part_s, part_z, zt, lossc;                                    // forward's workspace
+    size_t coef, gmax, dz, accx, accw, bpart;                                         // backward's
     size_t bytes;
     long long cpitch, np;              // bytes; rows
-    int scores, parts, piece, pieces, shares;
+    int scores, parts, places, piece, pieces, shares;
     GradWay grads;
     long long px, pw;
     bool pad_w;
@@ -852,13 +997,21 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.xc = take((size_t)n * L.cpitch);
     L.wc = take(L.pad_w ? (size_t)v * L.cpitch : 0);
     L.rowmap = take((size_t)n * 4);
+    L.place = take((size_t)n * 4);
     L.label = take((size_t)n * 4);
+    L.lsec = take((size_t)n * 4);
     L.count = take(4);
-    L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
+    L.kept = at;
+    at = 0;
     const long long steps = ceil_div(w * es, kRowBytes);
     if (!backward) {
+        L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
         L.scores = way_of_scores(fp32, v, n, steps);
         L.parts = ceil_div(v, kSide[L.scores]) * kWavesM[L.scores];
+        // one block for all rows, which then also adds up the loss, where that is 16 rounds of its threads at most
+        L.places = 1;
+        while (L.places < n && L.places < 128) L.places *= 2;
+        if (L.places < n || (long long)L.places * L.parts > 16 * 1024) L.places = n >= 1024 ? 32 : n >= 64 ? 8 : 1;
         L.part_m = take((size_t)L.parts * L.np * 4);
         L.part_s = take((size_t)L.parts * L.np * 4);
         L.part_z = take(d->smoothing > 0.f ? (size_t)L.parts * L.np * 4 : 0);
@@ -874,8 +1027,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.scores = way_of_scores(fp32, piece, n, steps);
         L.grads = way_of_grads(fp32, d->dx != nullptr, d->dw != nullptr, n, w, piece, L.pieces);
         L.px = L.pw = up_to(w, 4);
-        L.shares = n < kBiasRows * 32 ? ceil_div(n, 32) : kBiasRows;
-        L.lsec = take((size_t)n * 4);
+        L.shares = n <= 256 ? 1 : n < kBiasRows * 64 ? ceil_div(n, 64) : kBiasRows;
         L.coef = take((size_t)n * 4);
         L.gmax = take(4);
         L.dz = take((size_t)n * up_to(piece * es, 16));
@@ -905,39 +1057,36 @@ int check_desc(const y6_linear_ce_desc* d, const char* what) {
 struct Run {
     const y6_linear_ce_desc* d;
     const Layout& L;
-    char* ws;
+    char *keep, *ws;
     hipStream_t s;
+    template <class T>
+    T* kept(size_t o) const { return reinterpret_cast<T*>(keep + o); }
     template <class T>
     T* at(size_t o) const { return reinterpret_cast<T*>(ws + o); }
 };
 
 template <class E>
-int launch_gather(const Run& r, bool backward) {
+int launch_gather(const Run& r) {
     const y6_linear_ce_desc* d = r.d;
     GatherArgs a = {};
     a.x = (const char*)d->x, a.pitch = d->x_pitch * E::ES, a.target = d->target, a.ignore = d->ignore_index;
     a.rows = (int)d->rows, a.width = d->width, a.classes = d->classes;
     a.vec = (d->width * E::ES) % 16 == 0 && a.pitch % 16 == 0 && (uintptr_t)d->x % 16 == 0;
-    a.xc = r.at<char>(r.L.xc), a.cpitch = r.L.cpitch;
-    a.rowmap = r.at<int>(r.L.rowmap), a.label = r.at<int>(r.L.label), a.count = r.at<int>(r.L.count);
+    a.xc = r.kept<char>(r.L.xc), a.cpitch = r.L.cpitch;
+    a.rowmap = r.kept<int>(r.L.rowmap), a.place = r.kept<int>(r.L.place), a.label = r.kept<int>(r.L.label), a.count = r.kept<int>(r.L.count);
     const int segs = ceil_div(d->rows, kGatherRows);
     if (d->rows > kCountRows) {
         a.seg = r.at<int>(r.L.seg);
         hipLaunchKernelGGL(count_kernel, dim3(ceil_div(d->rows, 256)), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs);
         Y6_LAUNCH_CHECK();
     }
-    if (backward) {
-        a.lse = d->lse, a.lsec = r.at<float>(r.L.lsec);
-        a.dx = (char*)d->dx;
-    } else if (d->reduction == Y6_REDUCE_NONE) {
-        a.loss_rows = d->loss;
-    }
+    if (d->reduction == Y6_REDUCE_NONE) a.loss_rows = d->loss;
     hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(256), 0, r.s, a);
     Y6_LAUNCH_CHECK();
     if (r.L.pad_w) {
         const int blocks = ceil_div(d->classes, 4);
         hipLaunchKernelGGL(pad_kernel<E::ES>, dim3(blocks < 4096 ? blocks : 4096), dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes,
-                           d->width, r.at<char>(r.L.wc), r.L.cpitch);
+                           d->width, r.kept<char>(r.L.wc), r.L.cpitch);
         Y6_LAUNCH_CHECK();
     }
     return Y6_OK;
@@ -963,10 +1112,10 @@ int set_tiles(GemmArgs& g, unsigned* blocks) {
     *blocks = (unsigned)((total + 7) / 8 * 8);
     return Y6_OK;
 }
-template <class E, bool AKC, bool BKC, class T, int EPI, int COUNT>
+template <class E, bool AKC, bool BKC, class T, int COUNT>
 int launch_tile(GemmArgs& g, hipStream_t s) {
     static std::atomic<unsigned long long> raised{0};
-    auto* const kern = gemm_kernel<E, AKC, BKC, T, EPI, COUNT>;
+    auto* const kern = gemm_kernel<E, AKC, BKC, T, COUNT>;
     unsigned blocks = 0;
     int rc = set_tiles<T>(g, &blocks);
     if (rc == Y6_OK) rc = raise_lds((const void*)kern, T::kLds, raised);
@@ -975,18 +1124,31 @@ int launch_tile(GemmArgs& g, hipStream_t s) {
     Y6_LAUNCH_CHECK();
     return Y6_OK;
 }
+template <class E, class T, int EPI>
+int launch_scores_tile(GemmArgs& g, hipStream_t s) {
+    static std::atomic<unsigned long long> raised{0};
+    auto* const kern = scores_kernel<E, T, EPI>;
+    unsigned blocks = 0;
+    int rc = set_tiles<T>(g, &blocks);
+    if (rc == Y6_OK) rc = raise_lds((const void*)kern, T::kLds, raised);
+    if (rc != Y6_OK) return rc;
+    if (EPI == EPI_DZ && blocks > 256u * T::BPC) blocks = 256u * T::BPC;
+    hipLaunchKernelGGL(kern, dim3(blocks), dim3(T::NW * 64), T::kLds, s, g);
+    Y6_LAUNCH_CHECK();
+    return Y6_OK;
+}
 template <class E, int EPI>
 int launch_scores(int tile, GemmArgs& g, hipStream_t s) {
-    if (tile == kSmall) return launch_tile<E, true, true, Small, EPI, COUNT_N>(g, s);
+    if (tile == kSmall) return launch_scores_tile<E, Small, EPI>(g, s);
     if constexpr (E::ES == 2) {
-        if (tile == kBig) return launch_tile<E, true, true, BigScores, EPI, COUNT_N>(g, s);
+        if (tile == kBig) return launch_scores_tile<E, BigScores, EPI>(g, s);
     }
-    return launch_tile<E, true, true, Mid, EPI, COUNT_N>(g, s);
+    return launch_scores_tile<E, Mid, EPI>(g, s);
 }
 template <class E, class T>
 int launch_grads_tile(GemmArgs* x, GemmArgs* w, hipStream_t s) {
-    if (!w) return launch_tile<E, false, true, T, EPI_STORE, COUNT_N>(*x, s);
-    if (!x) return launch_tile<E, false, false, T, EPI_STORE, COUNT_K>(*w, s);
+    if (!w) return launch_tile<E, false, true, T, COUNT_N>(*x, s);
+    if (!x) return launch_tile<E, false, false, T, COUNT_K>(*w, s);
     static std::atomic<unsigned long long> raised{0};
     auto* const kern = grads_kernel<E, T>;
     unsigned bx = 0, bw = 0;
@@ -1017,28 +1179,29 @@ template <class E>
 int forward(const Run& r) {
     const y6_linear_ce_desc* d = r.d;
     const Layout& L = r.L;
-    Y6_TRY(launch_gather<E>(r, false));
+    Y6_TRY(launch_gather<E>(r));
     GemmArgs g = {};
-    g.a = L.pad_w ? r.at<char>(L.wc) : (const char*)d->weight;
+    g.a = L.pad_w ? r.kept<char>(L.wc) : (const char*)d->weight;
     g.pa = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
-    g.b = r.at<char>(L.xc), g.pb = L.cpitch;
+    g.b = r.kept<char>(L.xc), g.pb = L.cpitch;
     g.M = d->classes, g.N = (int)d->rows, g.K = d->width;
-    g.count = r.at<int>(L.count), g.label = r.at<int>(L.label), g.bias = d->bias;
+    g.count = r.kept<int>(L.count), g.label = r.kept<int>(L.label), g.bias = d->bias;
     g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
     g.zt = r.at<float>(L.zt), g.np = L.np;
     Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
     FinishArgs f = {};
-    f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.zt = g.zt, f.np = L.np, f.parts = L.parts;
-    f.places = d->rows >= 1024 ? 32 : d->rows >= 64 ? 8 : 1;
-    f.rowmap = r.at<int>(L.rowmap), f.label = g.label, f.count = g.count;
+    f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.zt = g.zt, f.np = L.np, f.parts = L.parts, f.places = L.places;
+    f.rowmap = r.kept<int>(L.rowmap), f.label = g.label, f.count = g.count;
     f.smooth = d->smoothing, f.smooth_share = d->smoothing / d->classes;
-    f.lse = d->lse;
+    f.lsec = r.kept<float>(L.lsec), f.mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
+    const int blocks = ceil_div(d->rows, L.places);
     if (d->reduction == Y6_REDUCE_NONE) f.rows_out = d->loss;
+    else if (blocks == 1) f.loss = d->loss;
     else f.lossc = r.at<float>(L.lossc);
-    hipLaunchKernelGGL(finish_kernel, dim3(ceil_div(d->rows, f.places)), dim3(1024), 0, r.s, f);
+    hipLaunchKernelGGL(finish_kernel, dim3(blocks), dim3(1024), 0, r.s, f);
     Y6_LAUNCH_CHECK();
-    if (d->reduction != Y6_REDUCE_NONE) {
-        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, f.lossc, f.count, d->reduction == Y6_REDUCE_MEAN ? 1 : 0, d->loss);
+    if (f.lossc) {
+        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, f.lossc, f.count, f.mean, d->loss);
         Y6_LAUNCH_CHECK();
     }
     return Y6_OK;
@@ -1048,17 +1211,16 @@ template <class E>
 int backward(const Run& r) {
     const y6_linear_ce_desc* d = r.d;
     const Layout& L = r.L;
-    Y6_TRY(launch_gather<E>(r, true));
-    const int* const count = r.at<int>(L.count);
-    const int* const rowmap = r.at<int>(L.rowmap);
+    const int* const count = r.kept<int>(L.count);
+    const int* const place = r.kept<int>(L.place);
     const float *gmax = nullptr, *coef = nullptr;
     if (d->reduction == Y6_REDUCE_NONE) {
-        hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, r.s, d->grad_out, rowmap, count, r.at<float>(L.coef), r.at<float>(L.gmax));
+        hipLaunchKernelGGL(coef_kernel, dim3(1), dim3(1024), 0, r.s, d->grad_out, r.kept<int>(L.rowmap), count, r.at<float>(L.coef), r.at<float>(L.gmax));
         Y6_LAUNCH_CHECK();
         gmax = r.at<float>(L.gmax), coef = r.at<float>(L.coef);
     }
     const int mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
-    const char* const w = L.pad_w ? r.at<char>(L.wc) : (const char*)d->weight;
+    const char* const w = L.pad_w ? r.kept<char>(L.wc) : (const char*)d->weight;
     const long long wp = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
     char* const dz = r.at<char>(L.dz);
     const bool accx = L.pieces > 1 || L.grads.split_x > 1;
@@ -1066,19 +1228,23 @@ int backward(const Run& r) {
     for (int p = 0; p < L.pieces; ++p) {
         const int v0 = p * L.piece, vn = d->classes - v0 < L.piece ? d->classes - v0 : L.piece;
         GemmArgs g = {};
-        g.a = w + v0 * wp, g.pa = wp, g.b = r.at<char>(L.xc), g.pb = L.cpitch;
+        g.a = w + v0 * wp, g.pa = wp, g.b = r.kept<char>(L.xc), g.pb = L.cpitch;
         g.M = vn, g.N = (int)d->rows, g.K = d->width, g.count = count;
-        g.label = r.at<int>(L.label), g.bias = d->bias, g.class0 = v0;
-        g.lsec = r.at<float>(L.lsec), g.coef = coef;
+        g.label = r.kept<int>(L.label), g.bias = d->bias, g.class0 = v0;
+        g.lsec = r.kept<float>(L.lsec), g.coef = coef;
         g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
         g.dz = dz, g.dz_pitch = up_to((long long)vn * E::ES, 16);
         Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
         if (d->dbias) {
-            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 32 * (16 / E::ES)), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count, r.at<float>(L.bpart));
+            auto* const db = (typename E::S*)d->dbias + v0;
+            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 32 * (16 / E::ES)), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count,
+                               r.at<float>(L.bpart), L.shares == 1 ? db : nullptr, d->grad_out, gmax, mean);
             Y6_LAUNCH_CHECK();
-            hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), L.shares, vn,
-                               (typename E::S*)d->dbias + v0, d->grad_out, gmax, mean, count);
-            Y6_LAUNCH_CHECK();
+            if (L.shares > 1) {
+                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), L.shares, vn, db, d->grad_out, gmax,
+                                   mean, count);
+                Y6_LAUNCH_CHECK();
+            }
         }
         GemmArgs x = {}, y = {};
         x.a = w + v0 * wp, x.pa = wp, x.b = dz, x.pb = g.dz_pitch;
@@ -1087,10 +1253,10 @@ int backward(const Run& r) {
         if (accx) {
             x.part = r.at<float>(L.accx), x.part_pitch = L.px, x.add = p > 0;
         } else {
-            x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = rowmap;
+            x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = r.kept<int>(L.rowmap), x.place = place;
             x.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
         }
-        y.a = r.at<char>(L.xc), y.pa = L.cpitch, y.b = dz, y.pb = g.dz_pitch;
+        y.a = r.kept<char>(L.xc), y.pa = L.cpitch, y.b = dz, y.pb = g.dz_pitch;
         y.M = d->width, y.N = vn, y.K = (int)d->rows, y.count = count, y.splits = split_w;
         y.up = d->grad_out, y.gmax = gmax, y.mean = mean;
         char* const dw = (char*)d->dw + (long long)v0 * d->width * E::ES;
@@ -1110,7 +1276,7 @@ int backward(const Run& r) {
     if (d->dx && accx) {
         JoinArgs j = {};
         j.part = r.at<float>(L.accx), j.part_pitch = L.px, j.part_rows = d->rows, j.rows = (int)d->rows, j.width = d->width, j.splits = split_x;
-        j.out = (char*)d->dx, j.out_pitch = d->width, j.rowmap = rowmap, j.count = count, j.count_rows = 1;
+        j.out = (char*)d->dx, j.out_pitch = d->width, j.place = place, j.count = count;
         j.up = d->grad_out, j.gmax = gmax, j.mean = mean;
         j.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
         const long long need = (d->rows * ((d->width + 3) / 4) + 255) / 256;
@@ -1123,28 +1289,41 @@ int backward(const Run& r) {
 }  // namespace
 
 // ====================================================================== C ABI
+extern "C" size_t y6_linear_ce_saved_bytes(const y6_linear_ce_desc* d) {
+    if (check_desc(d, "linear_ce_saved_bytes") != Y6_OK) return 0;
+    return layout(d, false).kept;
+}
+
 extern "C" size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int backward_pass) {
     if (check_desc(d, "linear_ce_workspace_bytes") != Y6_OK) return 0;
-    return layout(d, backward_pass != 0).bytes;
+    const Layout L = layout(d, backward_pass != 0);
+    return L.bytes + (backward_pass || d->saved ? 0 : L.kept);
+}
+
+static int check_buffers(const y6_linear_ce_desc* d, const Layout& L, size_t need, const char* what) {
+    Y6_REQUIRE(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "%s: workspace of %zu bytes, %zu needed", what,
+               d->workspace_bytes, need);
+    Y6_REQUIRE(!d->saved || (d->saved_bytes >= L.kept && (uintptr_t)d->saved % 16 == 0), "%s: saved holds %zu bytes, %zu needed", what, d->saved_bytes, L.kept);
+    return Y6_OK;
 }
 
 extern "C" int y6_linear_ce_forward(const y6_linear_ce_desc* d, void* stream) {
     Y6_CLEAR_STALE_ERROR();
     Y6_TRY(check_desc(d, "linear_ce_forward"));
-    Y6_REQUIRE(d->loss && d->workspace, "linear_ce_forward: null argument");
+    Y6_REQUIRE(d->loss, "linear_ce_forward: null argument");
     const Layout L = layout(d, false);
-    Y6_REQUIRE(d->workspace_bytes >= L.bytes && (uintptr_t)d->workspace % 16 == 0, "linear_ce_forward: workspace of %zu bytes, %zu needed", d->workspace_bytes, L.bytes);
-    const Run r = {d, L, (char*)d->workspace, (hipStream_t)stream};
+    Y6_TRY(check_buffers(d, L, L.bytes + (d->saved ? 0 : L.kept), "linear_ce_forward"));
+    const Run r = {d, L, d->saved ? (char*)d->saved : (char*)d->workspace + L.bytes, (char*)d->workspace, (hipStream_t)stream};
     return d->dtype == Y6_F16 ? forward<Half>(r) : d->dtype == Y6_BF16 ? forward<Brain>(r) : forward<Single>(r);
 }
 
 extern "C" int y6_linear_ce_backward(const y6_linear_ce_desc* d, void* stream) {
     Y6_CLEAR_STALE_ERROR();
     Y6_TRY(check_desc(d, "linear_ce_backward"));
-    Y6_REQUIRE(d->lse && d->grad_out && d->workspace, "linear_ce_backward: null argument");
+    Y6_REQUIRE(d->saved && d->grad_out, "linear_ce_backward: null argument");
     if (!d->dx && !d->dw && !d->dbias) return Y6_OK;
     const Layout L = layout(d, true);
-    Y6_REQUIRE(d->workspace_bytes >= L.bytes && (uintptr_t)d->workspace % 16 == 0, "linear_ce_backward: workspace of %zu bytes, %zu needed", d->workspace_bytes, L.bytes);
-    const Run r = {d, L, (char*)d->workspace, (hipStream_t)stream};
+    Y6_TRY(check_buffers(d, L, L.bytes, "linear_ce_backward"));
+    const Run r = {d, L, (char*)d->saved, (char*)d->workspace, (hipStream_t)stream};
     return d->dtype == Y6_F16 ? backward<Half>(r) : d->dtype == Y6_BF16 ? backward<Brain>(r) : backward<Single>(r);
 }

@@ -30,6 +30,7 @@ using torch::autograd::variable_list;
 
 struct Library {
     decltype(&y6_last_error) last_error;
+    decltype(&y6_linear_ce_saved_bytes) ce_saved;
     decltype(&y6_linear_ce_workspace_bytes) ce_workspace;
     decltype(&y6_linear_ce_forward) ce_forward;
     decltype(&y6_linear_ce_backward) ce_backward;
@@ -66,28 +67,30 @@ y6_linear_ce_desc describe(const Tensor& x, const Tensor& w, const Tensor& b, co
     return d;
 }
 
-std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Options& o, bool want_lse) {
+std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Options& o, bool want_saved) {
     const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
     const int64_t n = x.size(0);
     const bool rows = o.reduction == Y6_REDUCE_NONE;
-    if (n == 0) return {rows ? at::empty({0}, f32) : at::zeros({}, f32), at::empty({0}, f32)};
+    if (n == 0) return {rows ? at::empty({0}, f32) : at::zeros({}, f32), bytes_on(x, 0)};
     const c10::DeviceGuard guard(x.device());
-    Tensor loss = rows ? at::empty({n}, f32) : at::empty({}, f32), lse;
+    Tensor loss = rows ? at::empty({n}, f32) : at::empty({}, f32), saved;
     y6_linear_ce_desc d = describe(x, w, b, t, o);
     d.loss = loss.data_ptr<float>();
-    if (want_lse) {
-        lse = at::empty({n}, f32);
-        d.lse = lse.data_ptr<float>();
+    if (want_saved) {
+        d.saved_bytes = lib.ce_saved(&d);
+        if (d.saved_bytes == 0) check(Y6_EINVAL, "linear_ce_forward");
+        saved = bytes_on(x, d.saved_bytes);
+        d.saved = saved.data_ptr();
     }
     d.workspace_bytes = lib.ce_workspace(&d, 0);
     if (d.workspace_bytes == 0) check(Y6_EINVAL, "linear_ce_forward");
     const Tensor ws = bytes_on(x, d.workspace_bytes);
     d.workspace = ws.data_ptr();
     check(lib.ce_forward(&d, stream_of(x.device())), "linear_ce_forward");
-    return {loss, lse};
+    return {loss, saved};
 }
 
-std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Tensor& lse,
+std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Tensor& saved,
                                                const Options& o, bool want_x, bool want_w, bool want_b) {
     want_b = want_b && b.defined();
     const auto like = x.options().requires_grad(false);
@@ -102,7 +105,7 @@ std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor&
     if (!want_x && !want_w && !want_b) return {dx, dw, db};
     const Tensor g = grad.detach().to(at::kFloat).contiguous();
     y6_linear_ce_desc d = describe(x, w, b, t, o);
-    d.lse = lse.data_ptr<float>(), d.grad_out = g.data_ptr<float>();
+    d.saved = saved.data_ptr(), d.saved_bytes = (size_t)saved.numel(), d.grad_out = g.data_ptr<float>();
     d.dx = want_x ? dx.data_ptr() : nullptr, d.dw = want_w ? dw.data_ptr() : nullptr, d.dbias = want_b ? db.data_ptr() : nullptr;
     d.workspace_bytes = lib.ce_workspace(&d, 1);
     if (d.workspace_bytes == 0) check(Y6_EINVAL, "linear_ce_backward");
@@ -117,8 +120,8 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
                           double smoothing, int64_t reduction) {
         const Tensor b = bias.has_value() ? *bias : Tensor();
         const Options o = {ignore, smoothing, reduction};
-        auto [loss, lse] = ce_forward(x, w, b, t, o, true);
-        ctx->save_for_backward({x, w, b, t, lse});
+        auto [loss, saved] = ce_forward(x, w, b, t, o, true);
+        ctx->save_for_backward({x, w, b, t, saved});
         ctx->saved_data["ignore"] = ignore;
         ctx->saved_data["smoothing"] = smoothing;
         ctx->saved_data["reduction"] = reduction;
@@ -280,23 +283,23 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
 
 PYBIND11_MODULE(_y6_torch, m) {
     m.def("bind", [](const std::vector<uintptr_t>& f) {
-        TORCH_CHECK(f.size() == 7, "seven entry points");
-        lib = {(decltype(lib.last_error))f[0], (decltype(lib.ce_workspace))f[1], (decltype(lib.ce_forward))f[2], (decltype(lib.ce_backward))f[3],
-               (decltype(lib.norm_workspace))f[4], (decltype(lib.norm))f[5], (decltype(lib.clip))f[6]};
+        TORCH_CHECK(f.size() == 8, "eight entry points");
+        lib = {(decltype(lib.last_error))f[0], (decltype(lib.ce_saved))f[1], (decltype(lib.ce_workspace))f[2], (decltype(lib.ce_forward))f[3],
+               (decltype(lib.ce_backward))f[4], (decltype(lib.norm_workspace))f[5], (decltype(lib.norm))f[6], (decltype(lib.clip))f[7]};
     });
     m.def("linear_cross_entropy", &linear_cross_entropy);
     m.def("linear_cross_entropy_forward", [](const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, int64_t ignore, double smoothing,
                                              const std::string& reduction) {
         const at::NoGradGuard off;
         const Operands p = operands(x, w, t, b, ignore, smoothing, reduction);
-        auto [loss, lse] = ce_forward(p.x, p.w, p.b, p.t, p.o, true);
-        return std::make_tuple(p.o.reduction == Y6_REDUCE_NONE ? loss.reshape(t.sizes()) : loss, lse);
+        auto [loss, saved] = ce_forward(p.x, p.w, p.b, p.t, p.o, true);
+        return std::make_tuple(p.o.reduction == Y6_REDUCE_NONE ? loss.reshape(t.sizes()) : loss, saved);
     });
-    m.def("linear_cross_entropy_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, const Tensor& lse,
+    m.def("linear_cross_entropy_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, const Tensor& saved,
                                               int64_t ignore, double smoothing, const std::string& reduction) {
         const at::NoGradGuard off;
         const Operands p = operands(x, w, t, b, ignore, smoothing, reduction);
-        auto [dx, dw, db] = ce_backward(grad.reshape({-1}), p.x, p.w, p.b, p.t, lse, p.o, true, true, p.b.defined());
+        auto [dx, dw, db] = ce_backward(grad.reshape({-1}), p.x, p.w, p.b, p.t, saved, p.o, true, true, p.b.defined());
         return std::make_tuple(dx.reshape(x.sizes()), dw, p.b.defined() ? db : at::empty({0}, dw.options()));
     });
     m.def("grad_norm", &grad_norm);

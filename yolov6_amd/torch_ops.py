@@ -107,7 +107,7 @@ def _(x, weight, bias, act, stride):
 @torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy", mutates_args=(), device_types="cuda")
 def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], ignore_index: int, label_smoothing: float,
                          reduction: str) -> Tuple[Tensor, Tensor]:
-    """(loss, log2 of each row's sum of exponentials [rows]; the latter for the backward only): models/losses/loss_ce.py with a schema."""
+    """(loss, bytes that the backward takes over): models/losses/loss_ce.py with a schema."""
     from . import _lib
     return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction)
 
@@ -115,18 +115,18 @@ def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias:
 @linear_cross_entropy.register_fake
 def _(features, weight, target, bias, ignore_index, label_smoothing, reduction):
     return (features.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32),
-            features.new_empty((target.numel(),), dtype=torch.float32))
+            features.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy_backward", mutates_args=(), device_types="cuda")
-def linear_cross_entropy_backward(grad: Tensor, features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], lse: Tensor,
+def linear_cross_entropy_backward(grad: Tensor, features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], saved: Tensor,
                                   ignore_index: int, label_smoothing: float, reduction: str) -> Tuple[Tensor, Tensor, Tensor]:
     from . import _lib
-    return _lib.torch_host().linear_cross_entropy_backward(grad, features, weight, target, bias, lse, ignore_index, label_smoothing, reduction)
+    return _lib.torch_host().linear_cross_entropy_backward(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction)
 
 
 @linear_cross_entropy_backward.register_fake
-def _(grad, features, weight, target, bias, lse, ignore_index, label_smoothing, reduction):
+def _(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction):
     return (features.new_empty(features.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else (weight.shape[0],)))
 
 
@@ -137,8 +137,8 @@ def _ce_setup(ctx, inputs, output):
 
 
 def _ce_grad(ctx, grad, _):
-    features, weight, target, bias, lse = ctx.saved_tensors
-    dx, dw, db = torch.ops.yolov6_hip.linear_cross_entropy_backward(grad, features, weight, target, bias, lse, *ctx.options)
+    features, weight, target, bias, saved = ctx.saved_tensors
+    dx, dw, db = torch.ops.yolov6_hip.linear_cross_entropy_backward(grad, features, weight, target, bias, saved, *ctx.options)
     return dx, dw, None, None if bias is None else db, None, None, None
 
 
