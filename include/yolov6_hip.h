@@ -864,7 +864,8 @@ int y6_scaler_update(float* scale, int32_t* found_inf, int32_t* growth_tracker, 
  *   c = min(1, max_norm / (norm + 1e-6));  every gradient *= c, one rounding to its type, nothing written when c is 1
  * A NaN gradient gives a NaN norm and NaN gradients, an infinite one norm = inf and c = 0.  The list's arrays are HOST arrays read
  * before the call returns; tensors are dense (any order of their elements), fp16 / bf16 / fp32 mixed, aligned to their elements.
- * y6_grad_clip refuses lists whose tensors overlap.  norm: one device float.  workspace: y6_grad_norm_workspace_bytes(count). */
+ * y6_grad_clip refuses lists whose tensors overlap.  norm: one device float.  workspace:
+ * y6_grad_norm_workspace_bytes(count, elements of all tensors). */
 enum { Y6_NORM_L2 = 0, Y6_NORM_L1 = 1, Y6_NORM_INF = 2 };
 typedef struct y6_grad_list {
     void* const* grads_host;
@@ -873,13 +874,13 @@ typedef struct y6_grad_list {
     int32_t count;
     int32_t norm_type;
 } y6_grad_list;
-size_t y6_grad_norm_workspace_bytes(int count);
+size_t y6_grad_norm_workspace_bytes(int count, int64_t elements);
 int y6_grad_norm(const y6_grad_list* l, void* workspace, size_t workspace_bytes, float* norm, void* stream);
 int y6_grad_clip(const y6_grad_list* l, double max_norm, void* workspace, size_t workspace_bytes, float* norm, void* stream);
 /* y6_sgd_step_grouped with the gradients clipped inside the update (they are not written): norm = |grad_mul / *scale| * ||grad||,
  * every gradient multiplied by min(1, max_norm / (norm + 1e-6)).  found_inf (NULL: none): set to 1 when a gradient is inf / nan -
  * no y6_grad_finite_check needed - and then, or when it was set before, nothing is updated.  norm: one device float or NULL.
- * param, grad, momentum_buf aligned to 16 bytes, group to 4.  workspace: y6_grad_norm_workspace_bytes(1). */
+ * param, grad, momentum_buf aligned to 16 bytes, group to 4.  workspace: y6_grad_norm_workspace_bytes(1, n). */
 int y6_sgd_step_clipped(float* param, const float* grad, float* momentum_buf, const uint8_t* group, size_t n, const float* lr3_host,
                         const float* wd3_host, float momentum, int nesterov, int first_step, float grad_mul, const float* scale,
                         int32_t* found_inf, double max_norm, void* workspace, size_t workspace_bytes, float* norm, void* stream);

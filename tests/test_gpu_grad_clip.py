@@ -248,3 +248,21 @@ def test_clipped_step_skips_on_overflow(bad):
     scaler.found_inf.fill_(1)                                       # another check's flag counts too
     opt.step(scaler, max_norm=1.0)
     assert torch.equal(arena.data, data)
+
+
+def test_a_gradient_of_more_than_2_to_the_30_elements():
+    """Several entries of one tensor, offsets past 32 bits: constant values, so that the sums are known."""
+    n = (1 << 31) + 5
+    g = torch.full((n,), 0.5, dtype=torch.bfloat16, device=DEV)
+    g[-1] = 4.0
+    want = math.sqrt(0.25 * (n - 1) + 16.0)
+    assert abs(float(grad_norm([g])) - want) <= 2.0 ** -23 * want
+    norm = clip_grad_norm_(_params([g[3:]]), 1.0)
+    want = math.sqrt(0.25 * (n - 4) + 16.0)
+    assert abs(float(norm) - want) <= 2.0 ** -23 * want
+    small = torch.tensor(0.5 / want, dtype=torch.float64).to(torch.bfloat16)
+    assert bool((g[:3] == 0.5).all())
+    for lo in range(3, n - 1, 1 << 28):
+        part = g[lo:min(lo + (1 << 28), n - 1)]
+        assert float((part.float() - float(small)).abs().max()) <= 2.0 ** -8 * float(small)
+    assert abs(float(g[-1]) - 4.0 / want) <= 2.0 ** -8 * 4.0 / want

@@ -364,3 +364,64 @@ def test_a_training_run_of_all_of_them():
     step()
     opt.step(scaler, max_norm=1.0)
     assert not torch.equal(before, arena.data) and bool(torch.isfinite(arena.data).all())
+
+
+def test_rows_in_pieces():
+    """More rows than one piece of the tiles' statistics holds (256 MB)."""
+    n, d, v = 131072 + 300, 16, 33000
+    x, w, b, t = _inputs(n, d, v, torch.bfloat16, True, seed=11, ignored=0.0)
+    t[-300:] = -100
+    t[77] = -100
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    leaves = [o.detach().requires_grad_() for o in (x, w, b)]
+    rows = linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], reduction="none")
+    up = torch.zeros(n, device=DEV)
+    pick = torch.tensor([0, 5, 77, 65535, 65536, 100000, 130000, 131071, 131072 + 5], device=DEV)
+    up[pick] = 1.0
+    grads = torch.autograd.grad(rows, leaves, up)
+    total = linear_cross_entropy(x, w, t, b, reduction="sum")
+    err = _logit_error(x, w, b)
+    want = torch.cat([torch.nn.functional.cross_entropy(x[k:k + 8192].double() @ w.double().t() + b.double(), t[k:k + 8192], reduction="none")
+                      for k in range(0, n, 8192)])
+    assert float((rows.detach().double() - want).abs().max()) <= 2 * err
+    assert abs(float(total) - float(want.sum())) <= 2 * err * n
+    # rows whose upstream gradient is 0 add nothing: the gradients are those of the picked rows alone
+    _, exact, spread, soft = _oracle(x[pick], w, b, t[pick], up[pick], reduction="none")
+    u = torch.finfo(torch.bfloat16).eps / 2
+    others = torch.ones(n, dtype=torch.bool, device=DEV)
+    others[pick] = False
+    assert int(grads[0][others].count_nonzero()) == 0
+    for got, ex, sp, so in zip((grads[0][pick], grads[1], grads[2]), exact, spread, soft):
+        assert bool(((got.double() - ex).abs() <= 1.01 * (u * sp + u * ex.abs() + 2 * err * so + v * 2.0 ** -24 * sp + 2.0 ** -19 * so + 2.0 ** -100)).all())
+
+
+def test_a_weight_beyond_4_gigabytes():
+    """Offsets past 32 bits in the weight and its gradient."""
+    n, d, v = 5, 16384, 140001
+    g = torch.Generator(device=DEV).manual_seed(0)
+    w = torch.empty((v, d), dtype=torch.bfloat16, device=DEV)
+    for k in range(0, v, 10000):
+        w[k:k + 10000] = torch.randn((min(10000, v - k), d), generator=g, device=DEV) / 128
+    x = torch.randn((n, d), generator=g, device=DEV).bfloat16().requires_grad_()
+    t = torch.tensor([0, 70000, 131072, v - 1, -100], device=DEV)
+    w.requires_grad_()
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    loss = linear_cross_entropy(x, w, t, reduction="sum")
+    dx, dw = torch.autograd.grad(loss, [x, w])
+    z = torch.cat([x.detach().double() @ w.detach()[k:k + 10000].double().t() for k in range(0, v, 10000)], 1)[:4]
+    lse = torch.logsumexp(z, 1)
+    err = _logit_error(x.detach(), w.detach()[:1000], None) * 1.5
+    assert abs(float(loss) - float((lse - z[torch.arange(4), t[:4]]).sum())) <= 8 * err
+    dz = torch.exp(z - lse[:, None])
+    dz[torch.arange(4), t[:4]] -= 1
+    u = torch.finfo(torch.bfloat16).eps / 2
+    want = torch.zeros((4, d), dtype=torch.float64, device=DEV)
+    spread = torch.zeros_like(want)
+    for k in range(0, v, 10000):
+        part, xs = dz[:, k:k + 10000], x.detach()[:4].double()
+        ex, sp = part.t() @ xs, part.abs().t() @ xs.abs()
+        assert bool(((dw[k:k + 10000].double() - ex).abs() <= 1.01 * (u * sp + u * ex.abs() + 2 * err * sp + 2.0 ** -120)).all()), k
+        want += part @ w.detach()[k:k + 10000].double()
+        spread += part.abs() @ w.detach()[k:k + 10000].double().abs()
+    assert bool(((dx[:4].double() - want).abs() <= 1.01 * (u * spread + u * want.abs() + 2 * err * spread + v * 2.0 ** -24 * spread)).all())
+    assert int(dx[4].count_nonzero()) == 0

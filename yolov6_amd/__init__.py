@@ -26,6 +26,12 @@ def __getattr__(name):
     if name == "TaskAlignedAssigner":
         from .assigners import TaskAlignedAssigner
         return TaskAlignedAssigner
+    if name == "linear_cross_entropy":
+        from .models.losses.loss_ce import linear_cross_entropy
+        return linear_cross_entropy
+    if name in ("clip_grad_norm_", "grad_norm"):
+        from . import solver
+        return getattr(solver, name)
     raise AttributeError(name)
 
 

@@ -348,7 +348,7 @@ SIGNATURES = {
     "y6_linear_ce_workspace_bytes": (C.c_size_t, [C.POINTER(LinearCeDesc), C.c_int]),
     "y6_linear_ce_forward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
     "y6_linear_ce_backward": (C.c_int, [C.POINTER(LinearCeDesc), C.c_void_p]),
-    "y6_grad_norm_workspace_bytes": (C.c_size_t, [C.c_int]),
+    "y6_grad_norm_workspace_bytes": (C.c_size_t, [C.c_int, C.c_int64]),
     "y6_grad_norm": (C.c_int, [C.POINTER(GradList), C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
     "y6_grad_clip": (C.c_int, [C.POINTER(GradList), C.c_double, C.c_void_p, C.c_size_t, C.c_void_p, C.c_void_p]),
     "y6_sgd_step_clipped": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_float), C.POINTER(C.c_float),

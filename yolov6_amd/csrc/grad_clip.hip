@@ -20,21 +20,39 @@
 
 namespace {
 
-constexpr int kTable = 160;            // tensors per launch: the table rides in the kernel's arguments (no upload, safe to capture)
+constexpr int kTable = 330;            // entries per launch: the table rides in the kernel's arguments (no upload, safe to capture)
 constexpr int kThreads = 256;
 constexpr int kChunk = 16384;          // bytes a block takes of one tensor at a time: four 16-byte loads in flight per thread
 constexpr int kBlocks = 1024;          // four blocks per CU: 64 KB of loads in flight on each
 constexpr int kJoin = 4096;            // partial sums that every block adds by itself; more are added by one block in between
+constexpr long long kEntry = 1ll << 30;                // elements of one entry; a larger tensor is several
 
+// 12 bytes an entry, 4 KB in all: 489 gradients (YOLOv6-L) are two launches of each kernel, not four
 struct Table {
-    char* base[kTable];                // the tensor's address rounded down to 16 bytes
-    unsigned long long end[kTable];    // byte behind the last element, from base; the first element lies at (address - base)
-    unsigned first[kTable + 1];        // chunks in front of the tensor
-    unsigned char head[kTable];        // address - base
-    unsigned char type[kTable];
+    unsigned long long at[kTable];     // the address, its type in the upper two bits
+    unsigned n[kTable];                // elements
     int count;
 };
 static_assert(sizeof(Table) <= 4000, "kernel arguments");
+
+// An entry as the loads see it: its address rounded down to 16 bytes, the first and the last byte from there
+struct Entry {
+    char* base;
+    unsigned head, type;
+    unsigned long long end;
+};
+__host__ __device__ __forceinline__ Entry entry(unsigned long long at, unsigned n) {
+    Entry e;
+    e.type = (unsigned)(at >> 62);
+    const unsigned long long p = at & ((1ull << 62) - 1);
+    e.head = (unsigned)(p & 15);
+    e.base = (char*)(p - e.head);
+    e.end = e.head + (unsigned long long)n * (e.type == Y6_F32 ? 4 : 2);
+    return e;
+}
+__host__ __device__ __forceinline__ unsigned chunks_of(unsigned long long at, unsigned n) {
+    return (unsigned)((entry(at, n).end + kChunk - 1) / kChunk);
+}
 
 union Vec {
     uint4 v;
@@ -168,24 +186,40 @@ __device__ __forceinline__ void chunk_scale(char* base, unsigned long long at, u
     }
 }
 
-// The block's share of the launch's chunks is one contiguous run; f(tensor, byte offset of the chunk) for each.
+// The block's share of the launch's chunks is one contiguous run; f(entry, byte offset of the chunk) for each.  Every block adds up the
+// entries' chunks for itself (two entries a thread).
 template <class F>
 __device__ __forceinline__ void for_chunks(const Table& tb, F f) {
-    __shared__ unsigned first[kTable + 1];
-    for (int i = threadIdx.x; i <= tb.count; i += kThreads) first[i] = tb.first[i];
+    static_assert(kTable <= 2 * kThreads, "two entries a thread");
+    __shared__ unsigned first[2 * kThreads + 1], wave_sum[kThreads / 64];
+    const int i = threadIdx.x * 2, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const unsigned c0 = i < tb.count ? chunks_of(tb.at[i], tb.n[i]) : 0, c1 = i + 1 < tb.count ? chunks_of(tb.at[i + 1], tb.n[i + 1]) : 0;
+    unsigned sum = c0 + c1;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const unsigned v = __shfl_up(sum, d);
+        if (lane >= d) sum += v;
+    }
+    if (lane == 63) wave_sum[wave] = sum;
     __syncthreads();
-    const unsigned total = first[tb.count];
+    for (int w = 0; w < wave; ++w) sum += wave_sum[w];
+    first[i + 1] = sum - c1;
+    first[i + 2] = sum;
+    if (threadIdx.x == 0) first[0] = 0;
+    __syncthreads();
+    const unsigned total = first[2 * kThreads];
     unsigned c = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x);
-    const unsigned c1 = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
+    const unsigned end = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
     int lo = 0, hi = tb.count;         // first[lo] <= c < first[hi]
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
         if (first[mid] <= c) lo = mid;
         else hi = mid;
     }
-    for (; c < c1; ++c) {
+    for (; c < end; ++c) {
         while (c >= first[lo + 1]) ++lo;
-        f(__builtin_amdgcn_readfirstlane(lo), (unsigned long long)(c - first[lo]) * kChunk);
+        const int t = __builtin_amdgcn_readfirstlane(lo);
+        f(entry(tb.at[t], tb.n[t]), (unsigned long long)(c - first[lo]) * kChunk);
     }
 }
 
@@ -193,13 +227,10 @@ template <int NORM>
 __global__ __launch_bounds__(kThreads) void grad_part_kernel(const Table tb, double* __restrict__ parts) {
     __shared__ double sh[kThreads / 64];
     double a = 0;
-    for_chunks(tb, [&](int t, unsigned long long at) {
-        const char* const base = tb.base[t];
-        const unsigned head = tb.head[t];
-        const unsigned long long end = tb.end[t];
-        a = join<NORM>(a, tb.type[t] == Y6_F32   ? chunk_part<NORM, Y6_F32>(base, at, head, end)
-                          : tb.type[t] == Y6_F16 ? chunk_part<NORM, Y6_F16>(base, at, head, end)
-                                                 : chunk_part<NORM, Y6_BF16>(base, at, head, end));
+    for_chunks(tb, [&](const Entry& e, unsigned long long at) {
+        a = join<NORM>(a, e.type == Y6_F32   ? chunk_part<NORM, Y6_F32>(e.base, at, e.head, e.end)
+                          : e.type == Y6_F16 ? chunk_part<NORM, Y6_F16>(e.base, at, e.head, e.end)
+                                             : chunk_part<NORM, Y6_BF16>(e.base, at, e.head, e.end));
     });
     a = block_join<NORM>(a, sh);
     if (threadIdx.x == 0) parts[blockIdx.x] = a;
@@ -221,13 +252,10 @@ __global__ __launch_bounds__(kThreads) void grad_scale_kernel(const Table tb, in
     if (out && blockIdx.x == 0 && threadIdx.x == 0) *out = (float)v;
     const float c = clip_factor(v, max_norm);
     if (c == 1.f) return;              // nothing to clip: x * 1 is x, bit for bit
-    for_chunks(tb, [&](int t, unsigned long long at) {
-        char* const base = tb.base[t];
-        const unsigned head = tb.head[t];
-        const unsigned long long end = tb.end[t];
-        if (tb.type[t] == Y6_F32) chunk_scale<Y6_F32>(base, at, head, end, c);
-        else if (tb.type[t] == Y6_F16) chunk_scale<Y6_F16>(base, at, head, end, c);
-        else chunk_scale<Y6_BF16>(base, at, head, end, c);
+    for_chunks(tb, [&](const Entry& e, unsigned long long at) {
+        if (e.type == Y6_F32) chunk_scale<Y6_F32>(e.base, at, e.head, e.end, c);
+        else if (e.type == Y6_F16) chunk_scale<Y6_F16>(e.base, at, e.head, e.end, c);
+        else chunk_scale<Y6_BF16>(e.base, at, e.head, e.end, c);
     });
 }
 
@@ -313,40 +341,39 @@ int check_list(const y6_grad_list* l, const char* what) {
     for (int i = 0; i < l->count; ++i) {
         const int t = l->dtypes_host[i];
         Y6_REQUIRE(t == Y6_F32 || t == Y6_F16 || t == Y6_BF16, "%s: tensor %d has dtype %d (fp16, bf16 or fp32)", what, i, t);
-        Y6_REQUIRE(l->numels_host[i] >= 0 && l->numels_host[i] < (1ll << 40), "%s: tensor %d has %lld elements", what, i, (long long)l->numels_host[i]);
+        Y6_REQUIRE((uintptr_t)l->grads_host[i] >> 62 == 0 && l->numels_host[i] >= 0 && l->numels_host[i] < (1ll << 40), "%s: tensor %d has %lld elements", what, i, (long long)l->numels_host[i]);
         Y6_REQUIRE(l->numels_host[i] == 0 || l->grads_host[i], "%s: tensor %d is null", what, i);
         Y6_REQUIRE((uintptr_t)l->grads_host[i] % elem_bytes(t) == 0, "%s: tensor %d is not aligned to its elements", what, i);
     }
     return Y6_OK;
 }
 
-// the next tensors of the list from `i` on (empty ones left out); returns where to go on
-int fill_table(const y6_grad_list* l, int i, Table& tb) {
+// The next entries of the list from element `from` of tensor `i` on (empty tensors left out); moves i and from.  Returns the chunks.
+unsigned fill_table(const y6_grad_list* l, int& i, long long& from, Table& tb) {
     unsigned long long chunks = 0;
-    tb.count = 0;
-    tb.first[0] = 0;
-    for (; i < l->count && tb.count < kTable; ++i) {
-        if (l->numels_host[i] == 0) continue;
-        const int k = tb.count;
-        const uintptr_t p = (uintptr_t)l->grads_host[i];
-        const unsigned head = (unsigned)(p & 15);
-        const unsigned long long end = head + (unsigned long long)l->numels_host[i] * elem_bytes(l->dtypes_host[i]);
-        const unsigned long long c = (end + kChunk - 1) / kChunk;
-        if (chunks + c > 0x7fffffffull) break;      // (check_list: one tensor has at most 2^28 + 1 chunks)
-        tb.base[k] = (char*)(p - head);
-        tb.end[k] = end;
-        tb.head[k] = (unsigned char)head;
-        tb.type[k] = (unsigned char)l->dtypes_host[i];
-        chunks += c;
-        tb.first[k + 1] = (unsigned)chunks;
+    for (tb.count = 0; i < l->count && tb.count < kTable;) {
+        const long long left = l->numels_host[i] - from;
+        if (left <= 0) {
+            ++i, from = 0;
+            continue;
+        }
+        const int type = l->dtypes_host[i];
+        const unsigned n = (unsigned)(left < kEntry ? left : kEntry);
+        const unsigned long long at = ((unsigned long long)(uintptr_t)l->grads_host[i] + (unsigned long long)from * elem_bytes(type)) | (unsigned long long)type << 62;
+        tb.at[tb.count] = at;          // (the types are 0, 1 and 3)
+        tb.n[tb.count] = n;
         ++tb.count;
+        chunks += chunks_of(at, n);
+        from += n;
     }
-    return i;
+    return (unsigned)chunks;           // 330 entries of at most 2^18 + 1
 }
-int table_blocks(const Table& tb) { return tb.first[tb.count] < (unsigned)kBlocks ? (int)tb.first[tb.count] : kBlocks; }
+int table_blocks(unsigned chunks) { return chunks < (unsigned)kBlocks ? (int)chunks : kBlocks; }
+// tables of a list of so many tensors and elements, at most
+size_t tables_for(size_t tensors, unsigned long long elements) { return (tensors + elements / kEntry) / kTable + 1; }
 
-int launch_part(int norm, const Table& tb, double* parts, hipStream_t s) {
-    const dim3 g(table_blocks(tb)), b(kThreads);
+int launch_part(int norm, const Table& tb, int blocks, double* parts, hipStream_t s) {
+    const dim3 g(blocks), b(kThreads);
     if (norm == Y6_NORM_L2) hipLaunchKernelGGL(grad_part_kernel<Y6_NORM_L2>, g, b, 0, s, tb, parts);
     else if (norm == Y6_NORM_L1) hipLaunchKernelGGL(grad_part_kernel<Y6_NORM_L1>, g, b, 0, s, tb, parts);
     else hipLaunchKernelGGL(grad_part_kernel<Y6_NORM_INF>, g, b, 0, s, tb, parts);
@@ -358,13 +385,14 @@ int launch_part(int norm, const Table& tb, double* parts, hipStream_t s) {
 int list_parts(const y6_grad_list* l, double* parts, size_t cap, int* n, hipStream_t s) {
     Table tb;
     *n = 0;
-    for (int i = 0; i < l->count;) {
-        i = fill_table(l, i, tb);
-        if (tb.count == 0) break;
-        Y6_REQUIRE((size_t)*n + table_blocks(tb) + 1 <= cap, "grad_norm: workspace too small");
-        const int rc = launch_part(l->norm_type, tb, parts + *n, s);
+    int i = 0;
+    long long from = 0;
+    while (const unsigned chunks = fill_table(l, i, from, tb)) {
+        const int blocks = table_blocks(chunks);
+        Y6_REQUIRE((size_t)*n + blocks + 1 <= cap, "grad_norm: workspace too small");
+        const int rc = launch_part(l->norm_type, tb, blocks, parts + *n, s);
         if (rc != Y6_OK) return rc;
-        *n += table_blocks(tb);
+        *n += blocks;
     }
     return Y6_OK;
 }
@@ -372,9 +400,8 @@ int list_parts(const y6_grad_list* l, double* parts, size_t cap, int* n, hipStre
 }  // namespace
 
 // ====================================================================== C ABI
-extern "C" size_t y6_grad_norm_workspace_bytes(int count) {
-    const size_t tables = count > 0 ? ((size_t)count + kTable - 1) / kTable : 1;
-    return (tables * kBlocks + 1) * sizeof(double);
+extern "C" size_t y6_grad_norm_workspace_bytes(int count, int64_t elements) {
+    return (tables_for(count > 0 ? (size_t)count : 0, elements > 0 ? (unsigned long long)elements : 0) * kBlocks + 1) * sizeof(double);
 }
 
 extern "C" int y6_grad_norm(const y6_grad_list* l, void* workspace, size_t workspace_bytes, float* norm, void* stream) {
@@ -427,10 +454,10 @@ extern "C" int y6_grad_clip(const y6_grad_list* l, double max_norm, void* worksp
         n = 1;
     }
     Table tb;
-    for (int i = 0; i < l->count;) {
-        i = fill_table(l, i, tb);
-        if (tb.count == 0) break;
-        hipLaunchKernelGGL(grad_scale_kernel, dim3(table_blocks(tb)), dim3(kThreads), 0, s, tb, l->norm_type, parts, n, max_norm, norm);
+    int i = 0;
+    long long from = 0;
+    while (const unsigned chunks = fill_table(l, i, from, tb)) {
+        hipLaunchKernelGGL(grad_scale_kernel, dim3(table_blocks(chunks)), dim3(kThreads), 0, s, tb, l->norm_type, parts, n, max_norm, norm);
         Y6_LAUNCH_CHECK();
     }
     return Y6_OK;

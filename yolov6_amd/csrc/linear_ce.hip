@@ -26,7 +26,8 @@ typedef short s16x4_t __attribute__((ext_vector_type(4)));
 typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
-constexpr size_t kPieceBytes = (size_t)128 << 20;
+constexpr size_t kPieceBytes = (size_t)128 << 20;     // of dz: half the last-level cache, and tiles enough to fill the chip
+constexpr size_t kPartBytes = (size_t)256 << 20;      // of the tiles' statistics: the forward takes the rows in as many pieces
 constexpr int kRowBytes = 128;             // bytes of the reduction of a step, for the splits' count: 64 fp16 / bf16 or 32 fp32 values
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
@@ -59,11 +60,12 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_logf(v); }
 
 // ------------------------------------------------------------------------------------------------------------- rows with a label
-// Block b takes rows [16 b, 16 b + 16): counts the labelled rows before them (at most kCountRows / 256 loads a thread; with more rows a
+// Block b takes rows [16 b, 16 b + 16): counts the labelled rows before them (at most kCountRows / 1024 loads a thread; with more rows a
 // kernel of its own counts per block first), then copies its labelled rows to their places, each padded with zeros to a multiple of
-// 16 bytes.  Four rows a wave: 4096 x 1024 bf16 are 256 blocks.
+// 16 bytes, a row per wave.
 constexpr int kGatherRows = 16;
-constexpr int kCountRows = 2048;
+constexpr int kGatherThreads = kGatherRows * 64;
+constexpr int kCountRows = 4096;
 
 struct GatherArgs {
     const char* x;
@@ -82,12 +84,15 @@ struct GatherArgs {
     float* loss_rows;              // 0 for rows without a label (reduction none), or null
 };
 
-__device__ __forceinline__ int block_count(int mine, int* sh) {       // sum over the 256 threads
+__device__ __forceinline__ int block_count(int mine, int* sh) {       // sum over gather_kernel's threads
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1) mine += __shfl_down(mine, d);
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = mine;
     __syncthreads();
-    return sh[0] + sh[1] + sh[2] + sh[3];
+    int r = 0;
+#pragma unroll
+    for (int w = 0; w < kGatherRows; ++w) r += sh[w];
+    return r;
 }
 
 __global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg, int segs) {
@@ -97,15 +102,15 @@ __global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ 
 }
 
 template <int ES>
-__global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
-    __shared__ int sh[4];
+__global__ __launch_bounds__(kGatherThreads) void gather_kernel(const GatherArgs a) {
+    __shared__ int sh[kGatherRows];
     __shared__ int place[kGatherRows];
     const int r0 = blockIdx.x * kGatherRows;
     int before = 0;
     if (a.seg) {
-        for (int i = threadIdx.x; i < (int)blockIdx.x; i += 256) before += a.seg[i];
+        for (int i = threadIdx.x; i < (int)blockIdx.x; i += kGatherThreads) before += a.seg[i];
     } else {
-        for (int i = threadIdx.x; i < r0; i += 256) before += a.target[i] != a.ignore ? 1 : 0;
+        for (int i = threadIdx.x; i < r0; i += kGatherThreads) before += a.target[i] != a.ignore ? 1 : 0;
     }
     before = block_count(before, sh);
     if (threadIdx.x < 64) {
@@ -129,31 +134,46 @@ __global__ __launch_bounds__(256) void gather_kernel(const GatherArgs a) {
     const int rows = a.rows - r0 < kGatherRows ? a.rows - r0 : kGatherRows;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
-    for (int i = wave; i < rows; i += 4) {
-        const int p = place[i];
-        const char* const src = a.x + (long long)(r0 + i) * a.pitch;
-        if (p >= 0) {
-            char* const dst = a.xc + (long long)p * a.cpitch;
-            if (a.vec) {
-                for (int o = lane * 16; o < a.width * ES; o += 1024) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
-            } else {
-                for (int e = lane; e < a.cpitch / ES; e += 64)
-                    reinterpret_cast<U*>(dst)[e] = e < a.width ? reinterpret_cast<const U*>(src)[e] : (U)0;
-            }
-        }
+    if (wave >= rows || place[wave] < 0) return;
+    const char* const src = a.x + (long long)(r0 + wave) * a.pitch;
+    char* const dst = a.xc + (long long)place[wave] * a.cpitch;
+    if (a.vec) {
+        for (int o = lane * 16; o < a.width * ES; o += 1024) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
+    } else {
+#pragma unroll 8
+        for (int e = lane; e < a.cpitch / ES; e += 64) reinterpret_cast<U*>(dst)[e] = e < a.width ? reinterpret_cast<const U*>(src)[e] : (U)0;
     }
 }
 
-// rows padded with zeros to multiples of 16 bytes (a weight whose width or address the wide loads do not take)
+// Rows padded with zeros to multiples of 16 bytes (a weight whose width or address the wide loads do not take).  A thread writes 16
+// bytes; where its elements are all there it reads the aligned 4-byte words that hold them and shifts, else element by element.
 template <int ES>
 __global__ __launch_bounds__(256) void pad_kernel(const char* __restrict__ src, long long pitch, int rows, int width, char* __restrict__ dst,
                                                   long long dpitch) {
     typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    for (long long r = (long long)blockIdx.x * 4 + wave; r < rows; r += (long long)gridDim.x * 4) {
-        const U* const s = reinterpret_cast<const U*>(src + r * pitch);
-        U* const d = reinterpret_cast<U*>(dst + r * dpitch);
-        for (int e = lane; e < dpitch / ES; e += 64) d[e] = e < width ? s[e] : (U)0;
+    constexpr int V = 16 / ES;
+    const int q = (int)(dpitch / 16);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * q; i += (long long)gridDim.x * 256) {
+        const long long r = i / q;
+        const int c = (int)(i - r * q) * V;
+        const U* const s = reinterpret_cast<const U*>(src + r * pitch) + c;
+        uint4 o;
+        if (ES == 2 && c + V < width && (r > 0 || c > 0)) {           // (the words around them are the tensor's own)
+            const unsigned sh = (unsigned)((uintptr_t)s & 2) * 8;
+            const unsigned* const w = reinterpret_cast<const unsigned*>((uintptr_t)s & ~(uintptr_t)3);
+            unsigned x[5];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] = w[k];
+            x[4] = sh ? w[4] : 0;
+            o.x = __builtin_amdgcn_alignbit(x[1], x[0], sh), o.y = __builtin_amdgcn_alignbit(x[2], x[1], sh);
+            o.z = __builtin_amdgcn_alignbit(x[3], x[2], sh), o.w = __builtin_amdgcn_alignbit(x[4], x[3], sh);
+        } else {
+            U e[V];
+#pragma unroll
+            for (int k = 0; k < V; ++k) e[k] = c + k < width ? s[k] : (U)0;
+            __builtin_memcpy(&o, e, 16);
+        }
+        *reinterpret_cast<uint4*>(dst + r * dpitch + (long long)c * ES) = o;
     }
 }
 
@@ -275,6 +295,7 @@ struct GemmArgs {
     long long pa, pb;              // bytes between rows
     int M, N, K;
     const int* count;              // labelled rows: the extent that COUNT says
+    int row0;                      // scores: the first of these rows (b, label, lsec ... start there)
     int tiles_m, tiles_n, splits;
     // EPI_STATS, EPI_DZ: m = class, n = labelled row
     const void* bias;
@@ -369,9 +390,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char*
     const int N = COUNT == COUNT_N ? *g.count : g.N, K = COUNT == COUNT_K ? *g.count : g.K;
     if (COUNT == COUNT_N && !g.part && N < g.N) {        // dx of rows n0.. without a label: zeros
         const int wide = g.M - m0 < BM ? g.M - m0 : BM;
-        for (int r = n0 + wave; r < n0 + BN && r < g.N; r += NW)
-            if (g.place[r] < 0)
-                for (int c = lane; c < wide; c += 64) reinterpret_cast<typename E::S*>(g.out)[(long long)r * g.out_pitch + m0 + c] = E::put(0.f);
+        for (int r0 = n0; r0 < n0 + BN; r0 += 64) {
+            const unsigned long long none = __ballot(r0 + lane < g.N && g.place[r0 + lane < g.N ? r0 + lane : 0] < 0);
+            for (int k = wave; k < 64; k += NW)
+                if (none >> k & 1)
+                    for (int c = lane; c < wide; c += 64) reinterpret_cast<typename E::S*>(g.out)[(long long)(r0 + k) * g.out_pitch + m0 + c] = E::put(0.f);
+        }
     }
     if (n0 >= N) return;
     const int steps = (K + OA::KS - 1) / OA::KS;
@@ -486,7 +510,7 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave % WM, wn = wave / WM;
     const int half = lane >> 5, l31 = lane & 31;
-    const int N = *g.count, K = g.K;
+    const int N = *g.count - g.row0 < g.N ? *g.count - g.row0 : g.N, K = g.K;
     // (XCDs and groups of tiles: gemm_tile)
     const int total = g.tiles_m * g.tiles_n, per = (total + 7) >> 3;
     const int base = (blockIdx.x & 7) * per, stride = gridDim.x >> 3;
@@ -718,12 +742,12 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void grads_kernel(c
 }
 
 // ------------------------------------------------------------------------------------------------------------------- small kernels
-// lse and loss of each labelled row: `places` rows (a power of two) x 1024 / places slices of the tiles' statistics per block - 32 rows
-// read whole 128-byte lines, few rows are cut into more slices
+// lse and loss of each labelled row: `places` rows (a power of two) x 1024 / places slices of the tiles' statistics per block: 32 rows
+// read whole 128-byte lines, fewer rows are cut into more slices so that there are blocks enough
 struct FinishArgs {
     const float *part_m, *part_s, *part_z, *zt;
     long long np;
-    int parts, places;
+    int parts, places, row0, rows; // of the labelled rows those from row0 on, `rows` of them (the pointers start there)
     const int *rowmap, *label, *count;
     float smooth, smooth_share;
     float* lsec;                   // by place: log2 of the sum of exponentials
@@ -736,9 +760,10 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     __shared__ float sm[1024], ss[1024], sz[1024];
     const int i = threadIdx.x & (a.places - 1), sl = threadIdx.x / a.places;
     int slices = 1024 / a.places;
-    const int n = blockIdx.x * a.places + i, N = *a.count;
+    const int n = blockIdx.x * a.places + i, N = *a.count - a.row0 < a.rows ? *a.count - a.row0 : a.rows;
     float m = -INFINITY, s = 0.f, z = 0.f;
     if (n < N) {
+#pragma unroll 4
         for (int p = sl; p < a.parts; p += slices) {
             const float pm = a.part_m[(long long)p * a.np + n], ps = a.part_s[(long long)p * a.np + n];
             if (a.part_z) z += a.part_z[(long long)p * a.np + n];
@@ -974,7 +999,7 @@ struct Layout {
     size_t coef, gmax, dz, accx, accw, bpart;                                         // backward's
     size_t bytes;
     long long cpitch, np;              // bytes; rows
-    int scores, parts, places, piece, pieces, shares;
+    int scores, parts, places, stat_rows, piece, pieces, shares;
     GradWay grads;
     long long px, pw;
     bool pad_w;
@@ -992,7 +1017,6 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         return o;
     };
     L.cpitch = up_to(w * es, 16);
-    L.np = up_to(n, 64);
     L.pad_w = (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
     L.xc = take((size_t)n * L.cpitch);
     L.wc = take(L.pad_w ? (size_t)v * L.cpitch : 0);
@@ -1008,10 +1032,14 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
         L.scores = way_of_scores(fp32, v, n, steps);
         L.parts = ceil_div(v, kSide[L.scores]) * kWavesM[L.scores];
+        long long rows = (long long)(kPartBytes / ((size_t)L.parts * 8)) / 256 * 256;
+        if (rows < 256) rows = 256;
+        L.stat_rows = (int)(rows < n ? rows : n);
+        L.np = up_to(L.stat_rows, 64);
         // one block for all rows, which then also adds up the loss, where that is 16 rounds of its threads at most
         L.places = 1;
         while (L.places < n && L.places < 128) L.places *= 2;
-        if (L.places < n || (long long)L.places * L.parts > 16 * 1024) L.places = n >= 1024 ? 32 : n >= 64 ? 8 : 1;
+        if (L.places < n || (long long)L.places * L.parts > 16 * 1024) L.places = n >= 8192 ? 32 : n >= 64 ? 8 : 1;
         L.part_m = take((size_t)L.parts * L.np * 4);
         L.part_s = take((size_t)L.parts * L.np * 4);
         L.part_z = take(d->smoothing > 0.f ? (size_t)L.parts * L.np * 4 : 0);
@@ -1081,11 +1109,11 @@ int launch_gather(const Run& r) {
         Y6_LAUNCH_CHECK();
     }
     if (d->reduction == Y6_REDUCE_NONE) a.loss_rows = d->loss;
-    hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(256), 0, r.s, a);
+    hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(kGatherThreads), 0, r.s, a);
     Y6_LAUNCH_CHECK();
     if (r.L.pad_w) {
-        const int blocks = ceil_div(d->classes, 4);
-        hipLaunchKernelGGL(pad_kernel<E::ES>, dim3(blocks < 4096 ? blocks : 4096), dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes,
+        const long long blocks = ceil_div(d->classes * (r.L.cpitch / 16), 256);
+        hipLaunchKernelGGL(pad_kernel<E::ES>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes,
                            d->width, r.kept<char>(r.L.wc), r.L.cpitch);
         Y6_LAUNCH_CHECK();
     }
@@ -1183,25 +1211,34 @@ int forward(const Run& r) {
     GemmArgs g = {};
     g.a = L.pad_w ? r.kept<char>(L.wc) : (const char*)d->weight;
     g.pa = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
-    g.b = r.kept<char>(L.xc), g.pb = L.cpitch;
-    g.M = d->classes, g.N = (int)d->rows, g.K = d->width;
-    g.count = r.kept<int>(L.count), g.label = r.kept<int>(L.label), g.bias = d->bias;
+    g.pb = L.cpitch;
+    g.M = d->classes, g.K = d->width;
+    g.count = r.kept<int>(L.count), g.bias = d->bias;
     g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
-    g.zt = r.at<float>(L.zt), g.np = L.np;
-    Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
+    g.np = L.np;
     FinishArgs f = {};
-    f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.zt = g.zt, f.np = L.np, f.parts = L.parts, f.places = L.places;
-    f.rowmap = r.kept<int>(L.rowmap), f.label = g.label, f.count = g.count;
+    f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.np = L.np, f.parts = L.parts, f.places = L.places;
+    f.count = g.count;
     f.smooth = d->smoothing, f.smooth_share = d->smoothing / d->classes;
-    f.lsec = r.kept<float>(L.lsec), f.mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
-    const int blocks = ceil_div(d->rows, L.places);
-    if (d->reduction == Y6_REDUCE_NONE) f.rows_out = d->loss;
-    else if (blocks == 1) f.loss = d->loss;
-    else f.lossc = r.at<float>(L.lossc);
-    hipLaunchKernelGGL(finish_kernel, dim3(blocks), dim3(1024), 0, r.s, f);
-    Y6_LAUNCH_CHECK();
-    if (f.lossc) {
-        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, f.lossc, f.count, f.mean, d->loss);
+    f.mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
+    const bool sums = d->reduction != Y6_REDUCE_NONE, alone = d->rows <= L.places && L.stat_rows == d->rows;
+    for (long long n0 = 0; n0 < d->rows; n0 += L.stat_rows) {
+        g.row0 = f.row0 = (int)n0;
+        g.N = f.rows = (int)(d->rows - n0 < L.stat_rows ? d->rows - n0 : L.stat_rows);
+        g.b = r.kept<char>(L.xc) + n0 * L.cpitch;
+        g.label = f.label = r.kept<int>(L.label) + n0;
+        g.zt = r.at<float>(L.zt) + n0, f.zt = g.zt;
+        Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
+        f.rowmap = r.kept<int>(L.rowmap) + n0;
+        f.lsec = r.kept<float>(L.lsec) + n0;
+        if (!sums) f.rows_out = d->loss;
+        else if (alone) f.loss = d->loss;
+        else f.lossc = r.at<float>(L.lossc) + n0;
+        hipLaunchKernelGGL(finish_kernel, dim3(ceil_div(g.N, L.places)), dim3(1024), 0, r.s, f);
+        Y6_LAUNCH_CHECK();
+    }
+    if (sums && !alone) {
+        hipLaunchKernelGGL(loss_sum_kernel, dim3(1), dim3(1024), 0, r.s, r.at<float>(L.lossc), f.count, f.mean, d->loss);
         Y6_LAUNCH_CHECK();
     }
     return Y6_OK;

@@ -232,6 +232,7 @@ struct List {
     std::vector<int64_t> n;
     std::vector<int32_t> type;
     y6_grad_list c;
+    int64_t elements = 0;
     List(const std::vector<Tensor>& grads, int norm) {
         const auto device = grads[0].device();
         for (const Tensor& g : grads) {
@@ -242,6 +243,7 @@ struct List {
             dense.push_back(g.is_non_overlapping_and_dense() ? g : g.contiguous());
             at.push_back(dense.back().data_ptr());
             n.push_back(g.numel());
+            elements += g.numel();
             type.push_back(code);
         }
         c = {at.data(), n.data(), type.data(), (int32_t)at.size(), norm};
@@ -250,7 +252,7 @@ struct List {
 
 Tensor norm_of(const List& l) {
     const c10::DeviceGuard guard(l.dense[0].device());
-    const size_t size = lib.norm_workspace(l.c.count);
+    const size_t size = lib.norm_workspace(l.c.count, l.elements);
     const Tensor ws = bytes_on(l.dense[0], size), out = at::empty({}, l.dense[0].options().dtype(at::kFloat).requires_grad(false));
     check(lib.norm(&l.c, ws.data_ptr(), size, out.data_ptr<float>(), stream_of(ws.device())), "grad_norm");
     return out;
@@ -271,7 +273,7 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
     const List l(grads, norm);
     TORCH_CHECK(!error_if_nonfinite || std::isfinite(norm_of(l).item<float>()), "yolov6_amd: the norm of the gradients is not finite, so they cannot be clipped");
     const c10::DeviceGuard guard(l.dense[0].device());
-    const size_t size = lib.norm_workspace(l.c.count);
+    const size_t size = lib.norm_workspace(l.c.count, l.elements);
     const Tensor ws = bytes_on(l.dense[0], size), out = at::empty({}, l.dense[0].options().dtype(at::kFloat).requires_grad(false));
     check(lib.clip(&l.c, max_norm, ws.data_ptr(), size, out.data_ptr<float>(), stream_of(ws.device())), "grad_clip");
     for (size_t i = 0; i < grads.size(); ++i)

@@ -56,7 +56,7 @@ def grad_norm(grads, norm_type=2.0):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """Scale the gradients of `parameters` (a tensor or an iterable; those without `.grad` are left out, one that comes twice
     counts once) in place by min(1, max_norm / (norm + 1e-6)), norm = grad_norm of all of them; returns the norm before clipping.
-    The semantics of torch.nn.utils.clip_grad_norm_, in two launches for up to 160 tensors, without a host synchronisation unless
+    The semantics of torch.nn.utils.clip_grad_norm_, in two launches for up to 330 tensors, without a host synchronisation unless
     `error_if_nonfinite` asks for the check (then nothing has been scaled when it raises).  Gradients that share memory are
     refused.  Under a LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
@@ -117,7 +117,7 @@ class FusedSGD:
             scale, found = C.c_void_p(scaler.scale.data_ptr()), C.c_void_p(scaler.found_inf.data_ptr())
         lr3, wd3 = (C.c_float * 3)(*self.lr), (C.c_float * 3)(*self.wd)
         if max_norm is not None:
-            ws = torch.empty(lib.y6_grad_norm_workspace_bytes(1), dtype=torch.uint8, device=a.data.device)
+            ws = torch.empty(lib.y6_grad_norm_workspace_bytes(1, a.numel), dtype=torch.uint8, device=a.data.device)
             norm = torch.empty((), dtype=torch.float32, device=a.data.device)
             _lib.check(lib.y6_sgd_step_clipped(C.c_void_p(a.data.data_ptr()), C.c_void_p(a.grad.data_ptr()), C.c_void_p(self.buf.data_ptr()),
                                                C.c_void_p(self.group.data_ptr()), a.numel, lr3, wd3, self.momentum, int(self.nesterov),
