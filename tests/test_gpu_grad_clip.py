@@ -137,6 +137,11 @@ def test_refusals():
         grad_norm([a], 3)
     with pytest.raises(RuntimeError, match="one device"):
         grad_norm([a, torch.zeros(3)])
+    pe = torch.nn.Parameter(torch.zeros((4, 50), device=DEV))
+    pe.grad = a.expand(4, 50)
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_([pe], 1.0)
+    assert abs(float(grad_norm([pe.grad])) - 2 * _norm64([a], 2)) <= 2.0 ** -22 * _norm64([a], 2)
     pg = torch.nn.Parameter(torch.zeros(50, device=DEV))
     pg.grad = a * torch.nn.Parameter(torch.ones((), device=DEV))
     with pytest.raises(RuntimeError, match="graph"):

@@ -274,6 +274,22 @@ def test_autocast_and_the_torch_op():
     assert torch.autograd.grad(loss, low[0])[0].shape == low[0].shape
 
 
+def test_the_torch_op_under_compile():
+    import yolov6_amd.torch_ops  # noqa: F401
+
+    def step(x, w, t, b):
+        loss, _ = torch.ops.yolov6_hip.linear_cross_entropy(x * 2, w, t, b, -100, 0.1, "mean")
+        return loss * 3
+
+    x, w, b, t = _inputs(64, 48, 200, torch.bfloat16, True, seed=12)
+    got = []
+    for f in (step, torch.compile(step, backend="aot_eager", fullgraph=True)):
+        leaves = [o.detach().requires_grad_() for o in (x, w, b)]
+        loss = f(leaves[0], leaves[1], t, leaves[2])
+        got.append([loss.detach(), *torch.autograd.grad(loss, leaves)])
+    assert all(torch.equal(a, c) for a, c in zip(*got))
+
+
 def test_another_stream_and_graphs():
     """A side stream; then two captured steps whose replays alternate with eager ones on new inputs."""
     from yolov6_amd.models.losses.loss_ce import linear_cross_entropy

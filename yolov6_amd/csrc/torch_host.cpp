@@ -12,6 +12,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
@@ -270,6 +271,8 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
     const auto grads = tensors_of(parameters.ptr(), true);
     if (grads.empty()) return at::zeros({});
     for (const Tensor& g : grads) TORCH_CHECK(!g.requires_grad(), "yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place");
+    for (const Tensor& g : grads)
+        TORCH_CHECK(at::has_internal_overlap(g) != at::MemOverlap::Yes, "yolov6_amd: a gradient whose elements share memory is not scaled in place");
     const List l(grads, norm);
     TORCH_CHECK(!error_if_nonfinite || std::isfinite(norm_of(l).item<float>()), "yolov6_amd: the norm of the gradients is not finite, so they cannot be clipped");
     const c10::DeviceGuard guard(l.dense[0].device());

@@ -117,12 +117,13 @@ class FusedSGD:
             scale, found = C.c_void_p(scaler.scale.data_ptr()), C.c_void_p(scaler.found_inf.data_ptr())
         lr3, wd3 = (C.c_float * 3)(*self.lr), (C.c_float * 3)(*self.wd)
         if max_norm is not None:
-            ws = torch.empty(lib.y6_grad_norm_workspace_bytes(1, a.numel), dtype=torch.uint8, device=a.data.device)
-            norm = torch.empty((), dtype=torch.float32, device=a.data.device)
-            _lib.check(lib.y6_sgd_step_clipped(C.c_void_p(a.data.data_ptr()), C.c_void_p(a.grad.data_ptr()), C.c_void_p(self.buf.data_ptr()),
-                                               C.c_void_p(self.group.data_ptr()), a.numel, lr3, wd3, self.momentum, int(self.nesterov),
-                                               int(self.steps == 0), float(grad_mul), scale, found, float(max_norm), C.c_void_p(ws.data_ptr()),
-                                               ws.numel(), C.c_void_p(norm.data_ptr()), s), "sgd_step_clipped")
+            with torch.cuda.device(a.data.device):
+                ws = torch.empty(lib.y6_grad_norm_workspace_bytes(1, a.numel), dtype=torch.uint8, device=a.data.device)
+                norm = torch.empty((), dtype=torch.float32, device=a.data.device)
+                _lib.check(lib.y6_sgd_step_clipped(C.c_void_p(a.data.data_ptr()), C.c_void_p(a.grad.data_ptr()), C.c_void_p(self.buf.data_ptr()),
+                                                   C.c_void_p(self.group.data_ptr()), a.numel, lr3, wd3, self.momentum, int(self.nesterov),
+                                                   int(self.steps == 0), float(grad_mul), scale, found, float(max_norm), C.c_void_p(ws.data_ptr()),
+                                                   ws.numel(), C.c_void_p(norm.data_ptr()), _lib.current_stream_ptr()), "sgd_step_clipped")
             self.steps += 1
             bump_native_generation()
             return norm
