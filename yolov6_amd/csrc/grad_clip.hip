@@ -186,8 +186,8 @@ __device__ __forceinline__ void chunk_scale(char* base, unsigned long long at, u
     }
 }
 
-// The block's share of the launch's chunks is one contiguous run; f(entry, byte offset of the chunk) for each.  Every block adds up the
-// entries' chunks for itself (two entries a thread).
+// f(entry, byte offset of the chunk) for each of the block's chunks; all blocks together move over the tensors as one window.  Every block
+// adds up the entries' chunks for itself (two entries a thread).
 template <class F>
 __device__ __forceinline__ void for_chunks(const Table& tb, F f) {
     static_assert(kTable <= 2 * kThreads, "two entries a thread");
@@ -208,16 +208,14 @@ __device__ __forceinline__ void for_chunks(const Table& tb, F f) {
     if (threadIdx.x == 0) first[0] = 0;
     __syncthreads();
     const unsigned total = first[2 * kThreads];
-    unsigned c = (unsigned)((unsigned long long)total * blockIdx.x / gridDim.x);
-    const unsigned end = (unsigned)((unsigned long long)total * (blockIdx.x + 1) / gridDim.x);
-    int lo = 0, hi = tb.count;         // first[lo] <= c < first[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= c) lo = mid;
-        else hi = mid;
-    }
-    for (; c < end; ++c) {
-        while (c >= first[lo + 1]) ++lo;
+    int lo = 0;
+    for (unsigned c = blockIdx.x; c < total; c += gridDim.x) {
+        int hi = tb.count;             // first[lo] <= c < first[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first[mid] <= c) lo = mid;
+            else hi = mid;
+        }
         const int t = __builtin_amdgcn_readfirstlane(lo);
         f(entry(tb.at[t], tb.n[t]), (unsigned long long)(c - first[lo]) * kChunk);
     }

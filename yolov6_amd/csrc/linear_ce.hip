@@ -761,8 +761,13 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     const int i = threadIdx.x & (a.places - 1), sl = threadIdx.x / a.places;
     int slices = 1024 / a.places;
     const int n = blockIdx.x * a.places + i, N = *a.count - a.row0 < a.rows ? *a.count - a.row0 : a.rows;
-    float m = -INFINITY, s = 0.f, z = 0.f;
+    float m = -INFINITY, s = 0.f, z = 0.f, zt = 0.f;
+    int label = 0, row = 0;
     if (n < N) {
+        if (sl == 0) {                 // (asked for early: they are needed behind the last barrier)
+            zt = a.zt[n], label = a.label[n];
+            if (a.rows_out) row = a.rowmap[n];
+        }
 #pragma unroll 4
         for (int p = sl; p < a.parts; p += slices) {
             const float pm = a.part_m[(long long)p * a.np + n], ps = a.part_s[(long long)p * a.np + n];
@@ -789,11 +794,11 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     if (sl == 0 && n < N) {
         // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
         float l2 = (m == -INFINITY ? 0.f : m) + log2_fast(s);
-        loss = l2 * kLn2 - (1.f - a.smooth) * a.zt[n];
+        loss = l2 * kLn2 - (1.f - a.smooth) * zt;
         if (a.smooth > 0.f) loss -= a.smooth_share * z;
-        if (a.label[n] < 0) l2 = loss = NAN;   // a label that is no class
+        if (label < 0) l2 = loss = NAN;        // a label that is no class
         a.lsec[n] = l2;
-        if (a.rows_out) a.rows_out[a.rowmap[n]] = loss;
+        if (a.rows_out) a.rows_out[row] = loss;
         if (a.lossc) a.lossc[n] = loss;
     }
     if (!a.loss) return;
