@@ -5,12 +5,16 @@
 //   dz_nv = g_n (exp(z_nv - lse_n) - (1-e) [v = t(n)] - e/V)
 //   dx = dz W       dW = dz^T x      db = sum_n dz_n
 //
-// Four matrix products of one tiled kernel (gemm_kernel):
-//   forward     z = W x^T, tile by tile; the epilogue leaves a running maximum and a sum of exponentials per row and tile
+// Four matrix products, all of the time at sizes that matter; the matrix cores bound them:
+//   forward     z = W x^T tile by tile (scores_kernel); the epilogue leaves a running maximum and a sum of exponentials per row and tile
 //   backward    for a piece of the vocabulary: z again, its epilogue turns it into dz (16 bits for 16-bit inputs: the operand the
 //               matrix instructions of the next two products take, one rounding), then dx += dz W[piece] and dW[piece] = dz^T x
-// so memory holds one piece of dz (kPieceBytes), never the logits.  Labelled rows are gathered first (`gather_kernel`): rows with
-// ignore_index cost nothing, and an infinity or a NaN in one of them reaches no gradient.
+//               in one launch (gemm_tile)
+// so memory holds one piece of dz (kPieceBytes), never the logits, and a product of 2 N V D operations is done twice: 8 N V D where 6 would
+// do with all logits kept.  8192 rows x 131072 classes x 1024, bf16: 8.0 ms, 1.10 PFLOP/s over the four; torch's product of such
+// operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on the same card, which lowers its clock under either.
+// Labelled rows are gathered first (gather_kernel): rows with ignore_index cost nothing, and an infinity or a NaN in one of them reaches no
+// gradient.  What the forward gathered, and its statistics, are kept for the backward.
 //
 // No atomics: partial statistics and split products are joined in a fixed order, the same inputs give the same bits.
 #include <atomic>
@@ -28,33 +32,55 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
 constexpr size_t kPieceBytes = (size_t)128 << 20;     // of dz: half the last-level cache, and tiles enough to fill the chip
 constexpr size_t kPartBytes = (size_t)256 << 20;      // of the tiles' statistics: the forward takes the rows in as many pieces
-constexpr int kRowBytes = 128;             // bytes of the reduction of a step, for the splits' count: 64 fp16 / bf16 or 32 fp32 values
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
 // adds nothing that fp16 gradients show.  bf16 and fp32 have the range.
 constexpr float kHalfScale = 16384.f;
 
+// Types: S of the caller's tensors; PLANES 16-bit operands (O) that stand for one value in LDS, RB bytes of each plane that a step takes
+// from a row.  fp32 goes as three bf16 planes, h = the upper 8 significant bits, m = the next 8, l = the last 8: their sum is the value,
+// exactly, and six of their nine products (the other three are below 2^-23 of the whole) on the bf16 matrix cores take 6 / 16 of what
+// the fp32 ones take for the one.
 struct Half {
-    static constexpr int ES = 2, TYPE = Y6_F16;
+    static constexpr int ES = 2, TYPE = Y6_F16, PLANES = 1, RB = 128;
     static constexpr float kScale = kHalfScale;
     typedef _Float16 S;
+    typedef _Float16 O;
     static __device__ __forceinline__ float get(S v) { return (float)v; }
     static __device__ __forceinline__ S put(float v) { return (S)v; }
 };
 struct Brain {
-    static constexpr int ES = 2, TYPE = Y6_BF16;
+    static constexpr int ES = 2, TYPE = Y6_BF16, PLANES = 1, RB = 128;
     static constexpr float kScale = 1.f;
     typedef __bf16 S;
+    typedef __bf16 O;
     static __device__ __forceinline__ float get(S v) { return (float)v; }
     static __device__ __forceinline__ S put(float v) { return (S)v; }
 };
 struct Single {
-    static constexpr int ES = 4, TYPE = Y6_F32;
+    static constexpr int ES = 4, TYPE = Y6_F32, PLANES = 3, RB = 64;
     static constexpr float kScale = 1.f;
     typedef float S;
+    typedef __bf16 O;
     static __device__ __forceinline__ float get(S v) { return v; }
     static __device__ __forceinline__ S put(float v) { return v; }
 };
+
+// the planes of a value: cut, not rounded (a large value stays finite), so that each remainder is exact; an infinity or a NaN is the first
+// plane's alone
+__device__ __forceinline__ void split3(float v, unsigned short (&p)[3]) {
+    const unsigned u = __float_as_uint(v);
+    if ((u & 0x7f800000u) == 0x7f800000u) {
+        p[0] = (unsigned short)((u >> 16) | ((u & 0xffffu) ? 0x40u : 0u));
+        p[1] = p[2] = 0;
+        return;
+    }
+    const unsigned h = u & 0xffff0000u;
+    const float r = v - __uint_as_float(h);
+    const unsigned m = __float_as_uint(r) & 0xffff0000u;
+    const float q = r - __uint_as_float(m);
+    p[0] = (unsigned short)(h >> 16), p[1] = (unsigned short)(m >> 16), p[2] = (unsigned short)(__float_as_uint(q) >> 16);
+}
 
 __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_logf(v); }
@@ -73,10 +99,10 @@ struct GatherArgs {
     const int64_t* target;
     long long ignore;
     int rows, width, classes;
-    int vec;                       // rows are multiples of 16 bytes at 16-byte addresses
+    int vec;                       // rows start at 16-byte addresses, and 16-bit ones are multiples of 16 bytes
     const int* seg;                // labelled rows per block (above kCountRows), or null
     char* xc;
-    long long cpitch;              // bytes
+    long long cpitch, plane;       // bytes between rows, planes
     int* rowmap;                   // place -> row
     int* place;                    // row -> place, -1: no label
     int* label;                    // place -> label, -1: not a class
@@ -99,6 +125,24 @@ __global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ 
     const int r = blockIdx.x * 256 + threadIdx.x, s = r / kGatherRows;
     const unsigned long long m = __ballot(r < rows && target[r < rows ? r : 0] != ignore);
     if (s < segs && r % kGatherRows == 0) seg[s] = __popcll((m >> (threadIdx.x & 63)) & ((1ull << kGatherRows) - 1));
+}
+
+// the planes of four values of a row, zeros behind its width
+__device__ __forceinline__ void split_row4(const float* src, int c, int width, int vec, char* dst, long long plane) {
+    float v[4];
+    if (vec && c + 4 <= width) {
+        const float4 f = *reinterpret_cast<const float4*>(src + c);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = c + e < width ? src[c + e] : 0.f;
+    }
+    unsigned short p[4][3];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) split3(v[e], p[e]);
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        *reinterpret_cast<uint2*>(dst + k * plane + c * 2) = make_uint2(p[0][k] | (unsigned)p[1][k] << 16, p[2][k] | (unsigned)p[3][k] << 16);
 }
 
 template <int ES>
@@ -133,32 +177,42 @@ __global__ __launch_bounds__(kGatherThreads) void gather_kernel(const GatherArgs
     __syncthreads();
     const int rows = a.rows - r0 < kGatherRows ? a.rows - r0 : kGatherRows;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
     if (wave >= rows || place[wave] < 0) return;
     const char* const src = a.x + (long long)(r0 + wave) * a.pitch;
     char* const dst = a.xc + (long long)place[wave] * a.cpitch;
-    if (a.vec) {
-        for (int o = lane * 16; o < a.width * ES; o += 1024) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
+    if (ES == 4) {
+        for (int c = lane * 4; c < a.cpitch / 2; c += 256) split_row4(reinterpret_cast<const float*>(src), c, a.width, a.vec, dst, a.plane);
+    } else if (a.vec) {
+        for (int o = lane * 16; o < a.width * 2; o += 1024) *reinterpret_cast<uint4*>(dst + o) = *reinterpret_cast<const uint4*>(src + o);
     } else {
 #pragma unroll 8
-        for (int e = lane; e < a.cpitch / ES; e += 64) reinterpret_cast<U*>(dst)[e] = e < a.width ? reinterpret_cast<const U*>(src)[e] : (U)0;
+        for (int e = lane; e < a.cpitch / 2; e += 64)
+            reinterpret_cast<unsigned short*>(dst)[e] = e < a.width ? reinterpret_cast<const unsigned short*>(src)[e] : (unsigned short)0;
     }
 }
 
-// Rows padded with zeros to multiples of 16 bytes (a weight whose width or address the wide loads do not take).  A thread writes 16
+// The planes of an fp32 weight
+__global__ __launch_bounds__(256) void split_kernel(const char* __restrict__ src, long long pitch, int rows, int width, int vec, char* __restrict__ dst,
+                                                    long long dpitch, long long plane) {
+    const int q = (int)(dpitch / 8);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * q; i += (long long)gridDim.x * 256) {
+        const long long r = i / q;
+        split_row4(reinterpret_cast<const float*>(src + r * pitch), (int)(i - r * q) * 4, width, vec, dst + r * dpitch, plane);
+    }
+}
+
+// Rows of a 16-bit weight padded with zeros to multiples of 16 bytes (its width or address is not one the wide loads take).  A thread writes 16
 // bytes; where its elements are all there it reads the aligned 4-byte words that hold them and shifts, else element by element.
-template <int ES>
 __global__ __launch_bounds__(256) void pad_kernel(const char* __restrict__ src, long long pitch, int rows, int width, char* __restrict__ dst,
                                                   long long dpitch) {
-    typedef typename std::conditional<ES == 4, unsigned, unsigned short>::type U;
-    constexpr int V = 16 / ES;
+    typedef unsigned short U;
     const int q = (int)(dpitch / 16);
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)rows * q; i += (long long)gridDim.x * 256) {
         const long long r = i / q;
-        const int c = (int)(i - r * q) * V;
+        const int c = (int)(i - r * q) * 8;
         const U* const s = reinterpret_cast<const U*>(src + r * pitch) + c;
         uint4 o;
-        if (ES == 2 && c + V < width && (r > 0 || c > 0)) {           // (the words around them are the tensor's own)
+        if (c + 8 < width && (r > 0 || c > 0)) {                      // (the words around them are the tensor's own)
             const unsigned sh = (unsigned)((uintptr_t)s & 2) * 8;
             const unsigned* const w = reinterpret_cast<const unsigned*>((uintptr_t)s & ~(uintptr_t)3);
             unsigned x[5];
@@ -168,12 +222,12 @@ __global__ __launch_bounds__(256) void pad_kernel(const char* __restrict__ src, 
             o.x = __builtin_amdgcn_alignbit(x[1], x[0], sh), o.y = __builtin_amdgcn_alignbit(x[2], x[1], sh);
             o.z = __builtin_amdgcn_alignbit(x[3], x[2], sh), o.w = __builtin_amdgcn_alignbit(x[4], x[3], sh);
         } else {
-            U e[V];
+            U e[8];
 #pragma unroll
-            for (int k = 0; k < V; ++k) e[k] = c + k < width ? s[k] : (U)0;
+            for (int k = 0; k < 8; ++k) e[k] = c + k < width ? s[k] : (U)0;
             __builtin_memcpy(&o, e, 16);
         }
-        *reinterpret_cast<uint4*>(dst + r * dpitch + (long long)c * ES) = o;
+        *reinterpret_cast<uint4*>(dst + r * dpitch + (long long)c * 2) = o;
     }
 }
 
@@ -198,77 +252,62 @@ __device__ __forceinline__ void dma16(const i32x4_t& rsrc, unsigned voff, unsign
 }
 __device__ __forceinline__ unsigned lds_addr(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
 
-// One operand's tile of a stage: ROWS rows (of the result's m or n) by KB bytes (128 or 64) of the reduction.
-//   KC (reduction contiguous in memory): image [row][KB], its 16-byte pieces permuted so that eight consecutive rows read the same
+// One operand's tile of a stage: ROWS rows (of the result's m or n) by RB bytes of the reduction, for each plane an image.
+//   KC (reduction contiguous in memory): image [row][RB], its 16-byte pieces permuted so that eight consecutive rows read the same
 //      piece from eight different bank groups
-//   else (rows of the reduction, m / n contiguous), 16-bit: image [32 columns][reduction KB / 2][64 B], read by the transposing
-//      ds_read_b64_tr_b16; fp32: image [reduction KB / 4][ROWS], read a value at a time
-template <class E, bool KC, int ROWS, int NW, int KB>
+//   else (rows of the reduction, m / n contiguous): image [32 columns][reduction RB / 2][64 B], read by the transposing ds_read_b64_tr_b16
+template <class E, bool KC, int ROWS, int NW>
 struct Operand {
-    static constexpr int kBytes = ROWS * KB;
+    static constexpr int RB = E::RB, kPlane = ROWS * RB, kBytes = kPlane * E::PLANES;
     static constexpr int kInstr = kBytes / 1024;
     static constexpr int kPer = kInstr / NW;
-    static constexpr int KS = KB / E::ES;                // values of the reduction per stage
-    static_assert(kInstr % NW == 0, "requests divide over the waves");
-    static_assert(KB == 128 || KB == 64, "eight or four pieces a row");
+    static constexpr int KS = RB / 2;                    // values of the reduction per stage
+    static constexpr int kSubs = RB / 32;                // sub-steps of the matrix instructions per stage
+    static_assert(kInstr % NW == 0 && kPlane % 1024 == 0, "requests divide over the waves and the planes");
+    static_assert(RB == 128 || RB == 64, "eight or four pieces a row");
 
-    static __device__ __forceinline__ int permuted(int row, int piece) { return KB == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3); }
+    static __device__ __forceinline__ int permuted(int row, int piece) { return RB == 128 ? piece ^ (row & 7) : piece ^ ((row >> 1) & 3); }
 
     // requests of the stage that starts at value k0 of the reduction; rows r0.. of `extent`, reduction `depth` long
-    static __device__ __forceinline__ void issue(const char* base, long long pitch, int r0, int extent, int k0, int depth, unsigned lds, int wave, int lane) {
-        if (KC) {
-            constexpr int RPI = 1024 / KB;               // rows per request
-            const long long left = (long long)(extent - r0) * pitch;
-            const i32x4_t rs = make_rsrc(base + (long long)r0 * pitch, (unsigned)(left < kOob ? left : kOob));
-            const int lr = lane / (KB / 16);
-            const int kb = k0 * E::ES + (permuted(lr, lane & (KB / 16 - 1)) << 4);
-            const bool in = kb < depth * E::ES;
+    static __device__ __forceinline__ void issue(const char* base, long long pitch, long long plane, int r0, int extent, int k0, int depth, unsigned lds,
+                                                 int wave, int lane) {
+        const long long left = KC ? (long long)(extent - r0) * pitch : (long long)(depth - k0) * pitch;
+        const char* const at = base + (KC ? (long long)r0 : (long long)k0) * pitch;
+        const unsigned bytes = (unsigned)(left < kOob ? left : kOob);
 #pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int ins = wave * kPer + i;
-                const unsigned voff = (unsigned)(ins * RPI + lr) * (unsigned)pitch + (unsigned)kb;
-                dma16(rs, in ? voff : kOob, lds + ins * 1024);
+        for (int i = 0; i < kPer; ++i) {
+            const int ins = wave * kPer + i;
+            const int p = E::PLANES == 1 ? 0 : ins / (kPlane / 1024), in = E::PLANES == 1 ? ins : ins - p * (kPlane / 1024);
+            const i32x4_t rs = make_rsrc(at + p * plane, bytes);
+            unsigned voff;
+            bool inside;
+            if (KC) {
+                const int lr = lane / (RB / 16);         // 1024 / RB rows a request
+                const int kb = k0 * 2 + (permuted(lr, lane & (RB / 16 - 1)) << 4);
+                inside = kb < depth * 2;
+                voff = (unsigned)(in * (1024 / RB) + lr) * (unsigned)pitch + (unsigned)kb;
+            } else {
+                const int k = in % (RB / 32) * 16 + (lane >> 2), col = in / (RB / 32) * 32 + (lane & 3) * 8;
+                inside = r0 + col < extent;
+                voff = (unsigned)k * (unsigned)pitch + (unsigned)(r0 + col) * 2;
             }
-        } else {
-            const long long left = (long long)(depth - k0) * pitch;
-            const i32x4_t rs = make_rsrc(base + (long long)k0 * pitch, (unsigned)(left < kOob ? left : kOob));
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) {
-                const int ins = wave * kPer + i;
-                int k, col;
-                if (E::ES == 2) {
-                    constexpr int IPC = KB / 32;         // requests per 32 columns
-                    k = (ins % IPC) * 16 + (lane >> 2);
-                    col = (ins / IPC) * 32 + (lane & 3) * 8;
-                } else {
-                    const int b = ins * 1024 + lane * 16;
-                    k = b / (ROWS * 4);
-                    col = (b % (ROWS * 4)) / 4;
-                }
-                const unsigned voff = (unsigned)k * (unsigned)pitch + (unsigned)(r0 + col) * E::ES;
-                dma16(rs, r0 + col < extent ? voff : kOob, lds + ins * 1024);
-            }
+            dma16(rs, inside ? voff : kOob, lds + ins * 1024);
         }
     }
-    // the 32 rows from row f: lane's 16 bytes of sub-step kk (KB / 32 per stage).  16-bit: reduction values 16 kk + 8 (lane >> 5) +
-    // 0..7; fp32: 8 kk + 4 (lane >> 5) + 0..3
-    static __device__ __forceinline__ u32x4 frag(const char* img, int f, int kk, int lane) {
+    // plane p of the 32 rows from row f: lane's 16 bytes of sub-step kk, reduction values 16 kk + 8 (lane >> 5) + 0..7
+    static __device__ __forceinline__ u32x4 frag(const char* img, int p, int f, int kk, int lane) {
         const int half = lane >> 5, l31 = lane & 31;
+        img += p * kPlane;
         if (KC) {
-            return *reinterpret_cast<const u32x4*>(img + (f + l31) * KB + (permuted(l31, kk * 2 + half) << 4));
-        } else if (E::ES == 2) {
-            const char* const p = img + (f >> 5) * (KB * 32) + (kk * 16 + half * 8 + ((lane & 15) >> 2)) * 64 + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
-            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p));
-            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(p + 256));
+            return *reinterpret_cast<const u32x4*>(img + (f + l31) * RB + (permuted(l31, kk * 2 + half) << 4));
+        } else {
+            const char* const q = img + (f >> 5) * (RB * 32) + (kk * 16 + half * 8 + ((lane & 15) >> 2)) * 64 + (16 * ((lane >> 4) & 1) + 4 * (lane & 3)) * 2;
+            const s16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q));
+            const s16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4_t*)(q + 256));
             typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
             const u32x2 l2 = __builtin_bit_cast(u32x2, lo), h2 = __builtin_bit_cast(u32x2, hi);
             u32x4 r;
             r[0] = l2[0], r[1] = l2[1], r[2] = h2[0], r[3] = h2[1];
-            return r;
-        } else {
-            u32x4 r;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const unsigned*>(img + ((kk * 8 + half * 4 + i) * ROWS + f + l31) * 4);
             return r;
         }
     }
@@ -276,23 +315,36 @@ struct Operand {
 
 template <class E>
 __device__ __forceinline__ f32x16_t mma(const u32x4& a, const u32x4& b, f32x16_t c) {
-    if constexpr (E::TYPE == Y6_F16) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
-    } else if constexpr (E::TYPE == Y6_BF16) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
-    } else {
+    if constexpr (E::TYPE == Y6_F16) return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8_t, a), __builtin_bit_cast(h8_t, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8_t, a), __builtin_bit_cast(b8_t, b), c, 0, 0, 0);
+}
+// acc += the products of sub-step kk of a stage; of three planes the six products that count, the small ones first
+template <class E, class OA, class OB, int FM, int FN>
+__device__ __forceinline__ void sub_step(f32x16_t (&acc)[FM][FN], const char* ia, const char* ib, int fm, int fn, int kk, int lane) {
+    u32x4 fa[E::PLANES][FM], fb[E::PLANES][FN];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-        return c;
+    for (int p = 0; p < E::PLANES; ++p) {
+#pragma unroll
+        for (int i = 0; i < FM; ++i) fa[p][i] = OA::frag(ia, p, fm + i * 32, kk, lane);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[p][j] = OB::frag(ib, p, fn + j * 32, kk, lane);
     }
+#pragma unroll
+    for (int order = E::PLANES - 1; order >= 0; --order)
+#pragma unroll
+        for (int p = 0; p <= order; ++p)
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[p][i], fb[order - p][j], acc[i][j]);
 }
 
 enum { EPI_STATS, EPI_DZ };
-enum { COUNT_NONE, COUNT_N, COUNT_K };
+enum { COUNT_N, COUNT_K };
 
 struct GemmArgs {
     const char *a, *b;
-    long long pa, pb;              // bytes between rows
+    long long pa, pb, la, lb;      // bytes between rows, between planes
     int M, N, K;
     const int* count;              // labelled rows: the extent that COUNT says
     int row0;                      // scores: the first of these rows (b, label, lsec ... start there)
@@ -306,7 +358,7 @@ struct GemmArgs {
     float smooth, smooth_share;    // e, e / V
     int class0;                    // first class of the piece
     char* dz;
-    long long dz_pitch;            // bytes
+    long long dz_pitch, dz_plane;  // bytes
     // products into a gradient: m = column, n = row of the output
     float* part;                   // [split][N][part_pitch] or null: straight to out
     long long part_pitch;          // elements
@@ -327,15 +379,22 @@ __device__ __forceinline__ float grad_factor(const float* up, const float* gmax,
     return f * (1.f / E::kScale);
 }
 
+// four operands of each plane
 template <class E>
-__device__ __forceinline__ uint2 pack4(const float (&v)[4]) {
-    typedef typename E::S S4 __attribute__((ext_vector_type(4)));
-    S4 o;
+__device__ __forceinline__ void pack4(const float (&v)[4], uint2 (&r)[E::PLANES]) {
+    if constexpr (E::PLANES == 1) {
+        typedef typename E::O O4 __attribute__((ext_vector_type(4)));
+        O4 o;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = E::put(v[j]);
-    uint2 r;
-    __builtin_memcpy(&r, &o, sizeof(r));
-    return r;
+        for (int j = 0; j < 4; ++j) o[j] = (typename E::O)v[j];
+        __builtin_memcpy(&r[0], &o, sizeof(uint2));
+    } else {
+        unsigned short p[4][3];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split3(v[j], p[j]);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) r[k] = make_uint2(p[0][k] | (unsigned)p[1][k] << 16, p[2][k] | (unsigned)p[3][k] << 16);
+    }
 }
 template <class E, bool VEC>
 __device__ __forceinline__ void store4(char* dst, const float (&v)[4], int left) {
@@ -354,11 +413,11 @@ __device__ __forceinline__ void store4(char* dst, const float (&v)[4], int left)
     }
 }
 
-// Tile of a block: BM x BN of the result over WM x WN waves, KB bytes of the reduction per stage, STAGES stages, BPC blocks per CU.
-template <int BM_, int BN_, int WM_, int WN_, int KB_, int STAGES_, int BPC_>
+// Tile of a block: BM x BN of the result over WM x WN waves, STAGES stages of the operands (ROW bytes a row) in LDS, BPC blocks per CU.
+template <int BM_, int BN_, int WM_, int WN_, int STAGES_, int BPC_, int ROW_ = 128>
 struct Tile {
-    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KB = KB_, STAGES = STAGES_, BPC = BPC_, NW = WM_ * WN_;
-    static constexpr int kLds = STAGES_ * (BM_ + BN_) * KB_;
+    static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, STAGES = STAGES_, BPC = BPC_, NW = WM_ * WN_;
+    static constexpr int kLds = STAGES_ * (BM_ + BN_) * ROW_;         // ROW: bytes of all planes of a row
     static_assert(kLds * BPC_ <= 160 * 1024, "LDS of a CU");
 };
 
@@ -373,8 +432,8 @@ template <class E, bool AKC, bool BKC, class T, int COUNT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char* smem) {
     constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN;
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
-    typedef Operand<E, AKC, BM, NW, T::KB> OA;
-    typedef Operand<E, BKC, BN, NW, T::KB> OB;
+    typedef Operand<E, AKC, BM, NW> OA;
+    typedef Operand<E, BKC, BN, NW> OB;
     constexpr int kStage = OA::kBytes + OB::kBytes;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int wm = wave % WM, wn = wave / WM;
@@ -413,8 +472,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char*
     unsigned st_in = 0, st_out = 0;                      // stage the next requests fill, stage the next products read
     auto issue = [&](int s) {
         const unsigned st = lds0 + st_in;
-        OA::issue(g.a, g.pa, m0, g.M, s * OA::KS, K, st, wave, lane);
-        OB::issue(g.b, g.pb, n0, N, s * OA::KS, K, st + OA::kBytes, wave, lane);
+        OA::issue(g.a, g.pa, g.la, m0, g.M, s * OA::KS, K, st, wave, lane);
+        OB::issue(g.b, g.pb, g.lb, n0, N, s * OA::KS, K, st + OA::kBytes, wave, lane);
         st_in = st_in + kStage == T::STAGES * kStage ? 0 : st_in + kStage;
     };
     constexpr int kAhead = T::STAGES - 1;
@@ -430,17 +489,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& g, unsigned bid, char*
         const char* const ib = ia + OA::kBytes;
         st_out = st_out + kStage == T::STAGES * kStage ? 0 : st_out + kStage;
 #pragma unroll
-        for (int kk = 0; kk < T::KB / 32; ++kk) {
-            u32x4 fa[FM], fb[FN];
-#pragma unroll
-            for (int i = 0; i < FM; ++i) fa[i] = OA::frag(ia, wm * (BM / WM) + i * 32, kk, lane);
-#pragma unroll
-            for (int j = 0; j < FN; ++j) fb[j] = OB::frag(ib, wn * (BN / WN) + j * 32, kk, lane);
-#pragma unroll
-            for (int i = 0; i < FM; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[i], fb[j], acc[i][j]);
-        }
+        for (int kk = 0; kk < OA::kSubs; ++kk) sub_step<E, OA, OB, FM, FN>(acc, ia, ib, wm * (BM / WM), wn * (BN / WN), kk, lane);
     }
 
     // lane: row n = lane & 31 of a fragment; its 16 values are m = 8 (q >> 2) + 4 (lane >> 5) + (q & 3)
@@ -501,10 +550,9 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
     extern __shared__ __attribute__((aligned(16))) char smem[];
     constexpr int BM = T::BM, BN = T::BN, WM = T::WM, WN = T::WN;
     constexpr int NW = WM * WN, FM = BM / WM / 32, FN = BN / WN / 32;
-    typedef Operand<E, true, BM, NW, T::KB> OA;
-    typedef Operand<E, true, BN, NW, T::KB> OB;
+    typedef Operand<E, true, BM, NW> OA;
+    typedef Operand<E, true, BN, NW> OB;
     constexpr int kStage = OA::kBytes + OB::kBytes;
-    constexpr bool kPack = EPI == EPI_DZ && E::ES == 2;
     constexpr bool kStay = EPI == EPI_DZ;
     typedef typename E::S S;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -538,8 +586,8 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
     auto issue = [&]() {                                  // requests of the sequence's next step, if there is one
         if (pt >= end) return;
         const unsigned st = lds0 + st_in;
-        OA::issue(g.a, g.pa, ptm * BM, g.M, ps * OA::KS, K, st, wave, lane);
-        OB::issue(g.b, g.pb, ptn * BN, N, ps * OA::KS, K, st + OA::kBytes, wave, lane);
+        OA::issue(g.a, g.pa, g.la, ptm * BM, g.M, ps * OA::KS, K, st, wave, lane);
+        OB::issue(g.b, g.pb, g.lb, ptn * BN, N, ps * OA::KS, K, st + OA::kBytes, wave, lane);
         st_in = st_in + kStage == T::STAGES * kStage ? 0 : st_in + kStage;
         ++ahead;
         if (++ps == steps) {
@@ -570,35 +618,23 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
             const char* const ib = ia + OA::kBytes;
             st_out = st_out + kStage == T::STAGES * kStage ? 0 : st_out + kStage;
 #pragma unroll
-            for (int kk = 0; kk < T::KB / 32; ++kk) {
-                u32x4 fa[FM], fb[FN];
-#pragma unroll
-                for (int i = 0; i < FM; ++i) fa[i] = OA::frag(ia, wm * (BM / WM) + i * 32, kk, lane);
-#pragma unroll
-                for (int j = 0; j < FN; ++j) fb[j] = OB::frag(ib, wn * (BN / WN) + j * 32, kk, lane);
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[i], fb[j], acc[i][j]);
-            }
+            for (int kk = 0; kk < OA::kSubs; ++kk) sub_step<E, OA, OB, FM, FN>(acc, ia, ib, wm * (BM / WM), wn * (BN / WN), kk, lane);
         }
         const GemmArgs e = args_again();
         // lane: row n = lane & 31 of a fragment; its 16 values are m = 8 (q >> 2) + 4 (lane >> 5) + (q & 3)
         const int mw = tm * BM + wm * (BM / WM), nw = tn * BN + wn * (BN / WN);
         const bool whole = mw + BM / WM <= e.M;              // every class of this wave's tile is one
-        {
-            if (e.bias) {
-                const S* const bias = reinterpret_cast<const S*>(e.bias) + e.class0;
+        if (e.bias) {
+            const S* const bias = reinterpret_cast<const S*>(e.bias) + e.class0;
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
+            for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
-                        const float b = E::get(bias[m < e.M ? m : e.M - 1]);
+                for (int q = 0; q < 16; ++q) {
+                    const int m = mw + i * 32 + 8 * (q >> 2) + 4 * half + (q & 3);
+                    const float b = E::get(bias[m < e.M ? m : e.M - 1]);
 #pragma unroll
-                        for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
-                    }
-            }
+                    for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
+                }
         }
         if constexpr (EPI == EPI_STATS) {
 #pragma unroll
@@ -672,9 +708,9 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                 const float c = (e.coef ? e.coef[nl] : 1.f) * E::kScale;
                 const float share = -e.smooth_share * c, hit = (1.f - e.smooth) * c;
                 const int lab = e.label[nl] - e.class0 - mw - 4 * half;
-                char* const row = e.dz + (long long)n * e.dz_pitch + (long long)(mw + 4 * half) * E::ES;
+                char* const row = e.dz + (long long)n * e.dz_pitch + (long long)(mw + 4 * half) * 2;
                 const int left = e.M - mw - 4 * half;
-                const int room = (int)(e.dz_pitch / E::ES) - mw - 4 * half;
+                const int room = (int)(e.dz_pitch / 2) - mw - 4 * half;
                 auto emit = [&](auto labelled, auto inside) {
                     int at = lab, to = left, end16 = room;
                     asm volatile("" : "+v"(at), "+v"(to), "+v"(end16));   // (or the compiler forms every mask ahead of the branches, and they spill)
@@ -693,26 +729,32 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                                     if (labelled.value) d -= m == at ? hit : 0.f;
                                     v[k][c4] = d;
                                 }
-                            if (inside.value && kPack) {
+                            uint2 a[E::PLANES], b[E::PLANES];
+                            if (inside.value) {
                                 // the half-waves trade runs of four classes: each lane then holds eight in a row, one 16-byte store
-                                const uint2 a = pack4<E>(v[0]), b = pack4<E>(v[1]);
-                                const auto x = __builtin_amdgcn_permlane32_swap(a.x, b.x, false, false);
-                                const auto y = __builtin_amdgcn_permlane32_swap(a.y, b.y, false, false);
-                                if (live) *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * E::ES) = make_uint4(x[0], y[0], x[1], y[1]);
+                                pack4<E>(v[0], a);
+                                pack4<E>(v[1], b);
+#pragma unroll
+                                for (int p = 0; p < E::PLANES; ++p) {
+                                    const auto x = __builtin_amdgcn_permlane32_swap(a[p].x, b[p].x, false, false);
+                                    const auto y = __builtin_amdgcn_permlane32_swap(a[p].y, b[p].y, false, false);
+                                    if (live) *reinterpret_cast<uint4*>(row + p * e.dz_plane + (i * 32 + 16 * gp + 4 * half) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+                                }
                                 continue;
                             }
+                            // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it; runs
+                            // of four start at multiples of eight bytes, so a run is in the row or behind it)
 #pragma unroll
                             for (int k = 0; k < 2; ++k) {
                                 const int m = i * 32 + 16 * gp + 8 * k;
                                 __builtin_amdgcn_sched_barrier(0);
                                 if (!live || m >= end16) continue;
-                                // (the row is padded to 16 bytes: what lies behind the last class is zero, the reduction of dx runs over it)
-                                if (!inside.value) {
 #pragma unroll
-                                    for (int c4 = 0; c4 < 4; ++c4)
-                                        if (m + c4 >= to) v[k][c4] = 0.f;
-                                }
-                                store4<E, true>(row + m * E::ES, v[k], end16 - m);
+                                for (int c4 = 0; c4 < 4; ++c4)
+                                    if (m + c4 >= to) v[k][c4] = 0.f;
+                                pack4<E>(v[k], a);
+#pragma unroll
+                                for (int p = 0; p < E::PLANES; ++p) *reinterpret_cast<uint2*>(row + p * e.dz_plane + m * 2) = a[p];
                             }
                         }
                 };
@@ -883,11 +925,12 @@ __global__ __launch_bounds__(256) void join_kernel(const JoinArgs a) {
 // db of a piece: columns of dz summed over the labelled rows, blockIdx.y's share of them -> part[y][class].  A thread takes 16 bytes of
 // a row, 32 threads 512 bytes, eight rows at a time.
 constexpr int kBiasRows = 64;          // shares at most
+constexpr int kBiasCols = 256;         // classes of a block
 template <class E>
-__global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__ dz, long long pitch, int classes, const int* __restrict__ count,
-                                                        float* __restrict__ part, typename E::S* __restrict__ db, const float* up, const float* gmax,
-                                                        int mean) {
-    constexpr int V = 16 / E::ES;
+__global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__ dz, long long pitch, long long plane, int classes,
+                                                        const int* __restrict__ count, float* __restrict__ part, typename E::S* __restrict__ db,
+                                                        const float* up, const float* gmax, int mean) {
+    constexpr int V = 8;
     __shared__ float sh[8][32 * V + 1];
     const int N = *count, c = (blockIdx.x * 32 + (threadIdx.x & 31)) * V, w = threadIdx.x >> 5;
     const int r0 = (int)((long long)N * blockIdx.y / gridDim.y), r1 = (int)((long long)N * (blockIdx.y + 1) / gridDim.y);
@@ -897,10 +940,16 @@ __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__
     if (c < classes) {                 // (rows are padded to 16 bytes)
 #pragma unroll 4
         for (int r = r0 + w; r < r1; r += 8) {
-            typedef typename E::S SV __attribute__((ext_vector_type(V)));
-            const SV v = *reinterpret_cast<const SV*>(dz + (long long)r * pitch + (long long)c * E::ES);
+            typedef typename E::O OV __attribute__((ext_vector_type(V)));
+            float t[V];
 #pragma unroll
-            for (int e = 0; e < V; ++e) s[e] += E::get(v[e]);
+            for (int p = E::PLANES - 1; p >= 0; --p) {
+                const OV v = *reinterpret_cast<const OV*>(dz + p * plane + (long long)r * pitch + (long long)c * 2);
+#pragma unroll
+                for (int e = 0; e < V; ++e) t[e] = p == E::PLANES - 1 ? (float)v[e] : t[e] + (float)v[e];
+            }
+#pragma unroll
+            for (int e = 0; e < V; ++e) s[e] += t[e];
         }
     }
 #pragma unroll
@@ -934,19 +983,23 @@ int ceil_div(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 // ---- tiles.  kBig: 256 x 256, eight waves, one block per CU.  kMid: 128 x 128, four waves, two blocks per CU: a quarter of the tile for
 // what kBig leaves unfilled, and its epilogue hides behind the other block.  kSmall: 64 x 64 with three stages in flight: 64 rows x 1000 classes x
-// 512 in 6.0 us against kMid's 9.1, one row x 32000 classes x 1024 in 12.1 against 14.8.
-typedef Tile<256, 256, 2, 4, 128, 2, 1> BigScores;     // waves 2 x 4: a lane's row has 128 classes (32000 x 4096 x 1024 statistics 262 us, 4 x 2: 300)
-typedef Tile<256, 256, 4, 2, 128, 2, 1> BigGrads;      // dx, dW: 4 x 2: 1.20 PFLOP/s, 2 x 4: 1.15 (8192 x 8192 x 2048)
-typedef Tile<128, 128, 2, 2, 128, 2, 2> Mid;           // dx, dW 1.04 PFLOP/s; the same statistics 280 us
-typedef Tile<64, 64, 2, 2, 128, 4, 2> Small;
+// 512 in 6.0 us against kMid's 9.1, one row x 32000 classes x 1024 in 12.1 against 14.8.  The three planes of fp32 fill LDS sooner: one block
+// of 128 x 128 per CU.
+typedef Tile<256, 256, 2, 4, 2, 1> BigScores;     // waves 2 x 4: a lane's row has 128 classes (32000 x 4096 x 1024 statistics 262 us, 4 x 2: 300)
+typedef Tile<256, 256, 4, 2, 2, 1> BigGrads;      // dx, dW: 4 x 2: 1.20 PFLOP/s, 2 x 4: 1.15 (8192 x 8192 x 2048)
+typedef Tile<128, 128, 2, 2, 2, 2> Mid;           // dx, dW 1.04 PFLOP/s; the same statistics 280 us
+typedef Tile<64, 64, 2, 2, 4, 2> Small;
+typedef Tile<128, 128, 2, 4, 3, 1, 192> MidSplit;     // eight waves of 64 x 32: 4096 x 8192 x 2048 with gradients 2.93 ms, four of 64 x 64: 3.21
+typedef Tile<64, 64, 2, 2, 3, 2, 192> SmallSplit;
 enum { kBig, kMid, kSmall, kTiles };
 constexpr int kSide[kTiles] = {256, 128, 64};
-constexpr int kSlots[kTiles] = {256, 512, 512};
+constexpr int kSlots[2][kTiles] = {{256, 512, 512}, {1, 256, 512}};
 constexpr int kWavesM[kTiles] = {BigScores::WM, Mid::WM, Small::WM};
-// microseconds of one 128-byte step of a block, alone on its CU and beside another, and of its first loads and its epilogue (measured,
-// bf16; fp32 steps hold half the values at a sixteenth of the rate, and kBig is no faster than kMid there)
-constexpr double kStepAlone[2][kTiles] = {{1.85, 0.75, 0.38}, {1e9, 2.0, 0.6}};
-constexpr double kStepFull[2][kTiles] = {{1.85, 1.05, 0.5}, {1e9, 3.9, 1.0}};
+static_assert(MidSplit::WM == Mid::WM && SmallSplit::WM == Small::WM, "parts of the statistics");
+// microseconds of one step of a block (64 values of the reduction, of fp32 32), alone on its CU and beside another, and of its first loads
+// and its epilogue (measured)
+constexpr double kStepAlone[2][kTiles] = {{1.85, 0.75, 0.38}, {1e9, 1.35, 0.5}};
+constexpr double kStepFull[2][kTiles] = {{1.85, 1.05, 0.5}, {1e9, 1.4, 1.05}};
 constexpr double kEnds[kTiles] = {4.0, 2.0, 1.5};
 constexpr double kBytesPerUs = 4e6;
 
@@ -959,7 +1012,7 @@ int way_of_scores(bool fp32, long long m, long long n, long long steps) {
     double least = 1e300;
     for (int t = fp32 ? kMid : kBig; t < kTiles; ++t) {
         const long long blocks = (long long)ceil_div(m, kSide[t]) * ceil_div(n, kSide[t]);
-        const double us = ceil_div(blocks, kSlots[t]) * block_us(t, fp32, steps, blocks);
+        const double us = ceil_div(blocks, kSlots[fp32][t]) * block_us(t, fp32, steps, blocks);
         if (us < least) least = us, best = t;
     }
     return best;
@@ -985,7 +1038,7 @@ GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long widt
                     const double u = ux;
                     ux = uw, uw = u, nl = bw, ns = bx;
                 }
-                const long long p = kSlots[t], q = nl / p, r = nl % p;
+                const long long p = kSlots[fp32][t], q = nl / p, r = nl % p;
                 double us;
                 const long long fill = r ? (p - r) * (long long)(ux / uw) : 0;
                 if (ns <= fill) us = (q + (r ? 1 : 0)) * ux;
@@ -1003,11 +1056,11 @@ struct Layout {
     size_t seg, part_m, part_s, part_z, zt, lossc;                                    // forward's workspace
     size_t coef, gmax, dz, accx, accw, bpart;                                         // backward's
     size_t bytes;
-    long long cpitch, np;              // bytes; rows
-    int scores, parts, places, stat_rows, piece, pieces, shares;
+    long long cpitch, np;              // bytes between rows of the gathered features, of the weight's copy; rows
+    int planes, scores, parts, places, stat_rows, piece, pieces, shares;
     GradWay grads;
     long long px, pw;
-    bool pad_w;
+    bool copy_w;                       // the weight is used from a copy: padded, or its planes
 };
 
 Layout layout(const y6_linear_ce_desc* d, bool backward) {
@@ -1021,10 +1074,11 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         at += (bytes + 255) / 256 * 256;
         return o;
     };
-    L.cpitch = up_to(w * es, 16);
-    L.pad_w = (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
-    L.xc = take((size_t)n * L.cpitch);
-    L.wc = take(L.pad_w ? (size_t)v * L.cpitch : 0);
+    L.planes = fp32 ? 3 : 1;
+    L.cpitch = up_to(w * 2, 16);
+    L.copy_w = fp32 || (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
+    L.xc = take((size_t)n * L.cpitch * L.planes);
+    L.wc = take(L.copy_w ? (size_t)v * L.cpitch * L.planes : 0);
     L.rowmap = take((size_t)n * 4);
     L.place = take((size_t)n * 4);
     L.label = take((size_t)n * 4);
@@ -1032,7 +1086,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.count = take(4);
     L.kept = at;
     at = 0;
-    const long long steps = ceil_div(w * es, kRowBytes);
+    const long long steps = ceil_div(w, fp32 ? 32 : 64);
     if (!backward) {
         L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
         L.scores = way_of_scores(fp32, v, n, steps);
@@ -1052,7 +1106,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.lossc = take((size_t)n * 4);
     } else {
         // pieces of equal size, whole tiles, of about kPieceBytes of dz
-        const long long pieces = (long long)(((size_t)n * v * es + kPieceBytes - 1) / kPieceBytes);
+        const long long pieces = (long long)(((size_t)n * v * 2 * L.planes + kPieceBytes - 1) / kPieceBytes);
         long long piece = up_to((v + pieces - 1) / pieces, 256);
         if (piece > v) piece = v;
         L.pieces = ceil_div(v, piece);
@@ -1063,7 +1117,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.shares = n <= 256 ? 1 : n < kBiasRows * 64 ? ceil_div(n, 64) : kBiasRows;
         L.coef = take((size_t)n * 4);
         L.gmax = take(4);
-        L.dz = take((size_t)n * up_to(piece * es, 16));
+        L.dz = take((size_t)n * up_to(piece * 2, 16) * L.planes);
         L.accx = take(d->dx && (L.pieces > 1 || L.grads.split_x > 1) ? (size_t)L.grads.split_x * n * L.px * 4 : 0);
         L.accw = take(d->dw && L.grads.split_w > 1 ? (size_t)L.grads.split_w * piece * L.pw * 4 : 0);
         L.bpart = take(d->dbias ? (size_t)L.shares * piece * 4 : 0);
@@ -1104,8 +1158,8 @@ int launch_gather(const Run& r) {
     GatherArgs a = {};
     a.x = (const char*)d->x, a.pitch = d->x_pitch * E::ES, a.target = d->target, a.ignore = d->ignore_index;
     a.rows = (int)d->rows, a.width = d->width, a.classes = d->classes;
-    a.vec = (d->width * E::ES) % 16 == 0 && a.pitch % 16 == 0 && (uintptr_t)d->x % 16 == 0;
-    a.xc = r.kept<char>(r.L.xc), a.cpitch = r.L.cpitch;
+    a.vec = (E::ES == 4 || (d->width * E::ES) % 16 == 0) && a.pitch % 16 == 0 && (uintptr_t)d->x % 16 == 0;
+    a.xc = r.kept<char>(r.L.xc), a.cpitch = r.L.cpitch, a.plane = d->rows * r.L.cpitch;
     a.rowmap = r.kept<int>(r.L.rowmap), a.place = r.kept<int>(r.L.place), a.label = r.kept<int>(r.L.label), a.count = r.kept<int>(r.L.count);
     const int segs = ceil_div(d->rows, kGatherRows);
     if (d->rows > kCountRows) {
@@ -1116,10 +1170,15 @@ int launch_gather(const Run& r) {
     if (d->reduction == Y6_REDUCE_NONE) a.loss_rows = d->loss;
     hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(kGatherThreads), 0, r.s, a);
     Y6_LAUNCH_CHECK();
-    if (r.L.pad_w) {
-        const long long blocks = ceil_div(d->classes * (r.L.cpitch / 16), 256);
-        hipLaunchKernelGGL(pad_kernel<E::ES>, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes,
-                           d->width, r.kept<char>(r.L.wc), r.L.cpitch);
+    if (r.L.copy_w) {
+        const long long blocks = (d->classes * (r.L.cpitch / (E::ES == 4 ? 8 : 16)) + 255) / 256;
+        const dim3 grid((unsigned)(blocks < 8192 ? blocks : 8192));
+        const int vec = (d->w_pitch * E::ES) % 16 == 0 && (uintptr_t)d->weight % 16 == 0;
+        if (E::ES == 4)
+            hipLaunchKernelGGL(split_kernel, grid, dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes, d->width, vec, r.kept<char>(r.L.wc),
+                               r.L.cpitch, d->classes * r.L.cpitch);
+        else
+            hipLaunchKernelGGL(pad_kernel, grid, dim3(256), 0, r.s, (const char*)d->weight, d->w_pitch * E::ES, d->classes, d->width, r.kept<char>(r.L.wc), r.L.cpitch);
         Y6_LAUNCH_CHECK();
     }
     return Y6_OK;
@@ -1172,11 +1231,11 @@ int launch_scores_tile(GemmArgs& g, hipStream_t s) {
 }
 template <class E, int EPI>
 int launch_scores(int tile, GemmArgs& g, hipStream_t s) {
-    if (tile == kSmall) return launch_scores_tile<E, Small, EPI>(g, s);
-    if constexpr (E::ES == 2) {
-        if (tile == kBig) return launch_scores_tile<E, BigScores, EPI>(g, s);
+    if constexpr (E::PLANES == 3) {
+        return tile == kSmall ? launch_scores_tile<E, SmallSplit, EPI>(g, s) : launch_scores_tile<E, MidSplit, EPI>(g, s);
+    } else {
+        return tile == kSmall ? launch_scores_tile<E, Small, EPI>(g, s) : tile == kMid ? launch_scores_tile<E, Mid, EPI>(g, s) : launch_scores_tile<E, BigScores, EPI>(g, s);
     }
-    return launch_scores_tile<E, Mid, EPI>(g, s);
 }
 template <class E, class T>
 int launch_grads_tile(GemmArgs* x, GemmArgs* w, hipStream_t s) {
@@ -1195,11 +1254,11 @@ int launch_grads_tile(GemmArgs* x, GemmArgs* w, hipStream_t s) {
 }
 template <class E>
 int launch_grads(int tile, GemmArgs* x, GemmArgs* w, hipStream_t s) {
-    if (tile == kSmall) return launch_grads_tile<E, Small>(x, w, s);
-    if constexpr (E::ES == 2) {
-        if (tile == kBig) return launch_grads_tile<E, BigGrads>(x, w, s);
+    if constexpr (E::PLANES == 3) {
+        return tile == kSmall ? launch_grads_tile<E, SmallSplit>(x, w, s) : launch_grads_tile<E, MidSplit>(x, w, s);
+    } else {
+        return tile == kSmall ? launch_grads_tile<E, Small>(x, w, s) : tile == kMid ? launch_grads_tile<E, Mid>(x, w, s) : launch_grads_tile<E, BigGrads>(x, w, s);
     }
-    return launch_grads_tile<E, Mid>(x, w, s);
 }
 
 #define Y6_TRY(expr)                     \
@@ -1214,9 +1273,10 @@ int forward(const Run& r) {
     const Layout& L = r.L;
     Y6_TRY(launch_gather<E>(r));
     GemmArgs g = {};
-    g.a = L.pad_w ? r.kept<char>(L.wc) : (const char*)d->weight;
-    g.pa = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
+    g.a = L.copy_w ? r.kept<char>(L.wc) : (const char*)d->weight;
+    g.pa = L.copy_w ? L.cpitch : d->w_pitch * E::ES;
     g.pb = L.cpitch;
+    g.la = d->classes * L.cpitch, g.lb = d->rows * L.cpitch;
     g.M = d->classes, g.K = d->width;
     g.count = r.kept<int>(L.count), g.bias = d->bias;
     g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
@@ -1262,24 +1322,24 @@ int backward(const Run& r) {
         gmax = r.at<float>(L.gmax), coef = r.at<float>(L.coef);
     }
     const int mean = d->reduction == Y6_REDUCE_MEAN ? 1 : 0;
-    const char* const w = L.pad_w ? r.kept<char>(L.wc) : (const char*)d->weight;
-    const long long wp = L.pad_w ? L.cpitch : d->w_pitch * E::ES;
+    const char* const w = L.copy_w ? r.kept<char>(L.wc) : (const char*)d->weight;
+    const long long wp = L.copy_w ? L.cpitch : d->w_pitch * E::ES, wl = d->classes * L.cpitch, xl = d->rows * L.cpitch;
     char* const dz = r.at<char>(L.dz);
     const bool accx = L.pieces > 1 || L.grads.split_x > 1;
     const int split_x = L.grads.split_x, split_w = L.grads.split_w;
     for (int p = 0; p < L.pieces; ++p) {
         const int v0 = p * L.piece, vn = d->classes - v0 < L.piece ? d->classes - v0 : L.piece;
         GemmArgs g = {};
-        g.a = w + v0 * wp, g.pa = wp, g.b = r.kept<char>(L.xc), g.pb = L.cpitch;
+        g.a = w + v0 * wp, g.pa = wp, g.la = wl, g.b = r.kept<char>(L.xc), g.pb = L.cpitch, g.lb = xl;
         g.M = vn, g.N = (int)d->rows, g.K = d->width, g.count = count;
         g.label = r.kept<int>(L.label), g.bias = d->bias, g.class0 = v0;
         g.lsec = r.kept<float>(L.lsec), g.coef = coef;
         g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
-        g.dz = dz, g.dz_pitch = up_to((long long)vn * E::ES, 16);
+        g.dz = dz, g.dz_pitch = up_to((long long)vn * 2, 16), g.dz_plane = d->rows * g.dz_pitch;
         Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
         if (d->dbias) {
             auto* const db = (typename E::S*)d->dbias + v0;
-            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, 32 * (16 / E::ES)), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, vn, count,
+            hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, kBiasCols), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, g.dz_plane, vn, count,
                                r.at<float>(L.bpart), L.shares == 1 ? db : nullptr, d->grad_out, gmax, mean);
             Y6_LAUNCH_CHECK();
             if (L.shares > 1) {
@@ -1289,7 +1349,7 @@ int backward(const Run& r) {
             }
         }
         GemmArgs x = {}, y = {};
-        x.a = w + v0 * wp, x.pa = wp, x.b = dz, x.pb = g.dz_pitch;
+        x.a = w + v0 * wp, x.pa = wp, x.la = wl, x.b = dz, x.pb = g.dz_pitch, x.lb = g.dz_plane;
         x.M = d->width, x.N = (int)d->rows, x.K = vn, x.count = count, x.splits = split_x;
         x.up = d->grad_out, x.gmax = gmax, x.mean = mean;
         if (accx) {
@@ -1298,7 +1358,7 @@ int backward(const Run& r) {
             x.out = (char*)d->dx, x.out_pitch = d->width, x.rowmap = r.kept<int>(L.rowmap), x.place = place;
             x.vec = d->width % 4 == 0 && (uintptr_t)d->dx % (4 * E::ES) == 0;
         }
-        y.a = r.kept<char>(L.xc), y.pa = L.cpitch, y.b = dz, y.pb = g.dz_pitch;
+        y.a = r.kept<char>(L.xc), y.pa = L.cpitch, y.la = xl, y.b = dz, y.pb = g.dz_pitch, y.lb = g.dz_plane;
         y.M = d->width, y.N = vn, y.K = (int)d->rows, y.count = count, y.splits = split_w;
         y.up = d->grad_out, y.gmax = gmax, y.mean = mean;
         char* const dw = (char*)d->dw + (long long)v0 * d->width * E::ES;
