@@ -441,3 +441,39 @@ def test_a_weight_beyond_4_gigabytes():
         spread += part.abs() @ w.detach()[k:k + 10000].double().abs()
     assert bool(((dx[:4].double() - want).abs() <= 1.01 * (u * spread + u * want.abs() + 2 * err * spread + v * 2.0 ** -24 * spread)).all())
     assert int(dx[4].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("top", [1.0, 30.0, 1000.0])
+def test_small_losses_of_large_logits(top):
+    """A label far above the others: the loss is log(1 + sum exp(z - z_t)), whatever z_t is.  Logits are exact here (one feature, values of few
+    bits): the sum of exponentials is off by 4 * 2^-24 of itself or so, the loss by that."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    for classes in (3, 100, 5000):
+        w = torch.full((classes, 1), top - 8.0, device=DEV)
+        w[7 % classes] = top
+        x, t = torch.ones((2, 1), device=DEV), torch.tensor([7 % classes, 0], device=DEV)
+        got = linear_cross_entropy(x, w, t, reduction="none")
+        want = torch.log1p((classes - 1) * torch.exp(torch.tensor(-8.0, dtype=torch.float64)))
+        assert abs(float(got[0]) - float(want)) <= 8 * 2.0 ** -24 * (1 + float(want)), classes
+        assert abs(float(got[1]) - float(want) - (0 if 7 % classes == 0 else 8.0)) <= 8 * 2.0 ** -24 * (9 + float(want))
+
+
+@pytest.mark.parametrize("smooth", [0.0, 0.1])
+@pytest.mark.parametrize("top", [1.0, 30.0, 1000.0])
+def test_gradients_of_rows_that_are_almost_right(top, smooth):
+    """p - 1 of the label is minus the others' share, which is small and keeps its digits; exact logits as above.  The share is a quotient of sums
+    (8 * 2^-24 of itself at most), the smoothing's terms add two roundings of 0.1 at most."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    for classes in (3, 100, 5000):
+        w = torch.full((classes, 1), top - 12.0, device=DEV)
+        w[2] = top
+        w.requires_grad_()
+        linear_cross_entropy(torch.ones((1, 1), device=DEV), w, torch.tensor([2], device=DEV), label_smoothing=smooth, reduction="sum").backward()
+        z = w.detach().double().cpu().flatten()
+        p = torch.softmax(z, 0)
+        want = p - smooth / classes
+        want[2] = -(torch.exp(z[0] - z[2]) * (classes - 1) * p[2]) + smooth - smooth / classes
+        off = (w.grad.double().cpu().flatten() - want).abs()
+        bound = 16 * 2.0 ** -24 * p + 4 * 2.0 ** -24 * smooth
+        bound[2] = 16 * 2.0 ** -24 * (1 - p[2]).abs() + 4 * 2.0 ** -24 * smooth
+        assert bool((off <= bound + 1e-30).all()), (classes, off.max(), want[:4])

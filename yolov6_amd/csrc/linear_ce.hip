@@ -32,7 +32,7 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
 constexpr size_t kPieceBytes = (size_t)128 << 20;     // of dz: half the last-level cache, and tiles enough to fill the chip
 constexpr size_t kPartBytes = (size_t)256 << 20;      // of the tiles' statistics: the forward takes the rows in as many pieces
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kLog2e = 1.44269504088896340736f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
 // adds nothing that fp16 gradients show.  bf16 and fp32 have the range.
 constexpr float kHalfScale = 16384.f;
@@ -342,19 +342,27 @@ __device__ __forceinline__ void sub_step(f32x16_t (&acc)[FM][FN], const char* ia
 enum { EPI_STATS, EPI_DZ };
 enum { COUNT_N, COUNT_K };
 
+// What the backward pass needs of a row's softmax: p_j = 2^((z_j - top) log2 e - log2s), s = sum exp(z_j - top), and 1 - p of the label from
+// the others' sum.  Neither the loss, log(1 + sum over the others of exp(z_j - z_label)) where the label is the largest, nor its gradient
+// p - 1 is a difference of large numbers then: a row that is almost right keeps its digits, at logits of any size.
+struct RowStat {
+    float top, log2s, miss;
+};
+
 struct GemmArgs {
     const char *a, *b;
     long long pa, pb, la, lb;      // bytes between rows, between planes
     int M, N, K;
     const int* count;              // labelled rows: the extent that COUNT says
-    int row0;                      // scores: the first of these rows (b, label, lsec ... start there)
+    int row0;                      // scores: the first of these rows (b, label, stat ... start there)
     int tiles_m, tiles_n, splits;
     // EPI_STATS, EPI_DZ: m = class, n = labelled row
     const void* bias;
     const int* label;
     float *part_m, *part_s, *part_z, *zt;
     long long np;                  // rows of the partial statistics' arrays
-    const float *lsec, *coef;      // log2 of the sum of exponentials; g_n / max |g| (null: 1)
+    const RowStat* stat;
+    const float* coef;             // g_n / max |g| (null: 1)
     float smooth, smooth_share;    // e, e / V
     int class0;                    // first class of the piece
     char* dz;
@@ -642,6 +650,7 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                 const int n = nw + j * 32 + l31;
                 const bool live = n < N;
                 const long long o = (long long)(tm * WM + wm) * e.np + n;
+                const int lab = live ? e.label[n] - mw : -1;
                 int left = e.M - mw - 4 * half;              // classes of this lane's 4-runs: 32 i + 8 (q >> 2) + (q & 3) < left
                 if (e.part_z) {
                     float zsum = 0.f;
@@ -665,27 +674,8 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                             if (i * 32 + 8 * (q >> 2) + (q & 3) >= left) acc[i][j][q] = -INFINITY;
                     }
                 }
-                float top = acc[0][j][0];
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
-                top = fmaxf(top, __shfl_xor(top, 32));
-                // sums are relative to 2^m2; a tile whose classes are all at -infinity says m2 = -infinity, sum 0
-                const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < FM; ++i)
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
-                float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                all += __shfl_xor(all, 32);
-                if (live && half == 0) {
-                    e.part_m[o] = top == -INFINITY ? -INFINITY : m2;
-                    e.part_s[o] = all;
-                }
-                const int lab = live ? e.label[n] - mw : -1;
                 if (__ballot(lab >= 0 && lab < BM / WM)) {   // a label of these rows lies in this tile: few do
+                    // its logit is handed on by itself and left out of the sum (RowStat)
                     int mine = lab - 4 * half;
                     asm volatile("" : "+v"(mine));
                     float z = 0.f;
@@ -696,6 +686,33 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                         for (int q = 0; q < 16; ++q) z = mine == i * 32 + 8 * (q >> 2) + (q & 3) ? acc[i][j][q] : z;
                     }
                     if (mine >= 0 && mine < BM / WM && (mine & 4) == 0) e.zt[n] = z;
+                    asm volatile("" : "+v"(mine));
+#pragma unroll
+                    for (int i = 0; i < FM; ++i) {
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) acc[i][j][q] = mine == i * 32 + 8 * (q >> 2) + (q & 3) ? -INFINITY : acc[i][j][q];
+                    }
+                }
+                float top = acc[0][j][0];
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
+                top = fmaxf(top, __shfl_xor(top, 32));
+                // a tile says its largest logit and the sum of exp(z - it); one whose classes are all at -infinity says -infinity, 0
+                const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < FM; ++i)
+#pragma unroll
+                    for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
+                float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                all += __shfl_xor(all, 32);
+                if (live && half == 0) {
+                    e.part_m[o] = top;
+                    // (m2 was rounded: the terms are relative to it, the sum is not)
+                    e.part_s[o] = top == -INFINITY ? 0.f : all * exp2_fast(-fmaf(top, kLog2e, -m2));
                 }
             }
         } else if constexpr (EPI == EPI_DZ) {
@@ -704,9 +721,9 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                 const int n = nw + j * 32 + l31;
                 const bool live = n < N;
                 const int nl = live ? n : N - 1;
-                const float l2 = e.lsec[nl];
+                const float zmax = e.stat[nl].top, log2s = e.stat[nl].log2s;
                 const float c = (e.coef ? e.coef[nl] : 1.f) * E::kScale;
-                const float share = -e.smooth_share * c, hit = (1.f - e.smooth) * c;
+                const float share = -e.smooth_share * c, own = fmaf(-e.stat[nl].miss, c, fmaf(e.smooth, c, share));
                 const int lab = e.label[nl] - e.class0 - mw - 4 * half;
                 char* const row = e.dz + (long long)n * e.dz_pitch + (long long)(mw + 4 * half) * 2;
                 const int left = e.M - mw - 4 * half;
@@ -725,8 +742,8 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
 #pragma unroll
                                 for (int c4 = 0; c4 < 4; ++c4) {
                                     const int m = i * 32 + 16 * gp + 8 * k + c4;
-                                    float d = fmaf(exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + c4], kLog2e, -l2)), c, share);
-                                    if (labelled.value) d -= m == at ? hit : 0.f;
+                                    float d = fmaf(exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + c4] - zmax, kLog2e, -log2s)), c, share);
+                                    if (labelled.value) d = m == at ? own : d;
                                     v[k][c4] = d;
                                 }
                             uint2 a[E::PLANES], b[E::PLANES];
@@ -792,7 +809,7 @@ struct FinishArgs {
     int parts, places, row0, rows; // of the labelled rows those from row0 on, `rows` of them (the pointers start there)
     const int *rowmap, *label, *count;
     float smooth, smooth_share;
-    float* lsec;                   // by place: log2 of the sum of exponentials
+    RowStat* stat;                 // by place
     float* rows_out;               // by row (reduction none) or null
     float* lossc;                  // by place, unless this is the only block
     float* loss;                   // the only block: the sum, or the mean
@@ -803,7 +820,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     const int i = threadIdx.x & (a.places - 1), sl = threadIdx.x / a.places;
     int slices = 1024 / a.places;
     const int n = blockIdx.x * a.places + i, N = *a.count - a.row0 < a.rows ? *a.count - a.row0 : a.rows;
-    float m = -INFINITY, s = 0.f, z = 0.f, zt = 0.f;
+    float m = -INFINITY, s = 0.f, z = 0.f, zt = 0.f;      // largest logit but the label's; sum of exp(logit - m), the label's left out
     int label = 0, row = 0;
     if (n < N) {
         if (sl == 0) {                 // (asked for early: they are needed behind the last barrier)
@@ -815,7 +832,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
             const float pm = a.part_m[(long long)p * a.np + n], ps = a.part_s[(long long)p * a.np + n];
             if (a.part_z) z += a.part_z[(long long)p * a.np + n];
             const float nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
-            s = s * exp2_fast(m - ref) + ps * exp2_fast(pm - ref);
+            s = s * exp2_fast((m - ref) * kLog2e) + ps * exp2_fast((pm - ref) * kLog2e);
             m = nm;
         }
     }
@@ -825,7 +842,7 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
         if (sl < slices / 2) {
             const int o = threadIdx.x + slices / 2 * a.places;
             const float pm = sm[o], nm = fmaxf(m, pm), ref = nm == -INFINITY ? 0.f : nm;
-            s = s * exp2_fast(m - ref) + ss[o] * exp2_fast(pm - ref);
+            s = s * exp2_fast((m - ref) * kLog2e) + ss[o] * exp2_fast((pm - ref) * kLog2e);
             z += sz[o];
             m = nm;
             sm[threadIdx.x] = m, ss[threadIdx.x] = s, sz[threadIdx.x] = z;
@@ -834,12 +851,11 @@ __global__ __launch_bounds__(1024) void finish_kernel(const FinishArgs a) {
     __syncthreads();
     float loss = 0.f;
     if (sl == 0 && n < N) {
-        // (every class at -infinity: log2(0) = -infinity, and the loss -infinity - -infinity is a NaN)
-        float l2 = (m == -INFINITY ? 0.f : m) + log2_fast(s);
-        loss = l2 * kLn2 - (1.f - a.smooth) * zt;
-        if (a.smooth > 0.f) loss -= a.smooth_share * z;
-        if (label < 0) l2 = loss = NAN;        // a label that is no class
-        a.lsec[n] = l2;
+        const float top = fmaxf(m, zt), rest = s * exp2_fast((m - top) * kLog2e), own = exp2_fast((zt - top) * kLog2e), sum = rest + own;
+        loss = zt >= m ? log1pf(rest) * own : (m - zt) + logf(sum);      // (own is 1 there, or a NaN)
+        if (a.smooth > 0.f) loss = (1.f - a.smooth) * loss + (a.smooth * (top + logf(sum)) - a.smooth_share * z);
+        if (label < 0) loss = NAN;             // a label that is no class
+        a.stat[n] = {top, label < 0 ? NAN : log2_fast(sum), rest / sum};
         if (a.rows_out) a.rows_out[row] = loss;
         if (a.lossc) a.lossc[n] = loss;
     }
@@ -1052,7 +1068,7 @@ GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long widt
 }
 
 struct Layout {
-    size_t xc, wc, rowmap, place, label, count, lsec, kept;                           // what the backward takes over from the forward
+    size_t xc, wc, rowmap, place, label, count, stat, kept;                           // what the backward takes over from the forward
     size_t seg, part_m, part_s, part_z, zt, lossc;                                    // forward's workspace
     size_t coef, gmax, dz, accx, accw, bpart;                                         // backward's
     size_t bytes;
@@ -1082,7 +1098,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.rowmap = take((size_t)n * 4);
     L.place = take((size_t)n * 4);
     L.label = take((size_t)n * 4);
-    L.lsec = take((size_t)n * 4);
+    L.stat = take((size_t)n * sizeof(RowStat));
     L.count = take(4);
     L.kept = at;
     at = 0;
@@ -1295,7 +1311,7 @@ int forward(const Run& r) {
         g.zt = r.at<float>(L.zt) + n0, f.zt = g.zt;
         Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
         f.rowmap = r.kept<int>(L.rowmap) + n0;
-        f.lsec = r.kept<float>(L.lsec) + n0;
+        f.stat = r.kept<RowStat>(L.stat) + n0;
         if (!sums) f.rows_out = d->loss;
         else if (alone) f.loss = d->loss;
         else f.lossc = r.at<float>(L.lossc) + n0;
@@ -1333,7 +1349,7 @@ int backward(const Run& r) {
         g.a = w + v0 * wp, g.pa = wp, g.la = wl, g.b = r.kept<char>(L.xc), g.pb = L.cpitch, g.lb = xl;
         g.M = vn, g.N = (int)d->rows, g.K = d->width, g.count = count;
         g.label = r.kept<int>(L.label), g.bias = d->bias, g.class0 = v0;
-        g.lsec = r.kept<float>(L.lsec), g.coef = coef;
+        g.stat = r.kept<RowStat>(L.stat), g.coef = coef;
         g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
         g.dz = dz, g.dz_pitch = up_to((long long)vn * 2, 16), g.dz_plane = d->rows * g.dz_pitch;
         Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
