@@ -98,7 +98,7 @@ def build_torch_host(force=False, verbose=True):
     if not force and os.path.exists(TORCH_HOST) and os.path.exists(mark) and open(mark).read() == tag:
         return TORCH_HOST
     cmd = (["g++"] + flags + [a for i in dict.fromkeys(include) for a in ("-isystem", i)] +
-           [os.path.join(HERE, "torch_host.cpp"), "-o", TORCH_HOST, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip"])
+           [os.path.join(HERE, "torch_host.cpp"), "-o", TORCH_HOST, "-L" + libs, "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-L" + os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "lib"), "-lamdhip64"])
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"g++ failed for torch_host.cpp:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")

@@ -5,14 +5,16 @@
 //   dz_nv = g_n (exp(z_nv - lse_n) - (1-e) [v = t(n)] - e/V)
 //   dx = dz W       dW = dz^T x      db = sum_n dz_n
 //
-// Four matrix products, all of the time at sizes that matter; the matrix cores bound them:
-//   forward     z = W x^T tile by tile (scores_kernel); the epilogue leaves a running maximum and a sum of exponentials per row and tile
-//   backward    for a piece of the vocabulary: z again, its epilogue turns it into dz (16 bits for 16-bit inputs: the operand the
-//               matrix instructions of the next two products take, one rounding), then dx += dz W[piece] and dW[piece] = dz^T x
-//               in one launch (gemm_tile)
-// so memory holds one piece of dz (kPieceBytes), never the logits, and a product of 2 N V D operations is done twice: 8 N V D where 6 would
-// do with all logits kept.  8192 rows x 131072 classes x 1024, bf16: 8.0 ms, 1.10 PFLOP/s over the four; torch's product of such
-// operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on the same card, which lowers its clock under either.
+// Matrix products, all of the time at sizes that matter; the matrix cores bound them:
+//   forward     z = W x^T tile by tile (scores_kernel); the epilogue leaves a running maximum and a sum of exponentials per row and tile and,
+//               for training with 16-bit types, the exponentials in 16 bits (kKeepBytes)
+//   backward    for a piece of the vocabulary: dz from the kept exponentials (kept_kernel, a memory pass) or, where there are none, from z
+//               formed again; 16 bits for 16-bit inputs, the operand that the matrix instructions of the next two products take.  Then
+//               dx += dz W[piece] and dW[piece] = dz^T x in one launch (gemm_tile)
+// so a call holds one piece of dz (kPieceBytes) and what is kept, never the logits.  A kept exponential is rounded to 16 bits and dz once
+// more (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9 ms, 0.95
+// PFLOP/s over the three products; without the kept ones 8.1.  torch's product of such operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on
+// the same card, which lowers its clock under either.
 // Labelled rows are gathered first (gather_kernel): rows with ignore_index cost nothing, and an infinity or a NaN in one of them reaches no
 // gradient.  What the forward gathered, and its statistics, are kept for the backward.
 //
@@ -31,11 +33,19 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
 constexpr size_t kPieceBytes = (size_t)128 << 20;     // of dz: half the last-level cache, and tiles enough to fill the chip
+// Training keeps the forward's exponentials, 16 bits each, instead of forming the scores again, while they take at most kKeepBytes (below 1 %
+// of the card's memory); what is behind that, by whole pieces, is formed again.
+constexpr size_t kKeepBytes = (size_t)2 << 30;
+// Measured with bf16 gradients and bias, formed again against kept: 4096 rows x 16000 classes x 128 wide 207 -> 196 us, 256 249 -> 226, 384
+// 320 -> 281, 8192 x 32000 x 64 645 -> 663; few classes leave lanes empty, 20000 x 600 x 256 111 -> 113; few scores are latency, 512 x 1000 x 512
+// 45.7 -> 47.1, 1024 x 4001 x 256 61.8 -> 59.3.
+constexpr long long kKeepWidth = 128, kKeepClasses = 1024, kKeepScores = 1 << 22;
 constexpr size_t kPartBytes = (size_t)256 << 20;      // of the tiles' statistics: the forward takes the rows in as many pieces
 constexpr float kLog2e = 1.44269504088896340736f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
 // adds nothing that fp16 gradients show.  bf16 and fp32 have the range.
 constexpr float kHalfScale = 16384.f;
+// Kept exponentials are relative to the largest of their tile; fp16 ones times 2^15, normal down to 2^-29 of it.
 
 // Types: S of the caller's tensors; PLANES 16-bit operands (O) that stand for one value in LDS, RB bytes of each plane that a step takes
 // from a row.  fp32 goes as three bf16 planes, h = the upper 8 significant bits, m = the next 8, l = the last 8: their sum is the value,
@@ -43,7 +53,7 @@ constexpr float kHalfScale = 16384.f;
 // the fp32 ones take for the one.
 struct Half {
     static constexpr int ES = 2, TYPE = Y6_F16, PLANES = 1, RB = 128;
-    static constexpr float kScale = kHalfScale;
+    static constexpr float kScale = kHalfScale, kKeepExp = 15.f, kKeepUnit = 1.f / 32768;
     typedef _Float16 S;
     typedef _Float16 O;
     static __device__ __forceinline__ float get(S v) { return (float)v; }
@@ -51,7 +61,7 @@ struct Half {
 };
 struct Brain {
     static constexpr int ES = 2, TYPE = Y6_BF16, PLANES = 1, RB = 128;
-    static constexpr float kScale = 1.f;
+    static constexpr float kScale = 1.f, kKeepExp = 0.f, kKeepUnit = 1.f;
     typedef __bf16 S;
     typedef __bf16 O;
     static __device__ __forceinline__ float get(S v) { return (float)v; }
@@ -59,7 +69,7 @@ struct Brain {
 };
 struct Single {
     static constexpr int ES = 4, TYPE = Y6_F32, PLANES = 3, RB = 64;
-    static constexpr float kScale = 1.f;
+    static constexpr float kScale = 1.f, kKeepExp = 0.f, kKeepUnit = 1.f;
     typedef float S;
     typedef __bf16 O;
     static __device__ __forceinline__ float get(S v) { return v; }
@@ -339,7 +349,7 @@ __device__ __forceinline__ void sub_step(f32x16_t (&acc)[FM][FN], const char* ia
                 for (int j = 0; j < FN; ++j) acc[i][j] = mma<E>(fa[p][i], fb[order - p][j], acc[i][j]);
 }
 
-enum { EPI_STATS, EPI_DZ };
+enum { EPI_STATS, EPI_KEEP, EPI_DZ };
 enum { COUNT_N, COUNT_K };
 
 // What the backward pass needs of a row's softmax: p_j = 2^((z_j - top) log2 e - log2s), s = sum exp(z_j - top), and 1 - p of the label from
@@ -356,7 +366,7 @@ struct GemmArgs {
     const int* count;              // labelled rows: the extent that COUNT says
     int row0;                      // scores: the first of these rows (b, label, stat ... start there)
     int tiles_m, tiles_n, splits;
-    // EPI_STATS, EPI_DZ: m = class, n = labelled row
+    // scores: m = class, n = labelled row
     const void* bias;
     const int* label;
     float *part_m, *part_s, *part_z, *zt;
@@ -365,6 +375,9 @@ struct GemmArgs {
     const float* coef;             // g_n / max |g| (null: 1)
     float smooth, smooth_share;    // e, e / V
     int class0;                    // first class of the piece
+    char* keep;                    // EPI_KEEP: exponentials of the classes below `keeps`, by row
+    long long keep_pitch;          // bytes
+    int keeps;
     char* dz;
     long long dz_pitch, dz_plane;  // bytes
     // products into a gradient: m = column, n = row of the output
@@ -644,7 +657,7 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                     for (int j = 0; j < FN; ++j) acc[i][j][q] += b;
                 }
         }
-        if constexpr (EPI == EPI_STATS) {
+        if constexpr (EPI != EPI_DZ) {
 #pragma unroll
             for (int j = 0; j < FN; ++j) {
                 const int n = nw + j * 32 + l31;
@@ -701,18 +714,52 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                     for (int q = 0; q < 16; ++q) top = fmaxf(top, acc[i][j][q]);
                 top = fmaxf(top, __shfl_xor(top, 32));
                 // a tile says its largest logit and the sum of exp(z - it); one whose classes are all at -infinity says -infinity, 0
-                const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                float all;
+                if (EPI == EPI_KEEP && tm * BM < e.keeps) {
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    char* const row = e.keep + (long long)n * e.keep_pitch + (long long)(mw + 4 * half) * 2;
+                    int end16 = (int)(e.keep_pitch / 2) - mw - 4 * half;
+                    asm volatile("" : "+v"(end16));
 #pragma unroll
-                for (int i = 0; i < FM; ++i)
+                    for (int i = 0; i < FM; ++i)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
-                float all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                all += __shfl_xor(all, 32);
+                        for (int gp = 0; gp < 2; ++gp) {
+                            __builtin_amdgcn_sched_barrier(0);
+                            float v[2][4];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                                for (int c4 = 0; c4 < 4; ++c4) {
+                                    v[k][c4] = exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + c4] - ref, kLog2e, E::kKeepExp));
+                                    sum[c4] += v[k][c4];
+                                }
+                            uint2 a[E::PLANES], b[E::PLANES];
+                            pack4<E>(v[0], a);
+                            pack4<E>(v[1], b);
+                            const auto x = __builtin_amdgcn_permlane32_swap(a[0].x, b[0].x, false, false);
+                            const auto y = __builtin_amdgcn_permlane32_swap(a[0].y, b[0].y, false, false);
+                            // (as dz: sixteen bytes a lane; the row is padded to them, and classes behind the last are zeros)
+                            if (live && i * 32 + 16 * gp + 4 * half < end16)
+                                *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+                        }
+                    all = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * E::kKeepUnit;
+                    all += __shfl_xor(all, 32);
+                } else {
+                    const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int i = 0; i < FM; ++i)
+#pragma unroll
+                        for (int q = 0; q < 16; ++q) sum[q & 3] += exp2_fast(fmaf(acc[i][j][q], kLog2e, -m2));
+                    all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    all += __shfl_xor(all, 32);
+                    // (m2 was rounded: the terms are relative to it, the sum is not)
+                    all = top == -INFINITY ? 0.f : all * exp2_fast(-fmaf(top, kLog2e, -m2));
+                }
                 if (live && half == 0) {
                     e.part_m[o] = top;
-                    // (m2 was rounded: the terms are relative to it, the sum is not)
-                    e.part_s[o] = top == -INFINITY ? 0.f : all * exp2_fast(-fmaf(top, kLog2e, -m2));
+                    e.part_s[o] = all;
                 }
             }
         } else if constexpr (EPI == EPI_DZ) {
@@ -981,6 +1028,75 @@ __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__
         else part[(long long)blockIdx.y * classes + col] = t;
     }
 }
+// dz of a piece from the exponentials that the forward kept: dz = c (e 2^((tile's largest - top) log2 e - log2s) - share), the label's from
+// its RowStat.  A wave takes 512 classes, 16 bytes a lane, and 16 rows, four at a time, so that it also has their sum, which becomes db: the
+// block adds its four waves', in order.  Memory bounds it: 128 MB to 128 MB in 53 us, 4.9 TB/s, where forming the scores of 1024 features again
+// took 150.  (32 rows a wave: 37 instead of 31 us at 1383 x 25088.)
+constexpr int kKeptRows = 16, kKeptCols = 512;
+struct KeptArgs {
+    const char* e;                 // the piece's first class
+    long long e_pitch;
+    const float* part_m;           // [row piece][part][np]
+    long long np;
+    int parts, part_shift, stat_rows;
+    const RowStat* stat;
+    const float* coef;
+    const int *label, *count;
+    float smooth, smooth_share;
+    int class0, classes, col_blocks;
+    char* dz;
+    long long dz_pitch;
+    float* bpart;                  // [block of rows][classes] or null
+};
+template <class E>
+__global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
+    __shared__ float sh[4][8][64];
+    typedef typename E::O O8 __attribute__((ext_vector_type(8)));
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int bx = blockIdx.x % a.col_blocks, by = blockIdx.x / a.col_blocks;
+    const int N = *a.count, c0 = bx * kKeptCols + lane * 8, n0 = (by * 4 + wave) * kKeptRows;
+    const bool mine = c0 * 2 < a.dz_pitch;
+    const int part = (a.class0 + (mine ? c0 : 0)) >> a.part_shift;
+    float sum[8] = {};
+    constexpr int U = 4;
+    for (int k = n0; k < n0 + kKeptRows && k < N; k += U) {
+        O8 e[U];
+        float pm[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int n = k + u < N ? k + u : N - 1;
+            e[u] = __builtin_nontemporal_load(reinterpret_cast<const O8*>(a.e + n * a.e_pitch + (mine ? c0 * 2 : 0)));   // (read once: dz stays in the caches)
+            pm[u] = a.part_m[((long long)(n / a.stat_rows) * a.parts + part) * a.np + n % a.stat_rows];
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int n = k + u;
+            if (n >= N) break;
+            const RowStat st = a.stat[n];
+            const float c = (a.coef ? a.coef[n] : 1.f) * E::kScale, share = -a.smooth_share * c;
+            const float f = exp2_fast(fmaf(pm[u] - st.top, kLog2e, -st.log2s - E::kKeepExp)) * c, own = fmaf(-st.miss, c, fmaf(a.smooth, c, share));
+            const int at = a.label[n] - a.class0 - c0;
+            O8 o;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) {
+                float d = fmaf((float)e[u][q], f, share);
+                d = q == at ? own : c0 + q < a.classes ? d : 0.f;
+                sum[q] += d;
+                o[q] = (typename E::O)d;
+            }
+            if (mine) *reinterpret_cast<O8*>(a.dz + n * a.dz_pitch + c0 * 2) = o;
+        }
+    }
+    if (!a.bpart) return;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) sh[wave][q][lane] = sum[q];
+    __syncthreads();
+    for (int i = threadIdx.x; i < kKeptCols; i += 256) {
+        const int c = bx * kKeptCols + i;
+        if (c < a.classes) a.bpart[(long long)by * a.classes + c] = (sh[0][i & 7][i >> 3] + sh[1][i & 7][i >> 3]) + (sh[2][i & 7][i >> 3] + sh[3][i & 7][i >> 3]);
+    }
+}
+
 template <class E>
 __global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
                                                         const float* up, const float* gmax, int mean, const int* count) {
@@ -1035,14 +1151,14 @@ int way_of_scores(bool fp32, long long m, long long n, long long steps) {
 }
 struct GradWay {
     int tile, split_x, split_w;
+    double us;
 };
 // Tile and splits of a piece's dx (width x rows, reduction `classes`) and dW (width x classes, reduction `rows`) in one launch: the long
 // blocks go first, the short ones fill up behind them; splits cost the traffic of their partial products.
 GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long width, long long classes, int pieces) {
     const int ks = fp32 ? 32 : 64;
     const long long kx = ceil_div(classes, ks), kw = ceil_div(rows, ks);
-    GradWay best = {kMid, 1, 1};
-    double least = 1e300;
+    GradWay best = {kMid, 1, 1, 1e300};
     for (int t = fp32 ? kMid : kBig; t < kTiles; ++t)
         for (int sx = 1; sx <= (dx ? 32 : 1) && (sx == 1 || kx / sx >= 4); sx *= 2)
             for (int sw = 1; sw <= (dw ? 32 : 1) && (sw == 1 || kw / sw >= 4); sw *= 2) {
@@ -1062,18 +1178,21 @@ GradWay way_of_grads(bool fp32, bool dx, bool dw, long long rows, long long widt
                 if (dx && (sx > 1 || pieces > 1)) us += (pieces > 1 ? 2.0 : 1.0) * rows * width * 4 * sx / kBytesPerUs;
                 if (dx && sx > 1 && pieces == 1) us += 4 + 1.0 * rows * width * 4 * sx / kBytesPerUs;
                 if (dw && sw > 1) us += 4 + 2.0 * classes * width * 4 * sw / kBytesPerUs;
-                if (us < least) least = us, best = {t, sx, sw};
+                if (us < best.us) best = {t, sx, sw, us};
             }
     return best;
 }
 
 struct Layout {
     size_t xc, wc, rowmap, place, label, count, stat, kept;                           // what the backward takes over from the forward
+    size_t exps, kept_m, kept_all;                                                    // and, if it comes, these
     size_t seg, part_m, part_s, part_z, zt, lossc;                                    // forward's workspace
     size_t coef, gmax, dz, accx, accw, bpart;                                         // backward's
     size_t bytes;
     long long cpitch, np;              // bytes between rows of the gathered features, of the weight's copy; rows
     int planes, scores, parts, places, stat_rows, piece, pieces, shares;
+    int keeps, kept_scores;            // classes whose exponentials are kept (whole pieces), by tiles of this kind
+    long long keep_pitch;              // bytes
     GradWay grads;
     long long px, pw;
     bool copy_w;                       // the weight is used from a copy: padded, or its planes
@@ -1101,32 +1220,55 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.stat = take((size_t)n * sizeof(RowStat));
     L.count = take(4);
     L.kept = at;
-    at = 0;
     const long long steps = ceil_div(w, fp32 ? 32 : 64);
+    // the backward's pieces: of equal size, whole tiles, of about kPieceBytes of dz or, where the blocks of the gradients' products come
+    // out that much more evenly, twice that: the caches then hold less of it (8192 x 131072 x 1024: 7.24 ms, with 256 MB 7.47; 4096 x
+    // 32000: 967 us, in one piece of 262 MB 942)
+    auto cut = [&](long long bytes, int* count, int* size) {
+        const long long pieces = (long long)(((size_t)n * v * 2 * L.planes + bytes - 1) / bytes);
+        const long long piece = up_to((v + pieces - 1) / pieces, 256);
+        *size = (int)(piece < v ? piece : v);
+        *count = ceil_div(v, *size);
+    };
+    cut(kPieceBytes, &L.pieces, &L.piece);
+    if (L.pieces > 1) {
+        int count, size;
+        cut(2 * kPieceBytes, &count, &size);
+        auto us = [&](int count, int size) {
+            return (count - 1) * way_of_grads(fp32, true, true, n, w, size, count).us + way_of_grads(fp32, true, true, n, w, v - (count - 1ll) * size, count).us;
+        };
+        if (1.05 * us(count, size) < us(L.pieces, L.piece)) L.pieces = count, L.piece = size;
+    }
+    const long long piece = L.piece;
+    // the forward's tiles and statistics
+    L.kept_scores = way_of_scores(fp32, v, n, steps);
+    L.parts = ceil_div(v, kSide[L.kept_scores]) * kWavesM[L.kept_scores];
+    long long rows = (long long)(kPartBytes / ((size_t)L.parts * 8)) / 256 * 256;
+    if (rows < 256) rows = 256;
+    L.stat_rows = (int)(rows < n ? rows : n);
+    L.np = up_to(L.stat_rows, 64);
+    if (!fp32 && w >= kKeepWidth && v >= kKeepClasses && n * v >= kKeepScores) {
+        const long long most = (long long)(kKeepBytes / ((size_t)n * piece * 2));
+        L.keeps = (int)(most >= L.pieces ? v : most * piece);
+    }
+    L.keep_pitch = up_to((long long)L.keeps * 2, 16);
+    L.exps = take((size_t)n * L.keep_pitch);
+    L.kept_m = take(L.keeps ? (size_t)ceil_div(n, L.stat_rows) * L.parts * L.np * 4 : 0);
+    L.kept_all = at;
+    at = 0;
     if (!backward) {
         L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
-        L.scores = way_of_scores(fp32, v, n, steps);
-        L.parts = ceil_div(v, kSide[L.scores]) * kWavesM[L.scores];
-        long long rows = (long long)(kPartBytes / ((size_t)L.parts * 8)) / 256 * 256;
-        if (rows < 256) rows = 256;
-        L.stat_rows = (int)(rows < n ? rows : n);
-        L.np = up_to(L.stat_rows, 64);
+        L.scores = L.kept_scores;
         // one block for all rows, which then also adds up the loss, where that is 16 rounds of its threads at most
         L.places = 1;
         while (L.places < n && L.places < 128) L.places *= 2;
         if (L.places < n || (long long)L.places * L.parts > 16 * 1024) L.places = n >= 8192 ? 32 : n >= 64 ? 8 : 1;
-        L.part_m = take((size_t)L.parts * L.np * 4);
+        L.part_m = take(d->saved && L.keeps ? 0 : (size_t)L.parts * L.np * 4);
         L.part_s = take((size_t)L.parts * L.np * 4);
         L.part_z = take(d->smoothing > 0.f ? (size_t)L.parts * L.np * 4 : 0);
         L.zt = take((size_t)n * 4);
         L.lossc = take((size_t)n * 4);
     } else {
-        // pieces of equal size, whole tiles, of about kPieceBytes of dz
-        const long long pieces = (long long)(((size_t)n * v * 2 * L.planes + kPieceBytes - 1) / kPieceBytes);
-        long long piece = up_to((v + pieces - 1) / pieces, 256);
-        if (piece > v) piece = v;
-        L.pieces = ceil_div(v, piece);
-        L.piece = (int)piece;
         L.scores = way_of_scores(fp32, piece, n, steps);
         L.grads = way_of_grads(fp32, d->dx != nullptr, d->dw != nullptr, n, w, piece, L.pieces);
         L.px = L.pw = up_to(w, 4);
@@ -1136,7 +1278,8 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.dz = take((size_t)n * up_to(piece * 2, 16) * L.planes);
         L.accx = take(d->dx && (L.pieces > 1 || L.grads.split_x > 1) ? (size_t)L.grads.split_x * n * L.px * 4 : 0);
         L.accw = take(d->dw && L.grads.split_w > 1 ? (size_t)L.grads.split_w * piece * L.pw * 4 : 0);
-        L.bpart = take(d->dbias ? (size_t)L.shares * piece * 4 : 0);
+        const int kept_shares = L.keeps ? ceil_div(n, 4 * kKeptRows) : 0;
+        L.bpart = take(d->dbias ? (size_t)(L.shares > kept_shares ? L.shares : kept_shares) * piece * 4 : 0);
     }
     L.bytes = at;
     return L;
@@ -1248,7 +1391,8 @@ int launch_scores_tile(GemmArgs& g, hipStream_t s) {
 template <class E, int EPI>
 int launch_scores(int tile, GemmArgs& g, hipStream_t s) {
     if constexpr (E::PLANES == 3) {
-        return tile == kSmall ? launch_scores_tile<E, SmallSplit, EPI>(g, s) : launch_scores_tile<E, MidSplit, EPI>(g, s);
+        constexpr int kEpi = EPI == EPI_KEEP ? EPI_STATS : EPI;          // (fp32 keeps nothing)
+        return tile == kSmall ? launch_scores_tile<E, SmallSplit, kEpi>(g, s) : launch_scores_tile<E, MidSplit, kEpi>(g, s);
     } else {
         return tile == kSmall ? launch_scores_tile<E, Small, EPI>(g, s) : tile == kMid ? launch_scores_tile<E, Mid, EPI>(g, s) : launch_scores_tile<E, BigScores, EPI>(g, s);
     }
@@ -1297,6 +1441,8 @@ int forward(const Run& r) {
     g.count = r.kept<int>(L.count), g.bias = d->bias;
     g.part_m = r.at<float>(L.part_m), g.part_s = r.at<float>(L.part_s), g.part_z = d->smoothing > 0.f ? r.at<float>(L.part_z) : nullptr;
     g.np = L.np;
+    const bool keeps = d->saved && L.keeps;
+    g.keeps = L.keeps, g.keep_pitch = L.keep_pitch;
     FinishArgs f = {};
     f.part_m = g.part_m, f.part_s = g.part_s, f.part_z = g.part_z, f.np = L.np, f.parts = L.parts, f.places = L.places;
     f.count = g.count;
@@ -1309,7 +1455,11 @@ int forward(const Run& r) {
         g.b = r.kept<char>(L.xc) + n0 * L.cpitch;
         g.label = f.label = r.kept<int>(L.label) + n0;
         g.zt = r.at<float>(L.zt) + n0, f.zt = g.zt;
-        Y6_TRY((launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
+        if (keeps) {
+            g.part_m = r.kept<float>(L.kept_m) + n0 / L.stat_rows * (L.parts * L.np), f.part_m = g.part_m;
+            g.keep = r.kept<char>(L.exps) + n0 * L.keep_pitch;
+        }
+        Y6_TRY((keeps ? launch_scores<E, EPI_KEEP>(L.scores, g, r.s) : launch_scores<E, EPI_STATS>(L.scores, g, r.s)));
         f.rowmap = r.kept<int>(L.rowmap) + n0;
         f.stat = r.kept<RowStat>(L.stat) + n0;
         if (!sums) f.rows_out = d->loss;
@@ -1352,14 +1502,33 @@ int backward(const Run& r) {
         g.stat = r.kept<RowStat>(L.stat), g.coef = coef;
         g.smooth = d->smoothing, g.smooth_share = d->smoothing / d->classes;
         g.dz = dz, g.dz_pitch = up_to((long long)vn * 2, 16), g.dz_plane = d->rows * g.dz_pitch;
-        Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
+        const bool kept = v0 < L.keeps;
+        int shares = L.shares;
+        if constexpr (E::PLANES == 1) {
+            if (kept) {
+                KeptArgs k = {};
+                k.e = r.kept<char>(L.exps) + (long long)v0 * 2, k.e_pitch = L.keep_pitch;
+                k.part_m = r.kept<float>(L.kept_m), k.np = L.np, k.parts = L.parts, k.stat_rows = L.stat_rows;
+                k.part_shift = __builtin_ctz(kSide[L.kept_scores] / kWavesM[L.kept_scores]);
+                k.stat = g.stat, k.coef = coef, k.label = g.label, k.count = count, k.smooth = g.smooth, k.smooth_share = g.smooth_share;
+                k.col_blocks = ceil_div(g.dz_pitch, kKeptCols * 2);
+                k.class0 = v0, k.classes = vn, k.dz = dz, k.dz_pitch = g.dz_pitch;
+                shares = ceil_div(d->rows, 4 * kKeptRows);
+                if (d->dbias) k.bpart = r.at<float>(L.bpart);
+                hipLaunchKernelGGL(kept_kernel<E>, dim3((unsigned)(k.col_blocks * shares)), dim3(256), 0, r.s, k);
+                Y6_LAUNCH_CHECK();
+            }
+        }
+        if (!kept) Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
         if (d->dbias) {
             auto* const db = (typename E::S*)d->dbias + v0;
+            if (!kept) {
             hipLaunchKernelGGL(bias_part_kernel<E>, dim3(ceil_div(vn, kBiasCols), L.shares), dim3(256), 0, r.s, dz, g.dz_pitch, g.dz_plane, vn, count,
                                r.at<float>(L.bpart), L.shares == 1 ? db : nullptr, d->grad_out, gmax, mean);
             Y6_LAUNCH_CHECK();
-            if (L.shares > 1) {
-                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), L.shares, vn, db, d->grad_out, gmax,
+            }
+            if (kept || shares > 1) {
+                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), shares, vn, db, d->grad_out, gmax,
                                    mean, count);
                 Y6_LAUNCH_CHECK();
             }
@@ -1409,7 +1578,7 @@ int backward(const Run& r) {
 // ====================================================================== C ABI
 extern "C" size_t y6_linear_ce_saved_bytes(const y6_linear_ce_desc* d) {
     if (check_desc(d, "linear_ce_saved_bytes") != Y6_OK) return 0;
-    return layout(d, false).kept;
+    return layout(d, false).kept_all;
 }
 
 extern "C" size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int backward_pass) {
@@ -1421,7 +1590,7 @@ extern "C" size_t y6_linear_ce_workspace_bytes(const y6_linear_ce_desc* d, int b
 static int check_buffers(const y6_linear_ce_desc* d, const Layout& L, size_t need, const char* what) {
     Y6_REQUIRE(d->workspace && d->workspace_bytes >= need && (uintptr_t)d->workspace % 16 == 0, "%s: workspace of %zu bytes, %zu needed", what,
                d->workspace_bytes, need);
-    Y6_REQUIRE(!d->saved || (d->saved_bytes >= L.kept && (uintptr_t)d->saved % 16 == 0), "%s: saved holds %zu bytes, %zu needed", what, d->saved_bytes, L.kept);
+    Y6_REQUIRE(!d->saved || (d->saved_bytes >= L.kept_all && (uintptr_t)d->saved % 16 == 0), "%s: saved holds %zu bytes, %zu needed", what, d->saved_bytes, L.kept_all);
     return Y6_OK;
 }
 

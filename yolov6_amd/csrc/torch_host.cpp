@@ -16,6 +16,8 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include <cmath>
 #include <unordered_set>
@@ -154,6 +156,21 @@ std::string shape(const Tensor& t) {
     return s.str();
 }
 
+// While a stream is captured, a leaf's gradient accumulator must be the capture's own: one that a living eager graph made belongs to that
+// graph's stream, the engine would make it wait, and the capture's end brings the process down.
+void refuse_outer_graph(const std::initializer_list<const Tensor*>& operands) {
+    for (const Tensor* t : operands) {
+        if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
+        const auto stream = c10::hip::getCurrentHIPStream(t->device().index());
+        hipStreamCaptureStatus state = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing(stream.stream(), &state) != hipSuccess || state == hipStreamCaptureStatusNone) return;
+        const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
+        TORCH_CHECK(!node || node->input_metadata(0).stream() == stream.unwrap(),
+                    "yolov6_amd: linear_cross_entropy is captured into a graph while an eager graph over one of its operands is alive "
+                    "(drop the loss that holds it before the capture, or capture on a detached operand)");
+    }
+}
+
 struct Operands {
     Tensor x, w, b, t;
     Options o;
@@ -197,6 +214,10 @@ Tensor linear_cross_entropy(const Tensor& features, const Tensor& weight, const 
                             double smoothing, const std::string& reduction) {
     const Operands p = operands(features, weight, target, bias, ignore, smoothing, reduction);
     Tensor loss;
+    if (at::GradMode::is_enabled()) {
+        const Tensor given = bias.has_value() ? *bias : Tensor();
+        refuse_outer_graph({&features, &weight, &given});
+    }
     if (at::GradMode::is_enabled() && (p.x.requires_grad() || p.w.requires_grad() || (p.b.defined() && p.b.requires_grad())))
         loss = LinearCrossEntropy::apply(p.x, p.w, p.b.defined() ? std::optional<Tensor>(p.b) : std::nullopt, p.t, p.o.ignore, p.o.smoothing, p.o.reduction);
     else
