@@ -5,7 +5,7 @@ Tolerances.  u = torch.finfo(dtype).eps / 2, products exact, fp32 accumulation.
              width * 2^-24 * sum |x w| <= width * 2^-24 * |x| |w| (worst order), lse and the rest by a few 2^-24 of the largest logit
   gradients  dz is rounded once (u |dz|), the result once (u), both accumulated in fp32.  Norm-wise over a whole gradient:
              |d dx| <= u | |dz| |W| | + u |dx|, so each is held to (|dz| |W|) u + u |dx| + the logits' error, elementwise.
-             Kept exponentials (16-bit types, large calls) are rounded once more before dz: u p, except at the label.
+             Kept exponentials (large calls) are rounded once more before dz: u p, except at the label.
              A probability below fp32's smallest normal number, 2^-126, may be flushed to zero by the exponential and the products
              (hardware exp2; 1e-38 of a gradient): 2^-126 of the other operand's magnitudes, doubled.
 """
@@ -112,6 +112,11 @@ def test_options(dtype, reduction, smoothing, bias):
     _check(x, w, b, t, smoothing, reduction, up)
 
 
+def _keeps(n, d, v, dtype):
+    """Whether such a call keeps exponentials."""
+    return d >= 64 and v >= 512 and n * v >= 1 << 19 if dtype == torch.float32 else d >= 128 and v >= 1024 and n * v >= 1 << 22
+
+
 # (rows, width, classes): every tile size, several pieces of the vocabulary (over 128 MB of dz), splits of both gradient products
 LARGE = [(2100, 72, 33000), (4097, 40, 20011), (1100, 1032, 2057), (20000, 64, 81), (40, 136, 70001), (3000, 512, 4100)]
 
@@ -120,7 +125,7 @@ LARGE = [(2100, 72, 33000), (4097, 40, 20011), (1100, 1032, 2057), (20000, 64, 8
 @pytest.mark.parametrize("n,d,v", LARGE)
 def test_pieces_tiles_and_splits(n, d, v, dtype):
     x, w, b, t = _inputs(n, d, v, dtype, True, seed=v)
-    _check(x, w, b, t, smoothing=0.1, up=torch.tensor(16.0 * n if dtype == torch.float16 else 1.0, device=DEV), kept=n * v >= 1 << 22 and d >= 128)
+    _check(x, w, b, t, smoothing=0.1, up=torch.tensor(16.0 * n if dtype == torch.float16 else 1.0, device=DEV), kept=_keeps(n, d, v, dtype))
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
@@ -486,7 +491,7 @@ def test_gradients_of_rows_that_are_almost_right(top, smooth):
 KEPT = [(4100, 256, 4200), (300, 264, 60001), (9000, 300, 2101), (2050, 520, 33003)]
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("reduction,smoothing", [("mean", 0.0), ("none", 0.1)])
 @pytest.mark.parametrize("n,d,v", KEPT)
 def test_kept_exponentials(n, d, v, reduction, smoothing, dtype):
@@ -498,7 +503,7 @@ def test_kept_exponentials(n, d, v, reduction, smoothing, dtype):
     _check(x, w, b, t, smoothing, reduction, up, kept=True)
 
 
-@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
 def test_kept_exponentials_with_masked_classes(dtype):
     """Classes at minus infinity that fill whole tiles, begin and end inside one; large logits; no bias gradient asked for."""
     from yolov6_amd.models.losses.loss_ce import linear_cross_entropy

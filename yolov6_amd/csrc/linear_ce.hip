@@ -7,12 +7,12 @@
 //
 // Matrix products, all of the time at sizes that matter; the matrix cores bound them:
 //   forward     z = W x^T tile by tile (scores_kernel); the epilogue leaves a running maximum and a sum of exponentials per row and tile and,
-//               for training with 16-bit types, the exponentials in 16 bits (kKeepBytes)
+//               for training, the exponentials in the operands' type (kKeepBytes)
 //   backward    for a piece of the vocabulary: dz from the kept exponentials (kept_kernel, a memory pass) or, where there are none, from z
 //               formed again; 16 bits for 16-bit inputs, the operand that the matrix instructions of the next two products take.  Then
 //               dx += dz W[piece] and dW[piece] = dz^T x in one launch (gemm_tile)
-// so a call holds one piece of dz (kPieceBytes) and what is kept, never the logits.  A kept exponential is rounded to 16 bits and dz once
-// more (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9 ms, 0.95
+// so a call holds one piece of dz (kPieceBytes) and what is kept, never the logits.  A kept exponential is rounded and dz once more
+// (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9 ms, 0.95
 // PFLOP/s over the three products; without the kept ones 8.1.  torch's product of such operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on
 // the same card, which lowers its clock under either.
 // Labelled rows are gathered first (gather_kernel): rows with ignore_index cost nothing, and an infinity or a NaN in one of them reaches no
@@ -33,13 +33,13 @@ typedef __bf16 b8_t __attribute__((ext_vector_type(8)));
 
 constexpr unsigned kOob = 0xf0000000u;     // offset of a piece that must read zeros
 constexpr size_t kPieceBytes = (size_t)128 << 20;     // of dz: half the last-level cache, and tiles enough to fill the chip
-// Training keeps the forward's exponentials, 16 bits each, instead of forming the scores again, while they take at most kKeepBytes (below 1 %
-// of the card's memory); what is behind that, by whole pieces, is formed again.
+// Training keeps the forward's exponentials, in the operands' type, instead of forming the scores again, while they take at most kKeepBytes
+// (below 1 % of the card's memory); what is behind that, by whole pieces, is formed again.  Measured with gradients and bias, formed again
+// against kept, us.  bf16: 4096 rows x 16000 classes x 128 wide 207 -> 196, 256 249 -> 226, 384 320 -> 281, 8192 x 32000 x 64 645 -> 663; few
+// classes leave lanes empty, 20000 x 600 x 256 111 -> 113; few scores are latency, 512 x 1000 x 512 45.7 -> 47.1, 1024 x 4001 x 256 61.8 -> 59.3.
+// fp32, whose scores take six products: 4096 x 8000 x 64 264 -> 246, 2600 x 21000 x 256 907 -> 763, 512 x 1000 x 512 82 -> 75.
 constexpr size_t kKeepBytes = (size_t)2 << 30;
-// Measured with bf16 gradients and bias, formed again against kept: 4096 rows x 16000 classes x 128 wide 207 -> 196 us, 256 249 -> 226, 384
-// 320 -> 281, 8192 x 32000 x 64 645 -> 663; few classes leave lanes empty, 20000 x 600 x 256 111 -> 113; few scores are latency, 512 x 1000 x 512
-// 45.7 -> 47.1, 1024 x 4001 x 256 61.8 -> 59.3.
-constexpr long long kKeepWidth = 128, kKeepClasses = 1024, kKeepScores = 1 << 22;
+constexpr long long kKeepWidth[2] = {128, 64}, kKeepClasses[2] = {1024, 512}, kKeepScores[2] = {1 << 22, 1 << 19};     // 16 bits, fp32
 constexpr size_t kPartBytes = (size_t)256 << 20;      // of the tiles' statistics: the forward takes the rows in as many pieces
 constexpr float kLog2e = 1.44269504088896340736f;
 // dz of fp16 inputs is stored times 2^14 (|dz| <= 1 before): fp16's normal range then reaches down to 2^-28, below which a class
@@ -718,8 +718,8 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                 if (EPI == EPI_KEEP && tm * BM < e.keeps) {
                     const float ref = top == -INFINITY ? 0.f : top;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    char* const row = e.keep + (long long)n * e.keep_pitch + (long long)(mw + 4 * half) * 2;
-                    int end16 = (int)(e.keep_pitch / 2) - mw - 4 * half;
+                    char* const row = e.keep + (long long)n * e.keep_pitch + (long long)(mw + 4 * half) * E::ES;
+                    int end16 = (int)(e.keep_pitch / E::ES) - mw - 4 * half;
                     asm volatile("" : "+v"(end16));
 #pragma unroll
                     for (int i = 0; i < FM; ++i)
@@ -734,14 +734,21 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                                     v[k][c4] = exp2_fast(fmaf(acc[i][j][8 * gp + 4 * k + c4] - ref, kLog2e, E::kKeepExp));
                                     sum[c4] += v[k][c4];
                                 }
-                            uint2 a[E::PLANES], b[E::PLANES];
-                            pack4<E>(v[0], a);
-                            pack4<E>(v[1], b);
-                            const auto x = __builtin_amdgcn_permlane32_swap(a[0].x, b[0].x, false, false);
-                            const auto y = __builtin_amdgcn_permlane32_swap(a[0].y, b[0].y, false, false);
                             // (as dz: sixteen bytes a lane; the row is padded to them, and classes behind the last are zeros)
-                            if (live && i * 32 + 16 * gp + 4 * half < end16)
-                                *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+                            if constexpr (E::ES == 4) {
+#pragma unroll
+                                for (int k = 0; k < 2; ++k)
+                                    if (live && i * 32 + 16 * gp + 8 * k < end16)
+                                        *reinterpret_cast<float4*>(row + (i * 32 + 16 * gp + 8 * k) * 4) = make_float4(v[k][0], v[k][1], v[k][2], v[k][3]);
+                            } else {
+                                uint2 a[E::PLANES], b[E::PLANES];
+                                pack4<E>(v[0], a);
+                                pack4<E>(v[1], b);
+                                const auto x = __builtin_amdgcn_permlane32_swap(a[0].x, b[0].x, false, false);
+                                const auto y = __builtin_amdgcn_permlane32_swap(a[0].y, b[0].y, false, false);
+                                if (live && i * 32 + 16 * gp + 4 * half < end16)
+                                    *reinterpret_cast<uint4*>(row + (i * 32 + 16 * gp + 4 * half) * 2) = make_uint4(x[0], y[0], x[1], y[1]);
+                            }
                         }
                     all = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * E::kKeepUnit;
                     all += __shfl_xor(all, 32);
@@ -1045,13 +1052,14 @@ struct KeptArgs {
     float smooth, smooth_share;
     int class0, classes, col_blocks;
     char* dz;
-    long long dz_pitch;
+    long long dz_pitch, dz_plane;
     float* bpart;                  // [block of rows][classes] or null
 };
 template <class E>
 __global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
     __shared__ float sh[4][8][64];
-    typedef typename E::O O8 __attribute__((ext_vector_type(8)));
+    typedef typename E::S S4 __attribute__((ext_vector_type(E::ES == 4 ? 4 : 8)));     // 16 bytes
+    constexpr int L = E::ES == 4 ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int bx = blockIdx.x % a.col_blocks, by = blockIdx.x / a.col_blocks;
     const int N = *a.count, c0 = bx * kKeptCols + lane * 8, n0 = (by * 4 + wave) * kKeptRows;
@@ -1060,12 +1068,14 @@ __global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
     float sum[8] = {};
     constexpr int U = 4;
     for (int k = n0; k < n0 + kKeptRows && k < N; k += U) {
-        O8 e[U];
+        S4 e[U][L];
         float pm[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int n = k + u < N ? k + u : N - 1;
-            e[u] = __builtin_nontemporal_load(reinterpret_cast<const O8*>(a.e + n * a.e_pitch + (mine ? c0 * 2 : 0)));   // (read once: dz stays in the caches)
+#pragma unroll
+            for (int l = 0; l < L; ++l)            // (read once: dz stays in the caches)
+                e[u][l] = __builtin_nontemporal_load(reinterpret_cast<const S4*>(a.e + n * a.e_pitch + (mine ? c0 * E::ES : 0) + (mine ? l * 16 : 0)));
             pm[u] = a.part_m[((long long)(n / a.stat_rows) * a.parts + part) * a.np + n % a.stat_rows];
         }
 #pragma unroll
@@ -1076,15 +1086,20 @@ __global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
             const float c = (a.coef ? a.coef[n] : 1.f) * E::kScale, share = -a.smooth_share * c;
             const float f = exp2_fast(fmaf(pm[u] - st.top, kLog2e, -st.log2s - E::kKeepExp)) * c, own = fmaf(-st.miss, c, fmaf(a.smooth, c, share));
             const int at = a.label[n] - a.class0 - c0;
-            O8 o;
+            float d[2][4];
 #pragma unroll
             for (int q = 0; q < 8; ++q) {
-                float d = fmaf((float)e[u][q], f, share);
-                d = q == at ? own : c0 + q < a.classes ? d : 0.f;
-                sum[q] += d;
-                o[q] = (typename E::O)d;
+                float v = fmaf((float)e[u][q * L / 8][q % (8 / L)], f, share);
+                v = q == at ? own : c0 + q < a.classes ? v : 0.f;
+                sum[q] += v;
+                d[q / 4][q % 4] = v;
             }
-            if (mine) *reinterpret_cast<O8*>(a.dz + n * a.dz_pitch + c0 * 2) = o;
+            uint2 lo[E::PLANES], hi[E::PLANES];
+            pack4<E>(d[0], lo);
+            pack4<E>(d[1], hi);
+#pragma unroll
+            for (int p = 0; p < E::PLANES; ++p)
+                if (mine) *reinterpret_cast<uint4*>(a.dz + p * a.dz_plane + n * a.dz_pitch + c0 * 2) = make_uint4(lo[p].x, lo[p].y, hi[p].x, hi[p].y);
         }
     }
     if (!a.bpart) return;
@@ -1247,11 +1262,11 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     if (rows < 256) rows = 256;
     L.stat_rows = (int)(rows < n ? rows : n);
     L.np = up_to(L.stat_rows, 64);
-    if (!fp32 && w >= kKeepWidth && v >= kKeepClasses && n * v >= kKeepScores) {
-        const long long most = (long long)(kKeepBytes / ((size_t)n * piece * 2));
+    if (w >= kKeepWidth[fp32] && v >= kKeepClasses[fp32] && n * v >= kKeepScores[fp32]) {
+        const long long most = (long long)(kKeepBytes / ((size_t)n * piece * es));
         L.keeps = (int)(most >= L.pieces ? v : most * piece);
     }
-    L.keep_pitch = up_to((long long)L.keeps * 2, 16);
+    L.keep_pitch = up_to((long long)L.keeps, 8) * es;
     L.exps = take((size_t)n * L.keep_pitch);
     L.kept_m = take(L.keeps ? (size_t)ceil_div(n, L.stat_rows) * L.parts * L.np * 4 : 0);
     L.kept_all = at;
@@ -1391,8 +1406,7 @@ int launch_scores_tile(GemmArgs& g, hipStream_t s) {
 template <class E, int EPI>
 int launch_scores(int tile, GemmArgs& g, hipStream_t s) {
     if constexpr (E::PLANES == 3) {
-        constexpr int kEpi = EPI == EPI_KEEP ? EPI_STATS : EPI;          // (fp32 keeps nothing)
-        return tile == kSmall ? launch_scores_tile<E, SmallSplit, kEpi>(g, s) : launch_scores_tile<E, MidSplit, kEpi>(g, s);
+        return tile == kSmall ? launch_scores_tile<E, SmallSplit, EPI>(g, s) : launch_scores_tile<E, MidSplit, EPI>(g, s);
     } else {
         return tile == kSmall ? launch_scores_tile<E, Small, EPI>(g, s) : tile == kMid ? launch_scores_tile<E, Mid, EPI>(g, s) : launch_scores_tile<E, BigScores, EPI>(g, s);
     }
@@ -1504,20 +1518,18 @@ int backward(const Run& r) {
         g.dz = dz, g.dz_pitch = up_to((long long)vn * 2, 16), g.dz_plane = d->rows * g.dz_pitch;
         const bool kept = v0 < L.keeps;
         int shares = L.shares;
-        if constexpr (E::PLANES == 1) {
-            if (kept) {
-                KeptArgs k = {};
-                k.e = r.kept<char>(L.exps) + (long long)v0 * 2, k.e_pitch = L.keep_pitch;
-                k.part_m = r.kept<float>(L.kept_m), k.np = L.np, k.parts = L.parts, k.stat_rows = L.stat_rows;
-                k.part_shift = __builtin_ctz(kSide[L.kept_scores] / kWavesM[L.kept_scores]);
-                k.stat = g.stat, k.coef = coef, k.label = g.label, k.count = count, k.smooth = g.smooth, k.smooth_share = g.smooth_share;
-                k.col_blocks = ceil_div(g.dz_pitch, kKeptCols * 2);
-                k.class0 = v0, k.classes = vn, k.dz = dz, k.dz_pitch = g.dz_pitch;
-                shares = ceil_div(d->rows, 4 * kKeptRows);
-                if (d->dbias) k.bpart = r.at<float>(L.bpart);
-                hipLaunchKernelGGL(kept_kernel<E>, dim3((unsigned)(k.col_blocks * shares)), dim3(256), 0, r.s, k);
-                Y6_LAUNCH_CHECK();
-            }
+        if (kept) {
+            KeptArgs k = {};
+            k.e = r.kept<char>(L.exps) + (long long)v0 * E::ES, k.e_pitch = L.keep_pitch;
+            k.part_m = r.kept<float>(L.kept_m), k.np = L.np, k.parts = L.parts, k.stat_rows = L.stat_rows;
+            k.part_shift = __builtin_ctz(kSide[L.kept_scores] / kWavesM[L.kept_scores]);
+            k.stat = g.stat, k.coef = coef, k.label = g.label, k.count = count, k.smooth = g.smooth, k.smooth_share = g.smooth_share;
+            k.col_blocks = ceil_div(g.dz_pitch, kKeptCols * 2);
+            k.class0 = v0, k.classes = vn, k.dz = dz, k.dz_pitch = g.dz_pitch, k.dz_plane = g.dz_plane;
+            shares = ceil_div(d->rows, 4 * kKeptRows);
+            if (d->dbias) k.bpart = r.at<float>(L.bpart);
+            hipLaunchKernelGGL(kept_kernel<E>, dim3((unsigned)(k.col_blocks * shares)), dim3(256), 0, r.s, k);
+            Y6_LAUNCH_CHECK();
         }
         if (!kept) Y6_TRY((launch_scores<E, EPI_DZ>(L.scores, g, r.s)));
         if (d->dbias) {

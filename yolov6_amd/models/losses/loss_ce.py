@@ -1,4 +1,4 @@
-"""Softmax cross entropy of a linear classifier over many classes: value and gradients without keeping the logits.
+"""Softmax cross entropy of a linear classifier over many classes: value and gradients without the logits in memory.
 
     loss = linear_cross_entropy(features, weight, target, bias)     # = F.cross_entropy(F.linear(features, weight, bias), target)
     loss.backward()
@@ -8,6 +8,9 @@ label set, dense labels with a large vocabulary.  The detection losses (loss.py)
 softmax classifier; the semantics are torch's, except that the mean over no labelled row is 0 (as ComputeLoss's terms are without
 targets), not a NaN.  Kernels: csrc/linear_ce.hip (y6_linear_ce_forward / _backward); the
 autograd node and the operands' checks: csrc/torch_host.cpp.
+
+Memory of a training call beside its operands and gradients: the labelled rows gathered, at most 2 GiB of exponentials in the operands'
+type (they live from the forward to the end of the graph), and at most 256 MB of dz during the backward.
 """
 from ... import _lib
 
@@ -20,6 +23,7 @@ def linear_cross_entropy(features, weight, target, bias=None, *, ignore_index=-1
     come in the operands' type, once differentiable; under a loss scale (LossScaler) as usual.  Rows labelled ignore_index have loss
     0, a zero gradient, and are not read: a NaN in them goes nowhere.  A label that is neither a class nor ignore_index makes its
     row's loss and the gradients NaN (no host check: nothing synchronises).  Products of 16-bit operands accumulate in fp32; the
-    gradient of the logits is rounded to the operands' type once, where the matrix instructions of the two gradient products take
-    it.  Works on any view with a dense last dimension; others are copied."""
+    gradient of the logits is rounded to the operands' type where the matrix instructions of the two gradient products take it (in
+    large calls the probabilities of the other classes once before that, when they are kept for the backward).  Under stream capture no
+    eager graph over the operands may be alive (an error).  Works on any view with a dense last dimension; others are copied."""
     return _lib.torch_host().linear_cross_entropy(features, weight, target, bias, ignore_index, label_smoothing, reduction)
