@@ -565,7 +565,7 @@ __device__ __forceinline__ GemmArgs args_again() {
 // A tile's reduction is short (the features' width: 16 steps at 1024), so what lies around it counts.  For dz a block stays and walks
 // its tiles as one sequence of steps, the first loads of the next tile in flight while the last step of this one is multiplied and its
 // dz stored: 16384 x 4096 x 1024 in 151 instead of 164 us.  (Keeping dz in registers to store it during the next tile spills, 203 us.)  The
-// statistics have little to store, and in the loop their masks spill: there a block takes one tile.
+// statistics lose that way, with their masks kept from spilling too (a training step of 4096 x 32000 x 1024 925 -> 1065 us): a block takes one tile.
 template <class E, class T, int EPI>
 __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(const GemmArgs g) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -1039,7 +1039,7 @@ __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__
 // its RowStat.  A wave takes 512 classes, 16 bytes a lane, and 16 rows, four at a time, so that it also has their sum, which becomes db: the
 // block adds its four waves', in order.  Memory bounds it: 128 MB to 128 MB in 53 us, 4.9 TB/s, where forming the scores of 1024 features again
 // took 150.  (32 rows a wave: 37 instead of 31 us at 1383 x 25088.)
-constexpr int kKeptRows = 16, kKeptCols = 512;
+constexpr int kKeptCols = 512;
 struct KeptArgs {
     const char* e;                 // the piece's first class
     long long e_pitch;
@@ -1050,7 +1050,7 @@ struct KeptArgs {
     const float* coef;
     const int *label, *count;
     float smooth, smooth_share;
-    int class0, classes, col_blocks;
+    int class0, classes, col_blocks, rows;   // rows: of a wave, a multiple of four
     char* dz;
     long long dz_pitch, dz_plane;
     float* bpart;                  // [block of rows][classes] or null
@@ -1062,12 +1062,12 @@ __global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
     constexpr int L = E::ES == 4 ? 2 : 1;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
     const int bx = blockIdx.x % a.col_blocks, by = blockIdx.x / a.col_blocks;
-    const int N = *a.count, c0 = bx * kKeptCols + lane * 8, n0 = (by * 4 + wave) * kKeptRows;
+    const int N = *a.count, c0 = bx * kKeptCols + lane * 8, n0 = (by * 4 + wave) * a.rows;
     const bool mine = c0 * 2 < a.dz_pitch;
     const int part = (a.class0 + (mine ? c0 : 0)) >> a.part_shift;
     float sum[8] = {};
     constexpr int U = 4;
-    for (int k = n0; k < n0 + kKeptRows && k < N; k += U) {
+    for (int k = n0; k < n0 + a.rows && k < N; k += U) {
         S4 e[U][L];
         float pm[U];
 #pragma unroll
@@ -1206,7 +1206,7 @@ struct Layout {
     size_t bytes;
     long long cpitch, np;              // bytes between rows of the gathered features, of the weight's copy; rows
     int planes, scores, parts, places, stat_rows, piece, pieces, shares;
-    int keeps, kept_scores;            // classes whose exponentials are kept (whole pieces), by tiles of this kind
+    int keeps, kept_scores, kept_rows; // classes whose exponentials are kept (whole pieces), by tiles of this kind; rows of a kept_kernel wave
     long long keep_pitch;              // bytes
     GradWay grads;
     long long px, pw;
@@ -1266,6 +1266,9 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         const long long most = (long long)(kKeepBytes / ((size_t)n * piece * es));
         L.keeps = (int)(most >= L.pieces ? v : most * piece);
     }
+    // (a wave of kept_kernel takes 16 rows, fewer where four blocks a CU would not come together: 1024 x 4001 in fp32 22 us with 16)
+    L.kept_rows = 16;
+    while (L.kept_rows > 4 && (long long)ceil_div(n, 4 * L.kept_rows) * ceil_div(L.piece, kKeptCols) < 1024) L.kept_rows /= 2;
     L.keep_pitch = up_to((long long)L.keeps, 8) * es;
     L.exps = take((size_t)n * L.keep_pitch);
     L.kept_m = take(L.keeps ? (size_t)ceil_div(n, L.stat_rows) * L.parts * L.np * 4 : 0);
@@ -1293,7 +1296,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
         L.dz = take((size_t)n * up_to(piece * 2, 16) * L.planes);
         L.accx = take(d->dx && (L.pieces > 1 || L.grads.split_x > 1) ? (size_t)L.grads.split_x * n * L.px * 4 : 0);
         L.accw = take(d->dw && L.grads.split_w > 1 ? (size_t)L.grads.split_w * piece * L.pw * 4 : 0);
-        const int kept_shares = L.keeps ? ceil_div(n, 4 * kKeptRows) : 0;
+        const int kept_shares = L.keeps ? ceil_div(n, 4 * L.kept_rows) : 0;
         L.bpart = take(d->dbias ? (size_t)(L.shares > kept_shares ? L.shares : kept_shares) * piece * 4 : 0);
     }
     L.bytes = at;
@@ -1526,7 +1529,7 @@ int backward(const Run& r) {
             k.stat = g.stat, k.coef = coef, k.label = g.label, k.count = count, k.smooth = g.smooth, k.smooth_share = g.smooth_share;
             k.col_blocks = ceil_div(g.dz_pitch, kKeptCols * 2);
             k.class0 = v0, k.classes = vn, k.dz = dz, k.dz_pitch = g.dz_pitch, k.dz_plane = g.dz_plane;
-            shares = ceil_div(d->rows, 4 * kKeptRows);
+            k.rows = L.kept_rows, shares = ceil_div(d->rows, 4 * k.rows);
             if (d->dbias) k.bpart = r.at<float>(L.bpart);
             hipLaunchKernelGGL(kept_kernel<E>, dim3((unsigned)(k.col_blocks * shares)), dim3(256), 0, r.s, k);
             Y6_LAUNCH_CHECK();
