@@ -579,3 +579,20 @@ def test_capture_beside_a_living_eager_graph_is_refused():
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("n,d,v,dtype", [(1101, 136, 4003, torch.float16), (1101, 129, 4003, torch.bfloat16), (523, 71, 1005, torch.float32)])
+def test_kept_exponentials_of_odd_sizes(n, d, v, dtype):
+    """Just enough of them, in the order of the rows and in another, and each gradient by itself."""
+    from yolov6_amd.models.losses.loss_ce import linear_cross_entropy
+    assert _keeps(n, d, v, dtype)
+    x, w, b, t = _inputs(n, d, v, dtype, True, seed=n)
+    up = torch.tensor(16.0 * n if dtype == torch.float16 else 1.0, device=DEV)
+    _, every = _check(x, w, b, t, smoothing=0.1, up=up, kept=True)
+    u = torch.finfo(dtype).eps / 2
+    for k in range(3):
+        leaves = [o.detach().requires_grad_(i == k) for i, o in enumerate((x, w, b))]
+        (got,) = torch.autograd.grad(linear_cross_entropy(leaves[0], leaves[1], t, leaves[2], label_smoothing=0.1), leaves[k], up)
+        # (one gradient alone may be cut into other tiles: the same sums in another order, rounded once)
+        assert bool(((got.double() - every[k].double()).abs() <= 2 * u * every[k].double().abs() + 2.0 ** -12 * float(every[k].abs().max())).all())
+    _check(x[:, :d - 8].t().contiguous().t(), w[:, 8:], None, t, reduction="sum", up=torch.tensor(4.0, device=DEV), kept=True)

@@ -108,6 +108,8 @@ std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor&
     if (!want_x && !want_w && !want_b) return {dx, dw, db};
     const Tensor g = grad.detach().to(at::kFloat).contiguous();
     y6_linear_ce_desc d = describe(x, w, b, t, o);
+    TORCH_CHECK((size_t)saved.numel() == lib.ce_saved(&d),
+                "yolov6_amd: linear_cross_entropy's backward is given other operands, or operands that lie otherwise, than its forward");
     d.saved = saved.data_ptr(), d.saved_bytes = (size_t)saved.numel(), d.grad_out = g.data_ptr<float>();
     d.dx = want_x ? dx.data_ptr() : nullptr, d.dw = want_w ? dw.data_ptr() : nullptr, d.dbias = want_b ? db.data_ptr() : nullptr;
     d.workspace_bytes = lib.ce_workspace(&d, 1);

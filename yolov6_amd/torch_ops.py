@@ -107,7 +107,8 @@ def _(x, weight, bias, act, stride):
 @torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy", mutates_args=(), device_types="cuda")
 def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], ignore_index: int, label_smoothing: float,
                          reduction: str) -> Tuple[Tensor, Tensor]:
-    """(loss, bytes that the backward takes over): models/losses/loss_ce.py with a schema."""
+    """(loss, bytes that the backward takes over): models/losses/loss_ce.py with a schema.  They are made whether a backward follows or not, up to
+    2 GiB of them: a caller that wants the value alone calls models/losses/loss_ce.py without gradients."""
     from . import _lib
     return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction)
 
