@@ -271,3 +271,22 @@ def test_a_gradient_of_more_than_2_to_the_30_elements():
         part = g[lo:min(lo + (1 << 28), n - 1)]
         assert float((part.float() - float(small)).abs().max()) <= 2.0 ** -8 * float(small)
     assert abs(float(g[-1]) - 4.0 / want) <= 2.0 ** -8 * 4.0 / want
+
+
+def test_gradients_with_gaps():
+    """Columns of one buffer, interleaved: each is scaled; the same columns twice are refused and left as they were."""
+    from yolov6_amd.solver import clip_grad_norm_
+    buf = torch.randn(64, 10, device="cuda")
+    before = buf.clone()
+    params = [torch.nn.Parameter(torch.zeros(64, 5, device="cuda")) for _ in range(2)]
+    params[0].grad, params[1].grad = buf[:, ::2], buf[:, 1::2]
+    norm = clip_grad_norm_(params, 0.5)
+    want = before.double().norm()
+    assert abs(float(norm) - float(want)) <= 2 * 2.0 ** -24 * float(want)
+    assert torch.allclose(buf.double(), before.double() * (0.5 / (want + 1e-6)), rtol=4 * 2.0 ** -24, atol=0)
+    before = buf.clone()
+    params[1].grad = buf[:, ::2]
+    with pytest.raises(RuntimeError, match="share memory"):
+        clip_grad_norm_(params, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)

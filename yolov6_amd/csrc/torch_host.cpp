@@ -296,6 +296,13 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
     for (const Tensor& g : grads) TORCH_CHECK(!g.requires_grad(), "yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place");
     for (const Tensor& g : grads)
         TORCH_CHECK(at::has_internal_overlap(g) != at::MemOverlap::Yes, "yolov6_amd: a gradient whose elements share memory is not scaled in place");
+    // (y6_grad_clip refuses dense ones that overlap; those with gaps are scaled as copies, and it does not see them)
+    bool gaps = false;
+    for (const Tensor& g : grads) gaps |= !g.is_non_overlapping_and_dense();
+    std::unordered_set<const void*> starts;
+    if (gaps)
+        for (const Tensor& g : grads)
+            TORCH_CHECK(g.numel() == 0 || starts.insert(g.data_ptr()).second, "yolov6_amd: clip_grad_norm_: two gradients share memory");
     const List l(grads, norm);
     TORCH_CHECK(!error_if_nonfinite || std::isfinite(norm_of(l).item<float>()), "yolov6_amd: the norm of the gradients is not finite, so they cannot be clipped");
     const c10::DeviceGuard guard(l.dense[0].device());
