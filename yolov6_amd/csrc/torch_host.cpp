@@ -169,7 +169,7 @@ void refuse_outer_graph(const std::initializer_list<const Tensor*>& operands) {
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
         TORCH_CHECK(!node || node->input_metadata(0).stream() == stream.unwrap(),
                     "yolov6_amd: linear_cross_entropy is captured into a graph while an eager graph over one of its operands is alive "
-                    "(drop the loss that holds it before the capture, or capture on a detached operand)");
+                    "(drop the loss that holds it before the capture, capture on the stream it was made on, or with a detached operand)");
     }
 }
 
