@@ -43,7 +43,8 @@ fi
 if has guardtrain; then
   for mode in end start; do
     timeout -k 5 600 python3 tests/tight_probe.py --mode $mode bench.py --mode train --steps 3 --warmup 2 > "$OUT/guard_train_$mode.json" 2> "$OUT/guard_train_$mode.err"
-    echo "train step under the guard allocator ($mode) rc=$?"; grep -E "Memory access|Error" "$OUT/guard_train_$mode.err" | tail -2
+    rc=$?; echo "train step under the guard allocator ($mode) rc=$rc"; grep -E "Memory access|Error" "$OUT/guard_train_$mode.err" | tail -2
+    if [ $rc -ne 0 ]; then exit $rc; fi
   done
   lap guardtrain
 fi

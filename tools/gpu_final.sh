@@ -5,11 +5,12 @@ set -u
 export TMPDIR=/tmp HSA_ENABLE_IPC_MODE_LEGACY=0
 OUT=gpurun_out/${1:-final}; mkdir -p $OUT
 T0=$(date +%s); lap() { echo "[$(( $(date +%s) - T0 )) s] $*"; }
-bash tools/gpu_soak.sh ${1:-final}_soak ${2:-10} | tail -$(( ${2:-10} + 1 ))
+bash tools/gpu_soak.sh ${1:-final}_soak ${2:-10} || exit $?
 lap soak
-timeout 300 python3 -c "import __graft_entry__ as g; g.smoke()" 2>&1 | tail -1
+timeout 300 python3 -c "import __graft_entry__ as g; g.smoke()" 2>&1 || exit $?
 timeout 1500 python3 -m pytest tests -m gpu -q --tb=short --timeout 900 -p no:cacheprovider --durations 8 > $OUT/pytest_gpu.log 2>&1
-echo "pytest rc=$?"; tail -14 $OUT/pytest_gpu.log | cut -c1-200
+rc=$?; echo "pytest rc=$rc"; tail -14 $OUT/pytest_gpu.log | cut -c1-200
+if [ $rc -ne 0 ]; then exit $rc; fi
 lap tests
 python3 bench.py --gpus 1 --steps 20 --warmup 5 > $OUT/bench_driver.json 2> $OUT/bench_driver.err
 echo "driver command rc=$?"; cut -c1-420 $OUT/bench_driver.json
