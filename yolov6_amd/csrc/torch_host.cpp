@@ -178,14 +178,9 @@ struct Operands {
     Options o;
 };
 // Operands as the kernels take them: features [rows, width], weight [classes, width], target [rows]
-Operands operands(Tensor features, Tensor weight, const Tensor& target, const std::optional<Tensor>& bias_in, int64_t ignore, double smoothing,
+Operands operands(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias_in, int64_t ignore, double smoothing,
                   const std::string& reduction) {
-    Tensor bias = bias_in.has_value() ? *bias_in : Tensor();
-    if (at::autocast::is_autocast_enabled(at::kCUDA)) {
-        const auto dtype = at::autocast::get_autocast_dtype(at::kCUDA);
-        features = features.to(dtype), weight = weight.to(dtype);
-        if (bias.defined()) bias = bias.to(dtype);
-    }
+    const Tensor bias = bias_in.has_value() ? *bias_in : Tensor();
     const int64_t code = reduction == "none" ? Y6_REDUCE_NONE : reduction == "sum" ? Y6_REDUCE_SUM : reduction == "mean" ? Y6_REDUCE_MEAN : -1;
     TORCH_CHECK(code >= 0, "yolov6_amd: linear_cross_entropy reduction '", reduction, "' ('mean', 'sum' or 'none')");
     TORCH_CHECK(smoothing >= 0.0 && smoothing <= 1.0, "yolov6_amd: linear_cross_entropy label_smoothing ", smoothing, " is not in [0, 1]");
@@ -214,7 +209,10 @@ Operands operands(Tensor features, Tensor weight, const Tensor& target, const st
 
 Tensor linear_cross_entropy(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias, int64_t ignore,
                             double smoothing, const std::string& reduction) {
-    const Operands p = operands(features, weight, target, bias, ignore, smoothing, reduction);
+    // (here and not in operands(): the dispatcher's ops take their operands as they are, cast in front of them)
+    const bool cast = at::autocast::is_autocast_enabled(at::kCUDA);
+    const auto as = [&](const Tensor& t) { return cast ? t.to(at::autocast::get_autocast_dtype(at::kCUDA)) : t; };
+    const Operands p = operands(as(features), as(weight), target, bias.has_value() ? std::optional<Tensor>(as(*bias)) : bias, ignore, smoothing, reduction);
     Tensor loss;
     if (at::GradMode::is_enabled()) {
         const Tensor given = bias.has_value() ? *bias : Tensor();

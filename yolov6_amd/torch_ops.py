@@ -108,7 +108,7 @@ def _(x, weight, bias, act, stride):
 def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], ignore_index: int, label_smoothing: float,
                          reduction: str) -> Tuple[Tensor, Tensor]:
     """(loss, bytes that the backward takes over): models/losses/loss_ce.py with a schema.  They are made whether a backward follows or not, up to
-    2 GiB of them: a caller that wants the value alone calls models/losses/loss_ce.py without gradients."""
+    2 GiB of them: a caller that wants the value alone calls models/losses/loss_ce.py without gradients.  Under autocast the operands are cast first."""
     from . import _lib
     return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction)
 
@@ -144,3 +144,14 @@ def _ce_grad(ctx, grad, _):
 
 
 linear_cross_entropy.register_autograd(_ce_grad, setup_context=_ce_setup)
+
+
+def _ce_autocast(features, weight, target, bias, *options):
+    """The casts come before the op, so that they are differentiated and its backward sees the operands of its forward, wherever it runs."""
+    dtype = torch.get_autocast_dtype("cuda")
+    with torch._C._ExcludeDispatchKeyGuard(torch._C.DispatchKeySet(torch._C.DispatchKey.AutocastCUDA)):
+        return torch.ops.yolov6_hip.linear_cross_entropy(features.to(dtype), weight.to(dtype), target, None if bias is None else bias.to(dtype), *options)
+
+
+_fragment = torch.library.Library(NAMESPACE, "FRAGMENT")      # (the kernel is there as long as this object)
+_fragment.impl("linear_cross_entropy", _ce_autocast, "AutocastCUDA")
