@@ -290,3 +290,11 @@ def test_gradients_with_gaps():
         clip_grad_norm_(params, 0.1)
     torch.cuda.synchronize()
     assert torch.equal(buf, before)
+
+
+def test_forward_mode_is_refused():
+    g = _grads([50], [torch.float32])[0]
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
+        with pytest.raises(RuntimeError, match="forward mode"):
+            grad_norm([dual])

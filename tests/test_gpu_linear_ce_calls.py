@@ -53,3 +53,13 @@ def test_the_op_backward_inside_autocast():
         with torch.autocast("cuda", dtype=torch.bfloat16):
             got = torch.autograd.grad(loss, leaves)
         assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+def test_forward_mode_is_refused_by_the_op():
+    ops = _inputs(10, 16, 12, torch.float32, True)
+    with torch.autograd.forward_ad.dual_level():
+        for k in range(3):
+            duals = [torch.autograd.forward_ad.make_dual(o, torch.ones_like(o)) if i == k else o for i, o in enumerate(ops[:3])]
+            for f in (_loss, _op_loss):
+                with pytest.raises(RuntimeError, match="forward mode"):
+                    f(duals, ops[3])

@@ -75,3 +75,15 @@ def test_gradient_refusals(hip_lib):
         grad_norm([p.grad.double()])
     assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(4))], 1.0)) == 0.0
 
+
+
+def test_forward_mode_is_refused(hip_lib):
+    """A dual operand's tangent would vanish: refused before anything else is looked at."""
+    x, w, t, b = _operands()
+    with torch.autograd.forward_ad.dual_level():
+        for k in range(3):
+            ops = [torch.autograd.forward_ad.make_dual(o, torch.ones_like(o)) if i == k else o for i, o in enumerate((x, w, b))]
+            with pytest.raises(RuntimeError, match="forward mode"):
+                linear_cross_entropy(ops[0], ops[1], t, ops[2])
+            with pytest.raises(RuntimeError, match="forward mode"):
+                grad_norm([ops[k]])

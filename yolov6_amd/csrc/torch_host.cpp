@@ -51,6 +51,10 @@ int type_code(at::ScalarType t) {
 void require_gpu(const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda(), "yolov6_amd: ", name, " must live on a ROCm device (got ", t.device(), "); the hot path has no CPU fallback");
 }
+// a dual tensor does not require a gradient, and its tangent would be lost without a word
+void refuse_forward_mode(const Tensor& t, const char* what) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "yolov6_amd: ", what, " has no forward mode derivative (a dual tensor was given)");
+}
 Tensor bytes_on(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
 
 // ---------------------------------------------------------------------------------------------------------- linear cross entropy
@@ -181,6 +185,7 @@ struct Operands {
 Operands operands(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias_in, int64_t ignore, double smoothing,
                   const std::string& reduction) {
     const Tensor bias = bias_in.has_value() ? *bias_in : Tensor();
+    for (const Tensor& t : {features, weight, bias}) refuse_forward_mode(t, "linear_cross_entropy");
     const int64_t code = reduction == "none" ? Y6_REDUCE_NONE : reduction == "sum" ? Y6_REDUCE_SUM : reduction == "mean" ? Y6_REDUCE_MEAN : -1;
     TORCH_CHECK(code >= 0, "yolov6_amd: linear_cross_entropy reduction '", reduction, "' ('mean', 'sum' or 'none')");
     TORCH_CHECK(smoothing >= 0.0 && smoothing <= 1.0, "yolov6_amd: linear_cross_entropy label_smoothing ", smoothing, " is not in [0, 1]");
@@ -258,6 +263,7 @@ struct List {
     List(const std::vector<Tensor>& grads, int norm) {
         const auto device = grads[0].device();
         for (const Tensor& g : grads) {
+            refuse_forward_mode(g, "the gradients' norm");
             const int code = g.layout() == at::kStrided ? type_code(g.scalar_type()) : -1;
             TORCH_CHECK(code >= 0, "yolov6_amd: gradients must be dense fp16, bf16 or fp32 tensors (got ", g.scalar_type(), ", ", g.layout(), ")");
             TORCH_CHECK(g.device() == device, "yolov6_amd: gradients on ", device, " and ", g.device(), ": one norm is taken on one device");

@@ -20,7 +20,7 @@ def linear_cross_entropy(features, weight, target, bias=None, *, ignore_index=-1
 
     features [..., width], weight [classes, width], bias [classes] or None, in one type (fp16, bf16, fp32; under autocast they are cast
     to its type); target [...] int64.  Returns fp32: a scalar ('mean' over the labelled rows, 'sum'), or [...] ('none').  Gradients
-    come in the operands' type, once differentiable; under a loss scale (LossScaler) as usual.  Rows labelled ignore_index have loss
+    come in the operands' type, once differentiable, in reverse mode (dual tensors are refused); under a loss scale (LossScaler) as usual.  Rows labelled ignore_index have loss
     0, a zero gradient, and are not read: a NaN in them goes nowhere.  A label that is neither a class nor ignore_index makes its
     row's loss and the gradients NaN (no host check: nothing synchronises).  Products of 16-bit operands accumulate in fp32; the
     gradient of the logits is rounded to the operands' type where the matrix instructions of the two gradient products take it (in
