@@ -298,3 +298,22 @@ def test_forward_mode_is_refused():
         dual = torch.autograd.forward_ad.make_dual(g, torch.ones_like(g))
         with pytest.raises(RuntimeError, match="forward mode"):
             grad_norm([dual])
+
+
+def test_clipping_counts_as_a_write():
+    """Autograd sees it: version counters of dense gradients and of ones with gaps go up, a graph that saved one refuses its backward."""
+    buf = torch.randn(64, 10, device=DEV)
+    params = _params([_grads([500], [torch.float32])[0], _grads([77], [torch.float16])[0], buf[:, ::2]])
+    before = [p.grad._version for p in params]
+    grad_norm([p.grad for p in params])
+    assert [p.grad._version for p in params] == before
+    w = torch.ones(500, device=DEV, requires_grad=True)
+    y = (w * params[0].grad).sum()
+    clip_grad_norm_(params, 1.0)
+    assert all(p.grad._version > v for p, v in zip(params, before))
+    with pytest.raises(RuntimeError, match="inplace"):
+        y.backward()
+    with torch.inference_mode():
+        held = torch.nn.Parameter(torch.zeros(9, device=DEV), requires_grad=False)
+        held.grad = torch.full((9,), 2.0, device=DEV)
+        assert abs(float(clip_grad_norm_([held], 1.0)) - 6.0) <= 6 * 2.0 ** -23

@@ -313,8 +313,11 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
     const size_t size = lib.norm_workspace(l.c.count, l.elements);
     const Tensor ws = bytes_on(l.dense[0], size), out = at::empty({}, l.dense[0].options().dtype(at::kFloat).requires_grad(false));
     check(lib.clip(&l.c, max_norm, ws.data_ptr(), size, out.data_ptr<float>(), stream_of(ws.device())), "grad_clip");
-    for (size_t i = 0; i < grads.size(); ++i)
+    for (size_t i = 0; i < grads.size(); ++i) {
+        // (autograd has to see the write: a graph that saved the gradient would use it as it is now.  Inference tensors have no counter)
         if (!l.dense[i].is_same(grads[i])) const_cast<Tensor&>(grads[i]).copy_(l.dense[i]);
+        else if (!grads[i].is_inference()) grads[i].unsafeGetTensorImpl()->bump_version();
+    }
     return out;
 }
 
