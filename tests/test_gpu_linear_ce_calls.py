@@ -63,3 +63,30 @@ def test_forward_mode_is_refused_by_the_op():
             for f in (_loss, _op_loss):
                 with pytest.raises(RuntimeError, match="forward mode"):
                     f(duals, ops[3])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,v", [(150, 96, 333), (4100, 256, 4200)])
+def test_an_upstream_gradient_that_is_not_finite_stays_in_its_row(n, d, v, dtype, bad):
+    """reduction none, as F.cross_entropy: the row's dx and the sums over all rows (dW, db) are not finite, the other rows' dx are theirs."""
+    ops = _inputs(n, d, v, dtype, True, seed=3, ignored=0.2)
+    t = ops[3]
+    t[5] = 7
+    up = torch.linspace(-2, 3, n, device=DEV)
+    up[5] = 0.0
+    leaves = _leaves(ops, dtype)
+    want = torch.autograd.grad(_loss(leaves, t, reduction="none"), leaves, up)
+    up[5] = bad
+    got = torch.autograd.grad(_loss(leaves, t, reduction="none"), leaves, up)
+    others = torch.arange(n, device=DEV) != 5
+    assert torch.equal(got[0][others], want[0][others]) and not bool(got[0][5].isfinite().any())
+    assert not bool(got[1].isfinite().any()) and not bool(got[2].isfinite().any())
+    # all of them, and beside zeros only
+    for value in (bad, 0.0):
+        up = torch.full((n,), value, device=DEV)
+        up[5] = bad
+        got = torch.autograd.grad(_loss(leaves, t, reduction="none"), leaves, up)
+        labelled = t != -100
+        rows = labelled if value != 0.0 else ~others
+        assert not bool(got[0][rows].isfinite().any()) and int(got[0][~rows].count_nonzero()) == 0

@@ -372,7 +372,7 @@ struct GemmArgs {
     float *part_m, *part_s, *part_z, *zt;
     long long np;                  // rows of the partial statistics' arrays
     const RowStat* stat;
-    const float* coef;             // g_n / max |g| (null: 1)
+    const float* coef;             // g_n / max |g| of the finite ones (null: 1)
     float smooth, smooth_share;    // e, e / V
     int class0;                    // first class of the piece
     char* keep;                    // EPI_KEEP: exponentials of the classes below `keeps`, by row
@@ -936,7 +936,8 @@ __global__ __launch_bounds__(1024) void loss_sum_kernel(const float* __restrict_
     *loss = (float)(mean ? s / (N > 1 ? N : 1) : s);
 }
 
-// reduction none: gmax = max |g| over the labelled rows, coef = g / gmax.  A gradient that is not finite makes all of them NaN.
+// reduction none: gmax = max |g| over the labelled rows whose g is finite (1 where all of those are zero), coef = g / gmax.  A g that is not
+// finite stays with its row: its dz, hence its dx and the sums over rows, dW and db, are not finite; the other rows' dx do not see it.
 __global__ __launch_bounds__(1024) void coef_kernel(const float* __restrict__ up, const int* __restrict__ rowmap, const int* __restrict__ count,
                                                     float* __restrict__ coef, float* __restrict__ gmax) {
     __shared__ float sh[16];
@@ -944,19 +945,17 @@ __global__ __launch_bounds__(1024) void coef_kernel(const float* __restrict__ up
     float top = 0.f;
     for (int i = threadIdx.x; i < N; i += 1024) {
         const float v = fabsf(up[rowmap[i]]);
-        top = v > top || v != v ? v : top;
+        top = v > top && v < INFINITY ? v : top;             // (comparisons with a NaN are false)
     }
 #pragma unroll
-    for (int d = 32; d > 0; d >>= 1) {
-        const float v = __shfl_xor(top, d);
-        top = v > top || v != v ? v : top;
-    }
+    for (int d = 32; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
     if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = top;
     __syncthreads();
     top = sh[0];
-    for (int w = 1; w < 16; ++w) top = sh[w] > top || sh[w] != sh[w] ? sh[w] : top;
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, sh[w]);
+    if (top == 0.f) top = 1.f;
     if (threadIdx.x == 0) *gmax = top;
-    for (int i = threadIdx.x; i < N; i += 1024) coef[i] = top > 0.f || top != top ? up[rowmap[i]] / top : 0.f;
+    for (int i = threadIdx.x; i < N; i += 1024) coef[i] = up[rowmap[i]] / top;
 }
 
 // sum of the splits of a product, times the gradient's factor, rounded once

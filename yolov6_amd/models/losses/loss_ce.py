@@ -22,7 +22,8 @@ def linear_cross_entropy(features, weight, target, bias=None, *, ignore_index=-1
     to its type); target [...] int64.  Returns fp32: a scalar ('mean' over the labelled rows, 'sum'), or [...] ('none').  Gradients
     come in the operands' type, once differentiable, in reverse mode (dual tensors are refused); under a loss scale (LossScaler) as usual.  Rows labelled ignore_index have loss
     0, a zero gradient, and are not read: a NaN in them goes nowhere.  A label that is neither a class nor ignore_index makes its
-    row's loss and the gradients NaN (no host check: nothing synchronises).  Products of 16-bit operands accumulate in fp32; the
+    row's loss and the gradients NaN (no host check: nothing synchronises).  With 'none', an upstream gradient that is not
+    finite reaches its own row of the features' gradient and the gradients of weight and bias, as in torch.  Products of 16-bit operands accumulate in fp32; the
     gradient of the logits is rounded to the operands' type where the matrix instructions of the two gradient products take it (in
     large calls the probabilities of the other classes once before that, when they are kept for the backward).  Under stream capture no
     eager graph over the operands may be alive (an error).  Works on any view with a dense last dimension; others are copied."""
