@@ -90,3 +90,45 @@ def test_an_upstream_gradient_that_is_not_finite_stays_in_its_row(n, d, v, dtype
         labelled = t != -100
         rows = labelled if value != 0.0 else ~others
         assert not bool(got[0][rows].isfinite().any()) and int(got[0][~rows].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("n", [4096, 4097, 8192 + 15, 600_001, (1 << 22) + 4097])
+@pytest.mark.parametrize("share", [0.0, 0.5, 0.999])
+def test_many_rows(n, share):
+    """Labelled rows are counted block by block: two classes and one feature, so that value and gradient have closed forms, at rows before, at
+    and behind the borders of those blocks.  Logits +-x/2 of few bits: loss log(1 + exp(-+x)), off by 8 * 2^-24 of 1 + its size."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    x = (torch.randint(-64, 65, (n, 1), generator=g, device=DEV) / 16.0).requires_grad_()
+    w = torch.tensor([[0.5], [-0.5]], device=DEV)
+    t = torch.randint(0, 2, (n,), generator=g, device=DEV)
+    t[torch.rand(n, generator=g, device=DEV) < share] = -100
+    rows = _loss((x, w, None), t, reduction="none")
+    (dx,) = torch.autograd.grad(rows, x, torch.ones_like(rows))
+    z = x.detach().double().flatten() * torch.where(t == 1, -1.0, 1.0)           # label's logit - the other's
+    want = torch.where(t == -100, torch.zeros_like(z), torch.nn.functional.softplus(-z, threshold=100.0))
+    assert bool(((rows.detach().double() - want).abs() <= 8 * 2.0 ** -24 * (1 + want)).all())
+    slope = torch.where(t == -100, torch.zeros_like(z), -torch.sigmoid(-z) * torch.where(t == 1, -1.0, 1.0))
+    # two products of a probability (8 * 2^-24 of it) and 0.5, exact; the two planes' sums in fp32
+    assert bool(((dx.double().flatten() - slope).abs() <= 16 * 2.0 ** -24 * slope.abs() + 2.0 ** -100).all())
+    total = _loss((x.detach(), w, None), t, reduction="sum")
+    assert abs(float(total) - float(want.sum())) <= 8 * 2.0 ** -24 * float((1 + want).sum()) + 2.0 ** -24 * float(want.sum())
+    assert torch.equal(total.isfinite(), torch.ones((), dtype=torch.bool, device=DEV))
+
+
+def test_time_grows_with_the_rows():
+    """Eight times the rows take about eight times as long: a count that every block makes for itself takes sixty-four."""
+    def us(n):
+        x = torch.zeros((n, 8), dtype=torch.float16, device=DEV)
+        w, t = torch.zeros((2, 8), dtype=torch.float16, device=DEV), torch.zeros(n, dtype=torch.int64, device=DEV)
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            _loss((x, w, None), t, reduction="none")
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b) * 1000)
+        return best
+    times = [us(n) for n in (1 << 20, 1 << 23)]
+    print("us", times)
+    assert times[1] <= 16 * times[0], times

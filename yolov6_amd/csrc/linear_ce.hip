@@ -96,12 +96,16 @@ __device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_ex
 __device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_logf(v); }
 
 // ------------------------------------------------------------------------------------------------------------- rows with a label
-// Block b takes rows [16 b, 16 b + 16): counts the labelled rows before them (at most kCountRows / 1024 loads a thread; with more rows a
-// kernel of its own counts per block first), then copies its labelled rows to their places, each padded with zeros to a multiple of
-// 16 bytes, a row per wave.
+// Block b of gather_kernel takes rows [16 b, 16 b + 16): finds how many labelled rows lie before them, then copies its labelled rows to
+// their places, each padded with zeros to a multiple of 16 bytes, a row per wave.  Up to kCountRows rows it counts them itself (4 loads a
+// thread at most).  Above, count_kernel counts kCountRows rows a block and leaves each 16 rows' place within them and the block's total; a
+// gather block adds up the totals before its own, one load a thread at most, and with more than kTotals of them scan_kernel has done that
+// once: the work grows with the rows (value of 2^20 rows x 8 x 2 classes, fp16, 0.51 ms, of 2^23 rows 3.85; with every block adding the
+// counts of all blocks before it 0.89 and 30.7).
 constexpr int kGatherRows = 16;
 constexpr int kGatherThreads = kGatherRows * 64;
 constexpr int kCountRows = 4096;
+constexpr int kTotals = kGatherThreads;
 
 struct GatherArgs {
     const char* x;
@@ -110,7 +114,9 @@ struct GatherArgs {
     long long ignore;
     int rows, width, classes;
     int vec;                       // rows start at 16-byte addresses, and 16-bit ones are multiples of 16 bytes
-    const int* seg;                // labelled rows per block (above kCountRows), or null
+    const int* seg;                // above kCountRows rows: labelled rows before each 16 within their kCountRows; or null
+    const int* total;              // of each kCountRows, or, `scanned`, of all before them
+    int scanned;
     char* xc;
     long long cpitch, plane;       // bytes between rows, planes
     int* rowmap;                   // place -> row
@@ -131,10 +137,56 @@ __device__ __forceinline__ int block_count(int mine, int* sh) {       // sum ove
     return r;
 }
 
-__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg, int segs) {
-    const int r = blockIdx.x * 256 + threadIdx.x, s = r / kGatherRows;
-    const unsigned long long m = __ballot(r < rows && target[r < rows ? r : 0] != ignore);
-    if (s < segs && r % kGatherRows == 0) seg[s] = __popcll((m >> (threadIdx.x & 63)) & ((1ull << kGatherRows) - 1));
+__device__ __forceinline__ int wave_scan(int v, int lane) {           // inclusive
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int o = __shfl_up(v, d);
+        if (lane >= d) v += o;
+    }
+    return v;
+}
+
+__global__ __launch_bounds__(kCountRows / kGatherRows) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg,
+                                                                         int segs, int* __restrict__ total) {
+    constexpr int T = kCountRows / kGatherRows;                          // threads; each has 16 rows in the end
+    __shared__ int n16[T], wave_sum[T / 64];
+    const int r0 = blockIdx.x * kCountRows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int i = 0; i < kGatherRows; ++i) {
+        const int k = i * T + threadIdx.x, r = rows - r0 > k ? r0 + k : -1;
+        const unsigned long long m = __ballot(r >= 0 && target[r >= 0 ? r : 0] != ignore);
+        if (lane % kGatherRows == 0) n16[k / kGatherRows] = __popcll((m >> lane) & ((1ull << kGatherRows) - 1));
+    }
+    __syncthreads();
+    const int mine = n16[threadIdx.x], upto = wave_scan(mine, lane);
+    if (lane == 63) wave_sum[wave] = upto;
+    __syncthreads();
+    int before = upto - mine;
+    for (int w = 0; w < wave; ++w) before += wave_sum[w];
+    const int s = r0 / kGatherRows + threadIdx.x;
+    if (s < segs) seg[s] = before;
+    if (threadIdx.x == T - 1) total[blockIdx.x] = before + mine;
+}
+
+// totals -> sums of those before each; one block, a chunk at a time
+__global__ __launch_bounds__(1024) void scan_kernel(int* __restrict__ total, int n) {
+    __shared__ int wave_sum[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int carry = 0;
+    for (int i0 = 0; i0 < n; i0 += 1024) {
+        const int i = i0 + threadIdx.x, mine = i < n ? total[i] : 0, upto = wave_scan(mine, lane);
+        if (lane == 63) wave_sum[wave] = upto;
+        __syncthreads();
+        int before = carry + upto - mine, all = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            before += w < wave ? wave_sum[w] : 0;
+            all += wave_sum[w];
+        }
+        if (i < n) total[i] = before;
+        carry += all;
+        __syncthreads();
+    }
 }
 
 // the planes of four values of a row, zeros behind its width
@@ -161,12 +213,15 @@ __global__ __launch_bounds__(kGatherThreads) void gather_kernel(const GatherArgs
     __shared__ int place[kGatherRows];
     const int r0 = blockIdx.x * kGatherRows;
     int before = 0;
-    if (a.seg) {
-        for (int i = threadIdx.x; i < (int)blockIdx.x; i += kGatherThreads) before += a.seg[i];
-    } else {
+    if (!a.seg) {
         for (int i = threadIdx.x; i < r0; i += kGatherThreads) before += a.target[i] != a.ignore ? 1 : 0;
+        before = block_count(before, sh);
+    } else {
+        const int c = r0 / kCountRows;
+        if (a.scanned) before = a.total[c];
+        else before = block_count((int)threadIdx.x < c ? a.total[threadIdx.x] : 0, sh);
+        before += a.seg[blockIdx.x];
     }
-    before = block_count(before, sh);
     if (threadIdx.x < 64) {
         const int r = r0 + threadIdx.x;
         const bool mine = threadIdx.x < kGatherRows && r < a.rows;
@@ -1274,7 +1329,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.kept_all = at;
     at = 0;
     if (!backward) {
-        L.seg = take(n > kCountRows ? (size_t)ceil_div(n, kGatherRows) * 4 : 0);
+        L.seg = take(n > kCountRows ? ((size_t)ceil_div(n, kGatherRows) + ceil_div(n, kCountRows)) * 4 : 0);
         L.scores = L.kept_scores;
         // one block for all rows, which then also adds up the loss, where that is 16 rounds of its threads at most
         L.places = 1;
@@ -1339,9 +1394,16 @@ int launch_gather(const Run& r) {
     a.rowmap = r.kept<int>(r.L.rowmap), a.place = r.kept<int>(r.L.place), a.label = r.kept<int>(r.L.label), a.count = r.kept<int>(r.L.count);
     const int segs = ceil_div(d->rows, kGatherRows);
     if (d->rows > kCountRows) {
-        a.seg = r.at<int>(r.L.seg);
-        hipLaunchKernelGGL(count_kernel, dim3(ceil_div(d->rows, 256)), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs);
+        const int totals = ceil_div(d->rows, kCountRows);
+        int* const total = r.at<int>(r.L.seg) + segs;
+        a.seg = r.at<int>(r.L.seg), a.total = total, a.scanned = totals > kTotals;
+        hipLaunchKernelGGL(count_kernel, dim3(totals), dim3(kCountRows / kGatherRows), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg),
+                           segs, total);
         Y6_LAUNCH_CHECK();
+        if (a.scanned) {
+            hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(1024), 0, r.s, total, totals);
+            Y6_LAUNCH_CHECK();
+        }
     }
     if (d->reduction == Y6_REDUCE_NONE) a.loss_rows = d->loss;
     hipLaunchKernelGGL(gather_kernel<E::ES>, dim3(segs), dim3(kGatherThreads), 0, r.s, a);
