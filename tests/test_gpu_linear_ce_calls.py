@@ -132,3 +132,12 @@ def test_time_grows_with_the_rows():
     times = [us(n) for n in (1 << 20, 1 << 23)]
     print("us", times)
     assert times[1] <= 16 * times[0], times
+
+
+def test_bias_gradient_of_many_rows_with_kept_exponentials():
+    """Thousands of partial sums of a class: joined in a fixed order, and right."""
+    x, w, b, t = _inputs(100_003, 128, 1040, torch.bfloat16, True, seed=17)
+    first = _check(x, w, b, t, reduction="sum", kept=True)
+    leaves = _leaves((x, w, b), torch.bfloat16)
+    again = torch.autograd.grad(_loss(leaves, t, reduction="sum"), leaves)
+    assert all(torch.equal(a, c) for a, c in zip(first[1], again))

@@ -1166,14 +1166,25 @@ __global__ __launch_bounds__(256) void kept_kernel(const KeptArgs a) {
     }
 }
 
+// db of a piece from its shares: 32 classes a block, 32 threads each, every one adds up each 32nd share, then the first their sums in order.
+// (Shares grow with the rows, 4096 of them at 262144; classes of a piece may be 256: with one thread a class db took 250 of a call's 1394 us at
+// 262144 rows x 128 x 1024 classes, so 52.)
+constexpr int kJoinCols = 32;
 template <class E>
-__global__ __launch_bounds__(256) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
-                                                        const float* up, const float* gmax, int mean, const int* count) {
-    const int c = blockIdx.x * 256 + threadIdx.x;
-    if (c >= classes) return;
+__global__ __launch_bounds__(1024) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
+                                                         const float* up, const float* gmax, int mean, const int* count) {
+    __shared__ float sh[1024 / kJoinCols][kJoinCols];
+    const int lane = threadIdx.x % kJoinCols, w = threadIdx.x / kJoinCols, c = blockIdx.x * kJoinCols + lane;
     float s = 0.f;
-#pragma unroll 16
-    for (int k = 0; k < shares; ++k) s += part[(long long)k * classes + c];
+    if (c < classes) {
+#pragma unroll 8
+        for (int k = w; k < shares; k += 1024 / kJoinCols) s += part[(long long)k * classes + c];
+    }
+    sh[w][lane] = s;
+    __syncthreads();
+    if (w || c >= classes) return;
+#pragma unroll
+    for (int k = 1; k < 1024 / kJoinCols; ++k) s += sh[k][lane];
     db[c] = E::put(s * grad_factor<E>(up, gmax, mean, count));
 }
 
@@ -1604,7 +1615,7 @@ int backward(const Run& r) {
             Y6_LAUNCH_CHECK();
             }
             if (kept || shares > 1) {
-                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, 256)), dim3(256), 0, r.s, r.at<float>(L.bpart), shares, vn, db, d->grad_out, gmax,
+                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, kJoinCols)), dim3(1024), 0, r.s, r.at<float>(L.bpart), shares, vn, db, d->grad_out, gmax,
                                    mean, count);
                 Y6_LAUNCH_CHECK();
             }
