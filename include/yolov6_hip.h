@@ -816,6 +816,9 @@ int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
  * width padded, an fp32 one in three bf16 planes; the exponentials in the operands' type, up to 2 GiB) and backward reads, with the same operands; NULL for a forward that no backward follows.
  * workspace: y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls.  Both 16-byte aligned. */
 enum { Y6_REDUCE_NONE = 0, Y6_REDUCE_SUM = 1, Y6_REDUCE_MEAN = 2 };
+/* COPY_WEIGHT: the forward copies the weight into `saved` although it could be read where it lies, and the backward reads the copy (then
+ * its `weight` may be any address): for a caller whose weight may lie otherwise by then.  An unaligned or fp32 weight is copied anyway. */
+enum { Y6_CE_COPY_WEIGHT = 1 };
 typedef struct y6_linear_ce_desc {
     const void* x;
     const void* weight;
@@ -824,7 +827,7 @@ typedef struct y6_linear_ce_desc {
     int64_t rows, x_pitch, w_pitch, ignore_index;
     int32_t width, classes, dtype /* Y6_F16 | Y6_BF16 | Y6_F32 */, reduction;
     float smoothing;
-    int32_t pad;
+    int32_t flags;                 /* Y6_CE_*, the same for forward and backward */
     float* loss;                   /* [rows] or one value */
     void* saved;
     size_t saved_bytes;

@@ -141,3 +141,32 @@ def test_bias_gradient_of_many_rows_with_kept_exponentials():
     leaves = _leaves((x, w, b), torch.bfloat16)
     again = torch.autograd.grad(_loss(leaves, t, reduction="sum"), leaves)
     assert all(torch.equal(a, c) for a, c in zip(first[1], again))
+
+
+class _Misplaced(torch.autograd.graph.saved_tensors_hooks):
+    """Hands every saved tensor back one element behind the start of a wider buffer."""
+
+    def __init__(self):
+        def unpack(t):
+            if t.dim() != 2:
+                return t
+            buf = torch.zeros((t.shape[0], t.shape[1] + 3), dtype=t.dtype, device=t.device)
+            buf[:, 1:1 + t.shape[1]] = t
+            return buf[:, 1:1 + t.shape[1]]
+        super().__init__(lambda t: t, unpack)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,v,cut", [(70, 40, 130, 0), (70, 40, 130, 1), (70, 37, 130, 0), (40, 136, 110_003, 0), (40, 136, 110_003, 3)])
+@pytest.mark.parametrize("hooks", [torch.autograd.graph.save_on_cpu, _Misplaced])
+@pytest.mark.parametrize("form", [_loss, _op_loss])
+def test_operands_that_come_back_elsewhere(form, hooks, n, d, v, cut, dtype):
+    """Saved-tensor hooks hand the backward the same values at other addresses and pitches: the same bits."""
+    ops = _inputs(n, d + cut, v, dtype, True, seed=d)
+    x, w = (o[:, cut:].detach().requires_grad_() for o in ops[:2])       # (views of a wider buffer: other pitch, odd start)
+    leaves = (x, w, ops[2].detach().requires_grad_())
+    want = torch.autograd.grad(_loss(leaves, ops[3]), leaves)
+    with hooks():
+        loss = form(leaves, ops[3])
+    got = torch.autograd.grad(loss, leaves)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))

@@ -87,3 +87,21 @@ def test_forward_mode_is_refused(hip_lib):
                 linear_cross_entropy(ops[0], ops[1], t, ops[2])
             with pytest.raises(RuntimeError, match="forward mode"):
                 grad_norm([ops[k]])
+
+
+def test_a_copied_weight_is_a_larger_saved_buffer(hip_lib):
+    """What the host side goes by when a weight comes back from saved-tensor hooks at another address."""
+    import ctypes as C
+    from yolov6_amd import _lib
+    for dtype in (0, 1, 3):
+        for rows, width, classes, pitch, at in ((1, 8, 1, 8, 4096), (4, 8, 5, 8, 4096), (4, 8, 5, 8, 4100), (4, 7, 5, 9, 4096), (3000, 512, 4096, 512, 1 << 20)):
+            d = _lib.LinearCeDesc()
+            d.x = d.target = 4096
+            d.weight, d.rows, d.width, d.classes, d.x_pitch, d.w_pitch, d.dtype = at, rows, width, classes, width, pitch, dtype
+            plain = hip_lib.y6_linear_ce_saved_bytes(C.byref(d))
+            d.flags = 1
+            copied = hip_lib.y6_linear_ce_saved_bytes(C.byref(d))
+            needs = dtype == 1 or (width * 2) % 16 or (pitch * 2) % 16 or at % 16
+            assert plain > 0 and (copied == plain if needs else copied >= plain + classes * width * 2)
+            d.weight, d.w_pitch = 8192, width
+            assert hip_lib.y6_linear_ce_saved_bytes(C.byref(d)) == copied

@@ -229,7 +229,7 @@ class GradList(C.Structure):
 class LinearCeDesc(C.Structure):
     _fields_ = [("x", C.c_void_p), ("weight", C.c_void_p), ("bias", C.c_void_p), ("target", C.c_void_p), ("rows", C.c_int64),
                 ("x_pitch", C.c_int64), ("w_pitch", C.c_int64), ("ignore_index", C.c_int64), ("width", C.c_int32), ("classes", C.c_int32),
-                ("dtype", C.c_int32), ("reduction", C.c_int32), ("smoothing", C.c_float), ("pad", C.c_int32), ("loss", C.c_void_p),
+                ("dtype", C.c_int32), ("reduction", C.c_int32), ("smoothing", C.c_float), ("flags", C.c_int32), ("loss", C.c_void_p),
                 ("saved", C.c_void_p), ("saved_bytes", C.c_size_t), ("grad_out", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
                 ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 

@@ -1291,7 +1291,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     };
     L.planes = fp32 ? 3 : 1;
     L.cpitch = up_to(w * 2, 16);
-    L.copy_w = fp32 || (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
+    L.copy_w = (d->flags & Y6_CE_COPY_WEIGHT) || fp32 || (w * es) % 16 != 0 || (d->w_pitch * es) % 16 != 0 || (uintptr_t)d->weight % 16 != 0;
     L.xc = take((size_t)n * L.cpitch * L.planes);
     L.wc = take(L.copy_w ? (size_t)v * L.cpitch * L.planes : 0);
     L.rowmap = take((size_t)n * 4);

@@ -74,6 +74,13 @@ y6_linear_ce_desc describe(const Tensor& x, const Tensor& w, const Tensor& b, co
     return d;
 }
 
+// whether the kernels read such a weight where it lies; others are copied, row by row
+bool in_place(const Tensor& w) {
+    const int64_t rows = w.size(0), width = w.size(1), size = w.element_size();
+    return (width == 1 || w.stride(1) == 1) && (rows == 1 || (w.stride(0) >= width && w.stride(0) <= (1 << 21) && w.stride(0) * size % 16 == 0)) &&
+           (uintptr_t)w.data_ptr() % 16 == 0;
+}
+
 std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Options& o, bool want_saved) {
     const auto f32 = x.options().dtype(at::kFloat).requires_grad(false);
     const int64_t n = x.size(0);
@@ -110,10 +117,18 @@ std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor&
     const Tensor dx = want_x ? at::empty({n, width}, like) : Tensor(), dw = want_w ? at::empty({classes, width}, like) : Tensor(),
                  db = want_b ? at::empty({classes}, like) : Tensor();
     if (!want_x && !want_w && !want_b) return {dx, dw, db};
-    const Tensor g = grad.detach().to(at::kFloat).contiguous();
-    y6_linear_ce_desc d = describe(x, w, b, t, o);
-    TORCH_CHECK((size_t)saved.numel() == lib.ce_saved(&d),
-                "yolov6_amd: linear_cross_entropy's backward is given other operands, or operands that lie otherwise, than its forward");
+    const Tensor g = grad.detach().to(at::kFloat).contiguous(), bias = b.defined() ? b.contiguous() : b;
+    // Whether the forward took a copy of the weight went by where it lay; saved-tensor hooks may hand it back elsewhere.  The size of
+    // `saved` tells: with a copy (16 bytes at least) it is larger.
+    y6_linear_ce_desc d = describe(x, w, bias, t, o);
+    d.flags |= Y6_CE_COPY_WEIGHT;
+    d.weight = saved.data_ptr(), d.w_pitch = width;          // (not read then)
+    Tensor moved;
+    if ((size_t)saved.numel() != lib.ce_saved(&d)) {
+        moved = in_place(w) ? w : w.clone(at::MemoryFormat::Contiguous);
+        d = describe(x, moved, bias, t, o);
+        TORCH_CHECK((size_t)saved.numel() == lib.ce_saved(&d), "yolov6_amd: linear_cross_entropy's backward is given other operands than its forward");
+    }
     d.saved = saved.data_ptr(), d.saved_bytes = (size_t)saved.numel(), d.grad_out = g.data_ptr<float>();
     d.dx = want_x ? dx.data_ptr() : nullptr, d.dw = want_w ? dw.data_ptr() : nullptr, d.dbias = want_b ? db.data_ptr() : nullptr;
     d.workspace_bytes = lib.ce_workspace(&d, 1);
