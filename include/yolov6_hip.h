@@ -813,7 +813,7 @@ int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
  * A label that is neither a class nor ignore_index makes the row's loss, and every gradient, NaN.  Rows with ignore_index are not
  * read and get zeros.  x: rows x_pitch elements apart (0: all rows the same); weight: w_pitch >= width.  All in one type.
  * saved: y6_linear_ce_saved_bytes(d) that forward writes (the labelled rows gathered, their statistics; a weight of an unaligned
- * width padded, an fp32 one in three bf16 planes; the exponentials in the operands' type, up to 2 GiB) and backward reads, with the same operands; NULL for a forward that no backward follows.
+ * width padded, an fp32 one in three bf16 planes; the exponentials in the operands' type, up to 2 GiB) and backward reads, with the same operands (x and target are not read again); NULL for a forward that no backward follows.
  * workspace: y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls.  Both 16-byte aligned. */
 enum { Y6_REDUCE_NONE = 0, Y6_REDUCE_SUM = 1, Y6_REDUCE_MEAN = 2 };
 /* COPY_WEIGHT: the forward copies the weight into `saved` although it could be read where it lies, and the backward reads the copy (then

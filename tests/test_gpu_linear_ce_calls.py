@@ -170,3 +170,18 @@ def test_operands_that_come_back_elsewhere(form, hooks, n, d, v, cut, dtype):
         loss = form(leaves, ops[3])
     got = torch.autograd.grad(loss, leaves)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_the_features_go_when_the_caller_drops_them(dtype):
+    """The backward reads the labelled rows as the forward gathered them: an activation lives no longer than its caller keeps it."""
+    ops = _inputs(4000, 500, 30, dtype, True, seed=3)
+    leaves = _leaves(ops, dtype)
+    want = torch.autograd.grad(_loss(leaves, ops[3]), leaves)
+    feats = leaves[0] + 0
+    loss = _loss((feats, *leaves[1:]), ops[3])
+    torch.cuda.synchronize()
+    held, size = torch.cuda.memory_allocated(), feats.numel() * feats.element_size()
+    del feats
+    assert held - torch.cuda.memory_allocated() >= size
+    assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(loss, leaves), want))

@@ -64,11 +64,11 @@ struct Options {
     int64_t reduction;
 };
 
-y6_linear_ce_desc describe(const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Options& o) {
+// all but features and labels
+y6_linear_ce_desc describe(int64_t rows, const Tensor& w, const Tensor& b, const Options& o) {
     y6_linear_ce_desc d = {};
-    d.x = x.data_ptr(), d.weight = w.data_ptr(), d.bias = b.defined() ? b.data_ptr() : nullptr, d.target = t.data_ptr<int64_t>();
-    d.rows = x.size(0), d.width = (int32_t)x.size(1), d.classes = (int32_t)w.size(0), d.dtype = type_code(x.scalar_type());
-    d.x_pitch = d.rows > 1 ? x.stride(0) : d.width;
+    d.weight = w.data_ptr(), d.bias = b.defined() ? b.data_ptr() : nullptr;
+    d.rows = rows, d.width = (int32_t)w.size(1), d.classes = (int32_t)w.size(0), d.dtype = type_code(w.scalar_type());
     d.w_pitch = d.classes > 1 ? w.stride(0) : d.width;
     d.ignore_index = o.ignore, d.smoothing = (float)o.smoothing, d.reduction = (int32_t)o.reduction;
     return d;
@@ -88,7 +88,8 @@ std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Te
     if (n == 0) return {rows ? at::empty({0}, f32) : at::zeros({}, f32), bytes_on(x, 0)};
     const c10::DeviceGuard guard(x.device());
     Tensor loss = rows ? at::empty({n}, f32) : at::empty({}, f32), saved;
-    y6_linear_ce_desc d = describe(x, w, b, t, o);
+    y6_linear_ce_desc d = describe(n, w, b, o);
+    d.x = x.data_ptr(), d.x_pitch = n > 1 ? x.stride(0) : d.width, d.target = t.data_ptr<int64_t>();
     d.loss = loss.data_ptr<float>();
     if (want_saved) {
         d.saved_bytes = lib.ce_saved(&d);
@@ -104,12 +105,12 @@ std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Te
     return {loss, saved};
 }
 
-std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& b, const Tensor& t, const Tensor& saved,
-                                               const Options& o, bool want_x, bool want_w, bool want_b) {
+std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, int64_t n, const Tensor& w, const Tensor& b, const Tensor& saved, const Options& o, bool want_x,
+                                               bool want_w, bool want_b) {
     want_b = want_b && b.defined();
-    const auto like = x.options().requires_grad(false);
-    const int64_t n = x.size(0), width = x.size(1), classes = w.size(0);
-    const c10::DeviceGuard guard(x.device());
+    const auto like = w.options().requires_grad(false);
+    const int64_t width = w.size(1), classes = w.size(0);
+    const c10::DeviceGuard guard(w.device());
     if (n == 0) {
         return {want_x ? at::zeros({0, width}, like) : Tensor(), want_w ? at::zeros({classes, width}, like) : Tensor(),
                 want_b ? at::zeros({classes}, like) : Tensor()};
@@ -120,22 +121,24 @@ std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, const Tensor&
     const Tensor g = grad.detach().to(at::kFloat).contiguous(), bias = b.defined() ? b.contiguous() : b;
     // Whether the forward took a copy of the weight went by where it lay; saved-tensor hooks may hand it back elsewhere.  The size of
     // `saved` tells: with a copy (16 bytes at least) it is larger.
-    y6_linear_ce_desc d = describe(x, w, bias, t, o);
+    y6_linear_ce_desc d = describe(n, w, bias, o);
+    d.x = saved.data_ptr(), d.x_pitch = width, d.target = (const int64_t*)saved.data_ptr();           // (the backward reads neither)
     d.flags |= Y6_CE_COPY_WEIGHT;
     d.weight = saved.data_ptr(), d.w_pitch = width;          // (not read then)
     Tensor moved;
     if ((size_t)saved.numel() != lib.ce_saved(&d)) {
         moved = in_place(w) ? w : w.clone(at::MemoryFormat::Contiguous);
-        d = describe(x, moved, bias, t, o);
+        const auto at = describe(n, moved, bias, o);
+        d.flags = at.flags, d.weight = at.weight, d.w_pitch = at.w_pitch;
         TORCH_CHECK((size_t)saved.numel() == lib.ce_saved(&d), "yolov6_amd: linear_cross_entropy's backward is given other operands than its forward");
     }
     d.saved = saved.data_ptr(), d.saved_bytes = (size_t)saved.numel(), d.grad_out = g.data_ptr<float>();
     d.dx = want_x ? dx.data_ptr() : nullptr, d.dw = want_w ? dw.data_ptr() : nullptr, d.dbias = want_b ? db.data_ptr() : nullptr;
     d.workspace_bytes = lib.ce_workspace(&d, 1);
     if (d.workspace_bytes == 0) check(Y6_EINVAL, "linear_ce_backward");
-    const Tensor ws = bytes_on(x, d.workspace_bytes);
+    const Tensor ws = bytes_on(w, d.workspace_bytes);
     d.workspace = ws.data_ptr();
-    check(lib.ce_backward(&d, stream_of(x.device())), "linear_ce_backward");
+    check(lib.ce_backward(&d, stream_of(w.device())), "linear_ce_backward");
     return {dx, dw, db};
 }
 
@@ -145,7 +148,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         const Tensor b = bias.has_value() ? *bias : Tensor();
         const Options o = {ignore, smoothing, reduction};
         auto [loss, saved] = ce_forward(x, w, b, t, o, true);
-        ctx->save_for_backward({x, w, b, t, saved});
+        // (neither features nor labels: the backward reads what the forward gathered of them, and they may go)
+        ctx->save_for_backward({w, b, saved});
+        ctx->saved_data["rows"] = x.size(0);
         ctx->saved_data["ignore"] = ignore;
         ctx->saved_data["smoothing"] = smoothing;
         ctx->saved_data["reduction"] = reduction;
@@ -157,8 +162,8 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         variable_list out;
         {
             const at::AutoGradMode off(false);
-            auto [dx, dw, db] = ce_backward(grads[0], s[0], s[1], s[2], s[3], s[4], o, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
-                                            s[2].defined() && ctx->needs_input_grad(2));
+            auto [dx, dw, db] = ce_backward(grads[0], ctx->saved_data["rows"].toInt(), s[0], s[1], s[2], o, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
+                                            s[1].defined() && ctx->needs_input_grad(2));
             out = {dx, dw, db};
         }
         if (at::GradMode::is_enabled()) {       // create_graph: once differentiable
@@ -356,7 +361,7 @@ PYBIND11_MODULE(_y6_torch, m) {
                                               int64_t ignore, double smoothing, const std::string& reduction) {
         const at::NoGradGuard off;
         const Operands p = operands(x, w, t, b, ignore, smoothing, reduction);
-        auto [dx, dw, db] = ce_backward(grad.reshape({-1}), p.x, p.w, p.b, p.t, saved, p.o, true, true, p.b.defined());
+        auto [dx, dw, db] = ce_backward(grad.reshape({-1}), p.x.size(0), p.w, p.b, saved, p.o, true, true, p.b.defined());
         return std::make_tuple(dx.reshape(x.sizes()), dw, p.b.defined() ? db : at::empty({0}, dw.options()));
     });
     m.def("grad_norm", &grad_norm);
