@@ -185,3 +185,39 @@ def test_the_features_go_when_the_caller_drops_them(dtype):
     del feats
     assert held - torch.cuda.memory_allocated() >= size
     assert all(torch.equal(a, c) for a, c in zip(torch.autograd.grad(loss, leaves), want))
+
+
+@pytest.mark.parametrize("how", ["backward", "grad"])
+def test_capture_beside_a_living_graph_of_a_side_stream(how):
+    """Warm-up on a side stream whose loss is still held, as in torch's recipe: that stream joins the capture.  Replays alternate with eager
+    steps on new inputs."""
+    x, w, b, t = _inputs(64, 40, 300, torch.bfloat16, True, seed=6)
+    leaves = _leaves((x, w, b), torch.bfloat16)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = _loss(leaves, t)
+        loss.backward()
+    torch.cuda.current_stream().wait_stream(side)
+    for o in leaves:
+        o.grad = None
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        inner = _loss(leaves, t)
+        if how == "backward":
+            inner.backward()
+            held = [o.grad for o in leaves]
+        else:
+            held = torch.autograd.grad(inner, leaves)
+    for seed in (7, 8, 9):
+        fresh = _inputs(64, 40, 300, torch.bfloat16, True, seed=seed)
+        with torch.no_grad():
+            for p, q in zip((*leaves, t), fresh):
+                p.copy_(q)
+        g.replay()
+        torch.cuda.synchronize()
+        others = _leaves(leaves, torch.bfloat16)
+        want = torch.autograd.grad(_loss(others, t), others)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, c) for a, c in zip(held, want)), seed
+    assert math.isfinite(float(loss.detach()))

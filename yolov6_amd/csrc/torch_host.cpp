@@ -182,8 +182,9 @@ std::string shape(const Tensor& t) {
     return s.str();
 }
 
-// While a stream is captured, a leaf's gradient accumulator must be the capture's own: one that a living eager graph made belongs to that
-// graph's stream, the engine would make it wait, and the capture's end brings the process down.
+// While a stream is captured, a leaf's gradient accumulator must not be one that a living eager graph made on the default stream: the
+// engine would make that stream wait for the captured one, which it cannot join, and the capture's end brings the process down.  (Another
+// stream joins the capture: a warm-up on a side stream may keep its loss.)
 void refuse_outer_graph(const std::initializer_list<const Tensor*>& operands) {
     for (const Tensor* t : operands) {
         if (!t->defined() || !t->requires_grad() || !t->is_leaf()) continue;
@@ -191,9 +192,10 @@ void refuse_outer_graph(const std::initializer_list<const Tensor*>& operands) {
         hipStreamCaptureStatus state = hipStreamCaptureStatusNone;
         if (hipStreamIsCapturing(stream.stream(), &state) != hipSuccess || state == hipStreamCaptureStatusNone) return;
         const auto node = torch::autograd::impl::try_get_grad_accumulator(*t);
-        TORCH_CHECK(!node || node->input_metadata(0).stream() == stream.unwrap(),
-                    "yolov6_amd: linear_cross_entropy is captured into a graph while an eager graph over one of its operands is alive "
-                    "(drop the loss that holds it before the capture, capture on the stream it was made on, or with a detached operand)");
+        // (by their ids: the two carry different device types, and the streams themselves are never equal)
+        TORCH_CHECK(!node || node->input_metadata(0).stream().id() != c10::hip::getDefaultHIPStream(t->device().index()).id(),
+                    "yolov6_amd: linear_cross_entropy is captured into a graph while an eager graph over one of its operands, made on the default stream, is "
+                    "alive (drop the loss that holds it before the capture, make it on another stream, or capture with a detached operand)");
     }
 }
 

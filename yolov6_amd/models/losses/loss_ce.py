@@ -26,5 +26,5 @@ def linear_cross_entropy(features, weight, target, bias=None, *, ignore_index=-1
     finite reaches its own row of the features' gradient and the gradients of weight and bias, as in torch.  Products of 16-bit operands accumulate in fp32; the
     gradient of the logits is rounded to the operands' type where the matrix instructions of the two gradient products take it (in
     large calls the probabilities of the other classes once before that, when they are kept for the backward).  Under stream capture no
-    eager graph over the operands may be alive (an error).  Works on any view with a dense last dimension; others are copied."""
+    eager graph over the operands that was made on the default stream may be alive (an error).  Works on any view with a dense last dimension; others are copied."""
     return _lib.torch_host().linear_cross_entropy(features, weight, target, bias, ignore_index, label_smoothing, reduction)
