@@ -221,3 +221,31 @@ def test_capture_beside_a_living_graph_of_a_side_stream(how):
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(held, want)), seed
     assert math.isfinite(float(loss.detach()))
+
+
+def test_the_op_captured_beside_a_living_eager_graph_is_refused():
+    x, w, b, t = _inputs(64, 40, 30, torch.bfloat16, True, seed=6)
+    for k in range(3):
+        ops = [o.detach().requires_grad_(i == k) for i, o in enumerate((x, w, b))]
+        loss = _op_loss(ops, t)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            torch.zeros(1, device=DEV)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                _op_loss(ops, t)
+            with pytest.raises(RuntimeError, match="eager graph"), torch.autocast("cuda", dtype=torch.float16):
+                _op_loss(ops, t)
+            with torch.no_grad():
+                value = _op_loss(ops, t)                     # no gradient, no accumulator
+        want = torch.autograd.grad(loss, ops[k])[0]
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(value, loss.detach())
+        del loss
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            held = torch.autograd.grad(_op_loss(ops, t), ops[k])[0]
+        for _ in range(3):
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(held, want)

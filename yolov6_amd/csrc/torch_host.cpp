@@ -352,6 +352,10 @@ PYBIND11_MODULE(_y6_torch, m) {
                (decltype(lib.ce_backward))f[4], (decltype(lib.norm_workspace))f[5], (decltype(lib.norm))f[6], (decltype(lib.clip))f[7]};
     });
     m.def("linear_cross_entropy", &linear_cross_entropy);
+    m.def("linear_cross_entropy_refuse_outer_graph", [](const Tensor& x, const Tensor& w, const std::optional<Tensor>& b) {
+        const Tensor given = b.has_value() ? *b : Tensor();
+        refuse_outer_graph({&x, &w, &given});
+    });
     m.def("linear_cross_entropy_forward", [](const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, int64_t ignore, double smoothing,
                                              const std::string& reduction) {
         const at::NoGradGuard off;

@@ -131,8 +131,16 @@ def _(grad, features, weight, target, bias, saved, ignore_index, label_smoothing
     return (features.new_empty(features.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else (weight.shape[0],)))
 
 
+def _ce_capture(features, weight, bias):
+    """What models/losses/loss_ce.py refuses under stream capture, for a call that a backward may follow."""
+    if torch.cuda.is_initialized() and torch.cuda.is_current_stream_capturing():
+        from . import _lib
+        _lib.torch_host().linear_cross_entropy_refuse_outer_graph(features, weight, bias)
+
+
 def _ce_setup(ctx, inputs, output):
     features, weight, target, bias, *ctx.options = inputs
+    _ce_capture(features, weight, bias)
     ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(features, weight, target, bias, output[1])
 
@@ -148,6 +156,8 @@ linear_cross_entropy.register_autograd(_ce_grad, setup_context=_ce_setup)
 
 def _ce_autocast(features, weight, target, bias, *options):
     """The casts come before the op, so that they are differentiated and its backward sees the operands of its forward, wherever it runs."""
+    if torch.is_grad_enabled():
+        _ce_capture(features, weight, bias)                  # (what is cast is a leaf no longer)
     dtype = torch.get_autocast_dtype("cuda")
     with torch._C._ExcludeDispatchKeyGuard(torch._C.DispatchKeySet(torch._C.DispatchKey.AutocastCUDA)):
         return torch.ops.yolov6_hip.linear_cross_entropy(features.to(dtype), weight.to(dtype), target, None if bias is None else bias.to(dtype), *options)
