@@ -804,7 +804,7 @@ int y6_loss_forward_backward(const y6_loss_grad_desc* d, void* stream);
 /* gradient only: d->fwd.out must hold the result of y6_loss_forward on the same operands */
 int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
 
-/* Softmax cross entropy of a linear classifier over many classes, without the logits in memory (no counterpart in the reference, whose
+/* Softmax cross entropy of a linear classifier over many classes, in tiles: the logits are never stored (no counterpart in the reference, whose
  * classification losses are sigmoid; the semantics are F.cross_entropy(F.linear(x, weight, bias), target)'s):
  *   z_nv = x_n . weight_v + bias_v;  lse_n = log sum_v exp z_nv
  *   loss_n = lse_n - (1 - smoothing) z_n,target(n) - (smoothing / classes) sum_v z_nv, 0 where target(n) == ignore_index
@@ -813,12 +813,14 @@ int y6_loss_backward(const y6_loss_grad_desc* d, void* stream);
  * A label that is neither a class nor ignore_index makes the row's loss, and every gradient, NaN.  Rows with ignore_index are not
  * read and get zeros.  x: rows x_pitch elements apart (0: all rows the same); weight: w_pitch >= width.  All in one type.
  * saved: y6_linear_ce_saved_bytes(d) that forward writes (the labelled rows gathered, their statistics; a weight of an unaligned
- * width padded, an fp32 one in three bf16 planes; the exponentials in the operands' type, up to 2 GiB) and backward reads, with the same operands (x and target are not read again); NULL for a forward that no backward follows.
+ * width padded, an fp32 one in three bf16 planes; the exponentials in the operands' type, rows x classes of
+ * them, up to 2 GiB, unless Y6_CE_RECOMPUTE) and backward reads, with the same operands (x and target are not read again); NULL for a forward that no backward follows.
  * workspace: y6_linear_ce_workspace_bytes(d, 0 forward | 1 backward); nothing is kept in it between calls.  Both 16-byte aligned. */
 enum { Y6_REDUCE_NONE = 0, Y6_REDUCE_SUM = 1, Y6_REDUCE_MEAN = 2 };
 /* COPY_WEIGHT: the forward copies the weight into `saved` although it could be read where it lies, and the backward reads the copy (then
- * its `weight` may be any address): for a caller whose weight may lie otherwise by then.  An unaligned or fp32 weight is copied anyway. */
-enum { Y6_CE_COPY_WEIGHT = 1 };
+ * its `weight` may be any address): for a caller whose weight may lie otherwise by then.  An unaligned or fp32 weight is copied anyway.
+ * RECOMPUTE: nothing of [rows][classes] is kept, the backward forms the scores again. */
+enum { Y6_CE_COPY_WEIGHT = 1, Y6_CE_RECOMPUTE = 2 };
 typedef struct y6_linear_ce_desc {
     const void* x;
     const void* weight;

@@ -249,3 +249,34 @@ def test_the_op_captured_beside_a_living_eager_graph_is_refused():
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(held, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("reduction,smoothing", [("mean", 0.0), ("none", 0.1)])
+def test_recompute(dtype, reduction, smoothing, monkeypatch):
+    """Nothing of [rows, classes] is kept, and the gradients have one rounding less: the tolerance is that of calls that keep nothing."""
+    from functools import partial
+    from yolov6_amd.models.losses import loss_ce
+    n, d, v = 4100, 264, 4200
+    ops = _inputs(n, d, v, dtype, True, seed=n)
+    up = torch.tensor(16.0 * n if dtype == torch.float16 else 1.0, device=DEV)
+    if reduction == "none":
+        up = torch.linspace(-2, 3, n, device=DEV)
+    logits = n * v * ops[0].element_size()
+    leaves = _leaves(ops, dtype)
+    for recompute in (False, True):
+        for form in (_loss, _op_loss):
+            before = torch.cuda.memory_allocated()
+            if form is _loss:
+                loss = _loss(leaves, ops[3], recompute=recompute)
+            else:
+                loss = _op_loss(leaves, ops[3], -100, 0.0, "mean", recompute)
+            torch.cuda.synchronize()
+            held = torch.cuda.memory_allocated() - before
+            assert held < logits / 2 if recompute else held >= logits
+            del loss
+    monkeypatch.setattr(loss_ce, "linear_cross_entropy", partial(loss_ce.linear_cross_entropy, recompute=True))
+    _, want = _check(*ops, smoothing, reduction, up, kept=False)
+    loss = _op_loss(leaves, ops[3], -100, smoothing, reduction, True)
+    got = torch.autograd.grad(loss, leaves, up)
+    assert all(torch.equal(a, c) for a, c in zip(got, want))

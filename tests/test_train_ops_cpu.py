@@ -105,3 +105,16 @@ def test_a_copied_weight_is_a_larger_saved_buffer(hip_lib):
             assert plain > 0 and (copied == plain if needs else copied >= plain + classes * width * 2)
             d.weight, d.w_pitch = 8192, width
             assert hip_lib.y6_linear_ce_saved_bytes(C.byref(d)) == copied
+
+
+def test_recompute_keeps_nothing_of_rows_by_classes(hip_lib):
+    import ctypes as C
+    from yolov6_amd import _lib
+    for dtype, size in ((0, 2), (1, 4), (3, 2)):
+        d = _lib.LinearCeDesc()
+        d.x = d.target = d.weight = 4096
+        d.rows, d.width, d.classes, d.x_pitch, d.w_pitch, d.dtype = 8192, 512, 8192, 512, 512, dtype
+        kept = hip_lib.y6_linear_ce_saved_bytes(C.byref(d))
+        d.flags = 2
+        without = hip_lib.y6_linear_ce_saved_bytes(C.byref(d))
+        assert kept >= 8192 * 8192 * size and 0 < without <= 2 * 8192 * 512 * 6 + (1 << 20)

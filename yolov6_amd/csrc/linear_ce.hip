@@ -11,7 +11,8 @@
 //   backward    for a piece of the vocabulary: dz from the kept exponentials (kept_kernel, a memory pass) or, where there are none, from z
 //               formed again; 16 bits for 16-bit inputs, the operand that the matrix instructions of the next two products take.  Then
 //               dx += dz W[piece] and dW[piece] = dz^T x in one launch (gemm_tile)
-// so a call holds one piece of dz (kPieceBytes) and what is kept, never the logits.  A kept exponential is rounded and dz once more
+// so a call holds one piece of dz (kPieceBytes) and what is kept, which is as large as logits of the operands' type up to kKeepBytes; a
+// caller who would rather have the memory, or the one rounding less, says so (Y6_CE_RECOMPUTE).  A kept exponential is rounded and dz once more
 // (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9 ms, 0.95
 // PFLOP/s over the three products; without the kept ones 8.1.  torch's product of such operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on
 // the same card, which lowers its clock under either.
@@ -1327,7 +1328,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     if (rows < 256) rows = 256;
     L.stat_rows = (int)(rows < n ? rows : n);
     L.np = up_to(L.stat_rows, 64);
-    if (w >= kKeepWidth[fp32] && v >= kKeepClasses[fp32] && n * v >= kKeepScores[fp32]) {
+    if (!(d->flags & Y6_CE_RECOMPUTE) && w >= kKeepWidth[fp32] && v >= kKeepClasses[fp32] && n * v >= kKeepScores[fp32]) {
         const long long most = (long long)(kKeepBytes / ((size_t)n * piece * es));
         L.keeps = (int)(most >= L.pieces ? v : most * piece);
     }

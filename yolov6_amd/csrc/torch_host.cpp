@@ -62,6 +62,7 @@ struct Options {
     int64_t ignore;
     double smoothing;
     int64_t reduction;
+    bool recompute;
 };
 
 // all but features and labels
@@ -71,6 +72,7 @@ y6_linear_ce_desc describe(int64_t rows, const Tensor& w, const Tensor& b, const
     d.rows = rows, d.width = (int32_t)w.size(1), d.classes = (int32_t)w.size(0), d.dtype = type_code(w.scalar_type());
     d.w_pitch = d.classes > 1 ? w.stride(0) : d.width;
     d.ignore_index = o.ignore, d.smoothing = (float)o.smoothing, d.reduction = (int32_t)o.reduction;
+    d.flags = o.recompute ? Y6_CE_RECOMPUTE : 0;
     return d;
 }
 
@@ -144,9 +146,9 @@ std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, int64_t n, co
 
 struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const std::optional<Tensor>& bias, const Tensor& t, int64_t ignore,
-                          double smoothing, int64_t reduction) {
+                          double smoothing, int64_t reduction, bool recompute) {
         const Tensor b = bias.has_value() ? *bias : Tensor();
-        const Options o = {ignore, smoothing, reduction};
+        const Options o = {ignore, smoothing, reduction, recompute};
         auto [loss, saved] = ce_forward(x, w, b, t, o, true);
         // (neither features nor labels: the backward reads what the forward gathered of them, and they may go)
         ctx->save_for_backward({w, b, saved});
@@ -154,11 +156,13 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         ctx->saved_data["ignore"] = ignore;
         ctx->saved_data["smoothing"] = smoothing;
         ctx->saved_data["reduction"] = reduction;
+        ctx->saved_data["recompute"] = recompute;
         return loss;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto s = ctx->get_saved_variables();
-        const Options o = {ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(), ctx->saved_data["reduction"].toInt()};
+        const Options o = {ctx->saved_data["ignore"].toInt(), ctx->saved_data["smoothing"].toDouble(), ctx->saved_data["reduction"].toInt(),
+                           ctx->saved_data["recompute"].toBool()};
         variable_list out;
         {
             const at::AutoGradMode off(false);
@@ -172,7 +176,7 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
             for (auto& g : out) marked.push_back(g.defined() ? g.set_requires_grad(true) : g);
             out = (*stop)(std::move(marked));
         }
-        return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor()};
+        return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
@@ -205,7 +209,7 @@ struct Operands {
 };
 // Operands as the kernels take them: features [rows, width], weight [classes, width], target [rows]
 Operands operands(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias_in, int64_t ignore, double smoothing,
-                  const std::string& reduction) {
+                  const std::string& reduction, bool recompute) {
     const Tensor bias = bias_in.has_value() ? *bias_in : Tensor();
     for (const Tensor& t : {features, weight, bias}) refuse_forward_mode(t, "linear_cross_entropy");
     const int64_t code = reduction == "none" ? Y6_REDUCE_NONE : reduction == "sum" ? Y6_REDUCE_SUM : reduction == "mean" ? Y6_REDUCE_MEAN : -1;
@@ -231,22 +235,24 @@ Operands operands(const Tensor& features, const Tensor& weight, const Tensor& ta
     Tensor x = features.dim() == 2 ? features : features.reshape({target.numel(), features.size(-1)}), w = weight;
     if (x.size(1) > 1 && x.stride(1) != 1) x = x.contiguous();
     if ((w.size(1) > 1 && w.stride(1) != 1) || (w.size(0) > 1 && (w.stride(0) < w.size(1) || w.stride(0) > (1 << 21)))) w = w.contiguous();   // (an expanded weight)
-    return {x, w, bias.defined() ? bias.contiguous() : bias, target.reshape({-1}).contiguous(), {ignore, smoothing, code}};
+    return {x, w, bias.defined() ? bias.contiguous() : bias, target.reshape({-1}).contiguous(), {ignore, smoothing, code, recompute}};
 }
 
 Tensor linear_cross_entropy(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias, int64_t ignore,
-                            double smoothing, const std::string& reduction) {
+                            double smoothing, const std::string& reduction, bool recompute) {
     // (here and not in operands(): the dispatcher's ops take their operands as they are, cast in front of them)
     const bool cast = at::autocast::is_autocast_enabled(at::kCUDA);
     const auto as = [&](const Tensor& t) { return cast ? t.to(at::autocast::get_autocast_dtype(at::kCUDA)) : t; };
-    const Operands p = operands(as(features), as(weight), target, bias.has_value() ? std::optional<Tensor>(as(*bias)) : bias, ignore, smoothing, reduction);
+    const Operands p = operands(as(features), as(weight), target, bias.has_value() ? std::optional<Tensor>(as(*bias)) : bias, ignore, smoothing, reduction,
+                                recompute);
     Tensor loss;
     if (at::GradMode::is_enabled()) {
         const Tensor given = bias.has_value() ? *bias : Tensor();
         refuse_outer_graph({&features, &weight, &given});
     }
     if (at::GradMode::is_enabled() && (p.x.requires_grad() || p.w.requires_grad() || (p.b.defined() && p.b.requires_grad())))
-        loss = LinearCrossEntropy::apply(p.x, p.w, p.b.defined() ? std::optional<Tensor>(p.b) : std::nullopt, p.t, p.o.ignore, p.o.smoothing, p.o.reduction);
+        loss = LinearCrossEntropy::apply(p.x, p.w, p.b.defined() ? std::optional<Tensor>(p.b) : std::nullopt, p.t, p.o.ignore, p.o.smoothing, p.o.reduction,
+                                         p.o.recompute);
     else
         loss = std::get<0>(ce_forward(p.x, p.w, p.b, p.t, p.o, false));
     return p.o.reduction == Y6_REDUCE_NONE && target.dim() != 1 ? loss.reshape(target.sizes()) : loss;
@@ -357,16 +363,16 @@ PYBIND11_MODULE(_y6_torch, m) {
         refuse_outer_graph({&x, &w, &given});
     });
     m.def("linear_cross_entropy_forward", [](const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, int64_t ignore, double smoothing,
-                                             const std::string& reduction) {
+                                             const std::string& reduction, bool recompute) {
         const at::NoGradGuard off;
-        const Operands p = operands(x, w, t, b, ignore, smoothing, reduction);
+        const Operands p = operands(x, w, t, b, ignore, smoothing, reduction, recompute);
         auto [loss, saved] = ce_forward(p.x, p.w, p.b, p.t, p.o, true);
         return std::make_tuple(p.o.reduction == Y6_REDUCE_NONE ? loss.reshape(t.sizes()) : loss, saved);
     });
     m.def("linear_cross_entropy_backward", [](const Tensor& grad, const Tensor& x, const Tensor& w, const Tensor& t, const std::optional<Tensor>& b, const Tensor& saved,
-                                              int64_t ignore, double smoothing, const std::string& reduction) {
+                                              int64_t ignore, double smoothing, const std::string& reduction, bool recompute) {
         const at::NoGradGuard off;
-        const Operands p = operands(x, w, t, b, ignore, smoothing, reduction);
+        const Operands p = operands(x, w, t, b, ignore, smoothing, reduction, recompute);
         auto [dx, dw, db] = ce_backward(grad.reshape({-1}), p.x.size(0), p.w, p.b, saved, p.o, true, true, p.b.defined());
         return std::make_tuple(dx.reshape(x.sizes()), dw, p.b.defined() ? db : at::empty({0}, dw.options()));
     });

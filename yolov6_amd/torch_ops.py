@@ -106,28 +106,30 @@ def _(x, weight, bias, act, stride):
 
 @torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy", mutates_args=(), device_types="cuda")
 def linear_cross_entropy(features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], ignore_index: int, label_smoothing: float,
-                         reduction: str) -> Tuple[Tensor, Tensor]:
+                         reduction: str, recompute: bool = False) -> Tuple[Tensor, Tensor]:
     """(loss, bytes that the backward takes over): models/losses/loss_ce.py with a schema.  They are made whether a backward follows or not, up to
-    2 GiB of them: a caller that wants the value alone calls models/losses/loss_ce.py without gradients.  Under autocast the operands are cast first."""
+    2 GiB of them unless `recompute`: a caller that wants the value alone calls models/losses/loss_ce.py without gradients.  Under autocast the operands are cast first."""
     from . import _lib
-    return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction)
+    return _lib.torch_host().linear_cross_entropy_forward(features, weight, target, bias, ignore_index, label_smoothing, reduction, recompute)
 
 
 @linear_cross_entropy.register_fake
-def _(features, weight, target, bias, ignore_index, label_smoothing, reduction):
+def _(features, weight, target, bias, ignore_index, label_smoothing, reduction, recompute=False):
     return (features.new_empty(target.shape if reduction == "none" else (), dtype=torch.float32),
             features.new_empty((torch.library.get_ctx().new_dynamic_size(),), dtype=torch.uint8))
 
 
 @torch.library.custom_op(f"{NAMESPACE}::linear_cross_entropy_backward", mutates_args=(), device_types="cuda")
 def linear_cross_entropy_backward(grad: Tensor, features: Tensor, weight: Tensor, target: Tensor, bias: Optional[Tensor], saved: Tensor,
-                                  ignore_index: int, label_smoothing: float, reduction: str) -> Tuple[Tensor, Tensor, Tensor]:
+                                  ignore_index: int, label_smoothing: float, reduction: str,
+                                  recompute: bool) -> Tuple[Tensor, Tensor, Tensor]:
     from . import _lib
-    return _lib.torch_host().linear_cross_entropy_backward(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction)
+    return _lib.torch_host().linear_cross_entropy_backward(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction,
+                                                             recompute)
 
 
 @linear_cross_entropy_backward.register_fake
-def _(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction):
+def _(grad, features, weight, target, bias, saved, ignore_index, label_smoothing, reduction, recompute):
     return (features.new_empty(features.shape), weight.new_empty(weight.shape), weight.new_empty((0,) if bias is None else (weight.shape[0],)))
 
 
@@ -148,7 +150,7 @@ def _ce_setup(ctx, inputs, output):
 def _ce_grad(ctx, grad, _):
     features, weight, target, bias, saved = ctx.saved_tensors
     dx, dw, db = torch.ops.yolov6_hip.linear_cross_entropy_backward(grad, features, weight, target, bias, saved, *ctx.options)
-    return dx, dw, None, None if bias is None else db, None, None, None
+    return dx, dw, None, None if bias is None else db, None, None, None, None
 
 
 linear_cross_entropy.register_autograd(_ce_grad, setup_context=_ce_setup)
