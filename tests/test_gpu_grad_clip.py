@@ -317,3 +317,14 @@ def test_clipping_counts_as_a_write():
         held = torch.nn.Parameter(torch.zeros(9, device=DEV), requires_grad=False)
         held.grad = torch.full((9,), 2.0, device=DEV)
         assert abs(float(clip_grad_norm_([held], 1.0)) - 6.0) <= 6 * 2.0 ** -23
+
+
+def test_gradients_with_gaps_that_share_a_part():
+    """Those that start apart are not told from ones that share nothing: each element is scaled once, the norm counts each gradient whole."""
+    buf = torch.randn(64, 10, device=DEV)
+    before = buf.double()
+    params = _params([buf[:, :6], buf[:, 4:9], buf[:, 9:]])
+    want = math.sqrt(float(before.square().sum() + before[:, 4:6].square().sum()))
+    norm = clip_grad_norm_(params, 0.5)
+    assert abs(float(norm) - want) <= 2 * 2.0 ** -24 * want
+    assert torch.allclose(buf.double(), before * (0.5 / (want + 1e-6)), rtol=4 * 2.0 ** -24, atol=0)

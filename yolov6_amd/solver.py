@@ -58,7 +58,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     counts once) in place by min(1, max_norm / (norm + 1e-6)), norm = grad_norm of all of them; returns the norm before clipping.
     The semantics of torch.nn.utils.clip_grad_norm_, in two launches for up to 330 tensors, without a host synchronisation unless
     `error_if_nonfinite` asks for the check (then nothing has been scaled when it raises).  Gradients that share memory are
-    refused.  Under a LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
+    refused, those with gaps where they start at the same element (else each counts whole in the norm and what they share is scaled
+    once).  Under a LossScaler clip what the update will see: `FusedSGD.step(scaler, max_norm=...)`."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
     code, max_norm = _norm_code(norm_type), float(max_norm)
     if not max_norm >= 0:
