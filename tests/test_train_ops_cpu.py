@@ -118,3 +118,18 @@ def test_recompute_keeps_nothing_of_rows_by_classes(hip_lib):
         d.flags = 2
         without = hip_lib.y6_linear_ce_saved_bytes(C.byref(d))
         assert kept >= 8192 * 8192 * size and 0 < without <= 2 * 8192 * 512 * 6 + (1 << 20)
+
+
+def test_sizes_whose_launches_would_leave_32_bits_are_refused(hip_lib):
+    """Up to 2^30 rows were accepted; a launch of theirs has 2^36 threads.  The largest that are taken, and one more."""
+    import ctypes as C
+    from yolov6_amd import _lib
+    d = _lib.LinearCeDesc()
+    d.x = d.target = d.weight = 4096
+    d.width = d.x_pitch = d.w_pitch = 8
+    for rows, classes, good in (((1 << 26) - 16, 5, True), ((1 << 26) - 15, 5, False), (1 << 30, 2, False), (4, (1 << 30) - 512, True), (4, 1 << 30, False)):
+        d.rows, d.classes = rows, classes
+        for size in (hip_lib.y6_linear_ce_saved_bytes(C.byref(d)), hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 0), hip_lib.y6_linear_ce_workspace_bytes(C.byref(d), 1)):
+            assert (size > 0) == good, (rows, classes)
+        if not good:
+            assert b"rows" in hip_lib.y6_last_error()

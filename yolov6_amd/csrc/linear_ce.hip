@@ -1175,18 +1175,24 @@ template <class E>
 __global__ __launch_bounds__(1024) void bias_join_kernel(const float* __restrict__ part, int shares, int classes, typename E::S* __restrict__ db,
                                                          const float* up, const float* gmax, int mean, const int* count) {
     __shared__ float sh[1024 / kJoinCols][kJoinCols];
-    const int lane = threadIdx.x % kJoinCols, w = threadIdx.x / kJoinCols, c = blockIdx.x * kJoinCols + lane;
-    float s = 0.f;
-    if (c < classes) {
+    const int lane = threadIdx.x % kJoinCols, w = threadIdx.x / kJoinCols;
+    const float f = grad_factor<E>(up, gmax, mean, count);
+    for (int c0 = blockIdx.x * kJoinCols; c0 < classes; c0 += gridDim.x * kJoinCols) {
+        const int c = c0 + lane;
+        float s = 0.f;
+        if (c < classes) {
 #pragma unroll 8
-        for (int k = w; k < shares; k += 1024 / kJoinCols) s += part[(long long)k * classes + c];
-    }
-    sh[w][lane] = s;
-    __syncthreads();
-    if (w || c >= classes) return;
+            for (int k = w; k < shares; k += 1024 / kJoinCols) s += part[(long long)k * classes + c];
+        }
+        sh[w][lane] = s;
+        __syncthreads();
+        if (w == 0 && c < classes) {
 #pragma unroll
-    for (int k = 1; k < 1024 / kJoinCols; ++k) s += sh[k][lane];
-    db[c] = E::put(s * grad_factor<E>(up, gmax, mean, count));
+            for (int k = 1; k < 1024 / kJoinCols; ++k) s += sh[k][lane];
+            db[c] = E::put(s * f);
+        }
+        __syncthreads();
+    }
 }
 
 // ----------------------------------------------------------------------------------------------------------------------- host side
@@ -1369,10 +1375,14 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     return L;
 }
 
+// A launch has less than 2^32 threads: gather_kernel's 1024 for 16 rows, scores_kernel's 256 for 64 classes of few rows.
+constexpr long long kMaxThreads = (1ll << 32) - 1;
+constexpr long long kMaxRows = kMaxThreads / kGatherThreads * kGatherRows, kMaxClasses = kMaxThreads / 256 / 8 * 8 * kSide[kSmall];
+
 int check_desc(const y6_linear_ce_desc* d, const char* what) {
     Y6_REQUIRE(d, "%s: null argument", what);
     Y6_REQUIRE(d->dtype == Y6_F16 || d->dtype == Y6_BF16 || d->dtype == Y6_F32, "%s: dtype %d (fp16, bf16 or fp32)", what, d->dtype);
-    Y6_REQUIRE(d->rows >= 1 && d->rows <= (1 << 30) && d->classes >= 1 && d->classes <= (1 << 30) && d->width >= 1 && d->width <= (1 << 20),
+    Y6_REQUIRE(d->rows >= 1 && d->rows <= kMaxRows && d->classes >= 1 && d->classes <= kMaxClasses && d->width >= 1 && d->width <= (1 << 20),
                "%s: %lld rows x %d wide, %d classes", what, (long long)d->rows, d->width, d->classes);
     Y6_REQUIRE(d->x && d->weight && d->target, "%s: null argument", what);
     Y6_REQUIRE(d->x_pitch >= 0 && d->w_pitch >= d->width && d->w_pitch <= (1 << 21), "%s: pitches %lld, %lld", what, (long long)d->x_pitch, (long long)d->w_pitch);
@@ -1450,7 +1460,7 @@ int set_tiles(GemmArgs& g, unsigned* blocks) {
     g.tiles_m = ceil_div(g.M, T::BM), g.tiles_n = ceil_div(g.N, T::BN);
     if (g.splits < 1) g.splits = 1;
     const long long total = (long long)g.tiles_m * g.tiles_n * g.splits;
-    Y6_REQUIRE(total <= (1ll << 30), "linear_ce: %lld tiles", total);
+    Y6_REQUIRE((total + 7) / 8 * 8 * (T::NW * 64) <= kMaxThreads, "linear_ce: %lld tiles", total);
     *blocks = (unsigned)((total + 7) / 8 * 8);
     return Y6_OK;
 }
@@ -1496,7 +1506,9 @@ int launch_grads_tile(GemmArgs* x, GemmArgs* w, hipStream_t s) {
     unsigned bx = 0, bw = 0;
     int rc = set_tiles<T>(*x, &bx);
     if (rc == Y6_OK) rc = set_tiles<T>(*w, &bw);
-    if (rc == Y6_OK) rc = raise_lds((const void*)kern, T::kLds, raised);
+    if (rc != Y6_OK) return rc;
+    Y6_REQUIRE(((long long)bx + bw) * (T::NW * 64) <= kMaxThreads, "linear_ce: %lld tiles", (long long)bx + bw);
+    rc = raise_lds((const void*)kern, T::kLds, raised);
     if (rc != Y6_OK) return rc;
     hipLaunchKernelGGL(kern, dim3(bx + bw), dim3(T::NW * 64), T::kLds, s, *x, *w, bx, x->K / x->splits >= w->K / w->splits ? 1 : 0);
     Y6_LAUNCH_CHECK();
@@ -1616,7 +1628,7 @@ int backward(const Run& r) {
             Y6_LAUNCH_CHECK();
             }
             if (kept || shares > 1) {
-                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(ceil_div(vn, kJoinCols)), dim3(1024), 0, r.s, r.at<float>(L.bpart), shares, vn, db, d->grad_out, gmax,
+                hipLaunchKernelGGL(bias_join_kernel<E>, dim3(vn < 65536 * kJoinCols ? ceil_div(vn, kJoinCols) : 65536), dim3(1024), 0, r.s, r.at<float>(L.bpart), shares, vn, db, d->grad_out, gmax,
                                    mean, count);
                 Y6_LAUNCH_CHECK();
             }
