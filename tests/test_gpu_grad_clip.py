@@ -328,3 +328,16 @@ def test_gradients_with_gaps_that_share_a_part():
     norm = clip_grad_norm_(params, 0.5)
     assert abs(float(norm) - want) <= 2 * 2.0 ** -24 * want
     assert torch.allclose(buf.double(), before * (0.5 / (want + 1e-6)), rtol=4 * 2.0 ** -24, atol=0)
+
+
+def test_a_step_over_nothing_has_norm_zero():
+    import ctypes as C
+    from yolov6_amd import _lib
+    lib = _lib.load()
+    buf, norm = torch.ones(64, device=DEV), torch.full((), 7.0, device=DEV)
+    at = C.c_void_p(buf.data_ptr())
+    three = (C.c_float * 3)(0.1, 0.1, 0.1)
+    _lib.check(lib.y6_sgd_step_clipped(at, at, at, at, 0, three, three, 0.9, 1, 0, 1.0, None, None, 1.0, at, 256, C.c_void_p(norm.data_ptr()),
+                                       _lib.current_stream_ptr()), "sgd_step_clipped")
+    torch.cuda.synchronize()
+    assert float(norm) == 0.0 and bool((buf == 1).all())

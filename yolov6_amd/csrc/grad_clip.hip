@@ -474,8 +474,13 @@ extern "C" int y6_sgd_step_clipped(float* param, const float* grad, float* momen
     Y6_REQUIRE(((uintptr_t)param | (uintptr_t)grad | (uintptr_t)momentum_buf) % 16 == 0 && (uintptr_t)group % 4 == 0,
                "sgd_step_clipped: the arena is not aligned to 16 bytes");
     Y6_REQUIRE(n < ((size_t)1 << 40), "sgd_step_clipped: %zu elements", n);
-    if (n == 0) return Y6_OK;
     hipStream_t s = (hipStream_t)stream;
+    if (n == 0) {                      // the norm of nothing is 0, as y6_grad_norm's
+        if (!norm) return Y6_OK;
+        hipLaunchKernelGGL(grad_join_kernel, dim3(1), dim3(kThreads), 0, s, Y6_NORM_L2, (double*)workspace, 0, norm);
+        Y6_LAUNCH_CHECK();
+        return Y6_OK;
+    }
     void* const grads[1] = {(void*)grad};
     const int64_t numels[1] = {(int64_t)n};
     const int32_t types[1] = {Y6_F32};
