@@ -280,3 +280,29 @@ def test_recompute(dtype, reduction, smoothing, monkeypatch):
     loss = _op_loss(leaves, ops[3], -100, smoothing, reduction, True)
     got = torch.autograd.grad(loss, leaves, up)
     assert all(torch.equal(a, c) for a, c in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,v", [(70, 32, 300), (300, 64, 1500), (2100, 72, 33000), (4100, 256, 4200)])
+def test_classes_at_the_lowest_value_fill_tiles(n, d, v, dtype):
+    """A bias of the type's lowest value switches classes off, whole tiles of them: finite everywhere, with and without gradients.  All of them
+    at it: as likely as each other, log(classes), off by 8 * 2^-24 of 1 + that.  One at the highest: 0 or that value."""
+    x, w, b, t = _inputs(n, d, v, dtype, True, seed=v)
+    lo, hi = 20, v - 30
+    b[lo:hi] = torch.finfo(dtype).min
+    t[(t >= lo) & (t < hi)] = 5
+    _check(x, w, b, t, kept=(d >= 128))
+    rows = _loss((x, w, b), t, reduction="none")
+    want = torch.nn.functional.cross_entropy(x.double() @ w.double().t() + b.double(), t, reduction="none")
+    from tests.test_gpu_linear_ce import _logit_error
+    assert bool(((rows.double() - want).abs() <= 2 * _logit_error(x, w, b)).all())
+    every = torch.full_like(b, torch.finfo(dtype).min)
+    rows = _loss((x, w, every), t, reduction="none")
+    want = torch.where(t == -100, 0.0, math.log(v))
+    assert bool(((rows.double() - want).abs() <= 8 * 2.0 ** -24 * (1 + want)).all())
+    one = torch.zeros_like(b)
+    one[lo] = torch.finfo(dtype).max
+    t[::3] = lo
+    rows = _loss((x / 64, w, one), t, reduction="none")
+    want = torch.where((t == -100) | (t == lo), 0.0, torch.finfo(dtype).max)
+    assert bool(((rows.double() - want).abs() <= 2.0 ** -23 * want).all())

@@ -809,7 +809,20 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                     all = ((sum[0] + sum[1]) + (sum[2] + sum[3])) * E::kKeepUnit;
                     all += __shfl_xor(all, 32);
                 } else {
-                    const float m2 = top == -INFINITY ? 0.f : top * kLog2e;
+                    float base = top == -INFINITY ? 0.f : top;
+                    if (__ballot(!(fabsf(base) <= 1e38f))) {
+                        // base log2 e would leave fp32's range (a tile whose classes a bias of the type's lowest value switches off): such rows
+                        // have it subtracted first
+                        const float far = fabsf(base) <= 1e38f ? 0.f : base;
+#pragma unroll
+                        for (int i = 0; i < FM; ++i) {
+                            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                            for (int q = 0; q < 16; ++q) acc[i][j][q] -= far;
+                        }
+                        base = far == 0.f ? base : 0.f;
+                    }
+                    const float m2 = base * kLog2e;
                     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int i = 0; i < FM; ++i)
@@ -818,7 +831,7 @@ __global__ __launch_bounds__(T::NW * 64, T::BPC * T::NW / 4) void scores_kernel(
                     all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     all += __shfl_xor(all, 32);
                     // (m2 was rounded: the terms are relative to it, the sum is not)
-                    all = top == -INFINITY ? 0.f : all * exp2_fast(-fmaf(top, kLog2e, -m2));
+                    all = top == -INFINITY ? 0.f : all * exp2_fast(-fmaf(base, kLog2e, -m2));
                 }
                 if (live && half == 0) {
                     e.part_m[o] = top;
