@@ -92,7 +92,7 @@ def test_an_upstream_gradient_that_is_not_finite_stays_in_its_row(n, d, v, dtype
         assert not bool(got[0][rows].isfinite().any()) and int(got[0][~rows].count_nonzero()) == 0
 
 
-@pytest.mark.parametrize("n", [4096, 4097, 8192 + 15, 600_001, (1 << 22) + 4097])
+@pytest.mark.parametrize("n", [4096, 4097, 8192 + 15, 600_001, 1 << 20, (1 << 20) + 1, (1 << 22) + 4097])
 @pytest.mark.parametrize("share", [0.0, 0.5, 0.999])
 def test_many_rows(n, share):
     """Labelled rows are counted block by block: two classes and one feature, so that value and gradient have closed forms, at rows before, at

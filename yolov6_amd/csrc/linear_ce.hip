@@ -99,14 +99,15 @@ __device__ __forceinline__ float log2_fast(float v) { return __builtin_amdgcn_lo
 // ------------------------------------------------------------------------------------------------------------- rows with a label
 // Block b of gather_kernel takes rows [16 b, 16 b + 16): finds how many labelled rows lie before them, then copies its labelled rows to
 // their places, each padded with zeros to a multiple of 16 bytes, a row per wave.  Up to kCountRows rows it counts them itself (4 loads a
-// thread at most).  Above, count_kernel counts kCountRows rows a block and leaves each 16 rows' place within them and the block's total; a
-// gather block adds up the totals before its own, one load a thread at most, and with more than kTotals of them scan_kernel has done that
-// once: the work grows with the rows (value of 2^20 rows x 8 x 2 classes, fp16, 0.51 ms, of 2^23 rows 3.85; with every block adding the
+// thread at most).  Above, count_kernel counts kTotalRows rows a block and leaves each 16 rows' place within them and the block's total; a
+// gather block's first wave adds up the totals before its own, 16 loads a lane at most, and with more than kTotals of them scan_kernel has
+// done that once: the work grows with the rows (value of 2^20 rows x 8 x 2 classes, fp16, 0.49 ms, of 2^23 rows 3.80; with every block adding the
 // counts of all blocks before it 0.89 and 30.7).
 constexpr int kGatherRows = 16;
 constexpr int kGatherThreads = kGatherRows * 64;
 constexpr int kCountRows = 4096;
-constexpr int kTotals = kGatherThreads;
+constexpr int kTotalRows = 1024;
+constexpr int kTotals = 1024;
 
 struct GatherArgs {
     const char* x;
@@ -115,8 +116,8 @@ struct GatherArgs {
     long long ignore;
     int rows, width, classes;
     int vec;                       // rows start at 16-byte addresses, and 16-bit ones are multiples of 16 bytes
-    const int* seg;                // above kCountRows rows: labelled rows before each 16 within their kCountRows; or null
-    const int* total;              // of each kCountRows, or, `scanned`, of all before them
+    const int* seg;                // above kCountRows rows: labelled rows before each 16 within their kTotalRows; or null
+    const int* total;              // of each kTotalRows, or, `scanned`, of all before them
     int scanned;
     char* xc;
     long long cpitch, plane;       // bytes between rows, planes
@@ -147,26 +148,23 @@ __device__ __forceinline__ int wave_scan(int v, int lane) {           // inclusi
     return v;
 }
 
-__global__ __launch_bounds__(kCountRows / kGatherRows) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg,
-                                                                         int segs, int* __restrict__ total) {
-    constexpr int T = kCountRows / kGatherRows;                          // threads; each has 16 rows in the end
-    __shared__ int n16[T], wave_sum[T / 64];
-    const int r0 = blockIdx.x * kCountRows, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__global__ __launch_bounds__(256) void count_kernel(const int64_t* __restrict__ target, long long ignore, int rows, int* __restrict__ seg, int segs,
+                                                    int* __restrict__ total) {
+    constexpr int S = kTotalRows / kGatherRows;
+    static_assert(S == 64, "one wave adds them up");
+    __shared__ int n16[S];
+    const int r0 = blockIdx.x * kTotalRows, lane = threadIdx.x & 63;
 #pragma unroll
-    for (int i = 0; i < kGatherRows; ++i) {
-        const int k = i * T + threadIdx.x, r = rows - r0 > k ? r0 + k : -1;
+    for (int i = 0; i < kTotalRows / 256; ++i) {
+        const int k = i * 256 + threadIdx.x, r = rows - r0 > k ? r0 + k : -1;
         const unsigned long long m = __ballot(r >= 0 && target[r >= 0 ? r : 0] != ignore);
         if (lane % kGatherRows == 0) n16[k / kGatherRows] = __popcll((m >> lane) & ((1ull << kGatherRows) - 1));
     }
     __syncthreads();
-    const int mine = n16[threadIdx.x], upto = wave_scan(mine, lane);
-    if (lane == 63) wave_sum[wave] = upto;
-    __syncthreads();
-    int before = upto - mine;
-    for (int w = 0; w < wave; ++w) before += wave_sum[w];
-    const int s = r0 / kGatherRows + threadIdx.x;
-    if (s < segs) seg[s] = before;
-    if (threadIdx.x == T - 1) total[blockIdx.x] = before + mine;
+    if (threadIdx.x >= S) return;
+    const int mine = n16[lane], upto = wave_scan(mine, lane), s = r0 / kGatherRows + lane;
+    if (s < segs) seg[s] = upto - mine;
+    if (lane == S - 1) total[blockIdx.x] = upto;
 }
 
 // totals -> sums of those before each; one block, a chunk at a time
@@ -217,11 +215,17 @@ __global__ __launch_bounds__(kGatherThreads) void gather_kernel(const GatherArgs
     if (!a.seg) {
         for (int i = threadIdx.x; i < r0; i += kGatherThreads) before += a.target[i] != a.ignore ? 1 : 0;
         before = block_count(before, sh);
-    } else {
-        const int c = r0 / kCountRows;
-        if (a.scanned) before = a.total[c];
-        else before = block_count((int)threadIdx.x < c ? a.total[threadIdx.x] : 0, sh);
-        before += a.seg[blockIdx.x];
+    } else if (threadIdx.x < 64) {     // (only the first wave asks)
+        const int c = r0 / kTotalRows, in = a.seg[blockIdx.x];
+        if (a.scanned) {
+            before = a.total[c];
+        } else {
+#pragma unroll 4
+            for (int i = threadIdx.x; i < c; i += 64) before += a.total[i];
+#pragma unroll
+            for (int d = 32; d > 0; d >>= 1) before += __shfl_xor(before, d);
+        }
+        before += in;
     }
     if (threadIdx.x < 64) {
         const int r = r0 + threadIdx.x;
@@ -1360,7 +1364,7 @@ Layout layout(const y6_linear_ce_desc* d, bool backward) {
     L.kept_all = at;
     at = 0;
     if (!backward) {
-        L.seg = take(n > kCountRows ? ((size_t)ceil_div(n, kGatherRows) + ceil_div(n, kCountRows)) * 4 : 0);
+        L.seg = take(n > kCountRows ? ((size_t)ceil_div(n, kGatherRows) + ceil_div(n, kTotalRows)) * 4 : 0);
         L.scores = L.kept_scores;
         // one block for all rows, which then also adds up the loss, where that is 16 rounds of its threads at most
         L.places = 1;
@@ -1429,11 +1433,10 @@ int launch_gather(const Run& r) {
     a.rowmap = r.kept<int>(r.L.rowmap), a.place = r.kept<int>(r.L.place), a.label = r.kept<int>(r.L.label), a.count = r.kept<int>(r.L.count);
     const int segs = ceil_div(d->rows, kGatherRows);
     if (d->rows > kCountRows) {
-        const int totals = ceil_div(d->rows, kCountRows);
+        const int totals = ceil_div(d->rows, kTotalRows);
         int* const total = r.at<int>(r.L.seg) + segs;
         a.seg = r.at<int>(r.L.seg), a.total = total, a.scanned = totals > kTotals;
-        hipLaunchKernelGGL(count_kernel, dim3(totals), dim3(kCountRows / kGatherRows), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg),
-                           segs, total);
+        hipLaunchKernelGGL(count_kernel, dim3(totals), dim3(256), 0, r.s, d->target, (long long)d->ignore_index, a.rows, r.at<int>(r.L.seg), segs, total);
         Y6_LAUNCH_CHECK();
         if (a.scanned) {
             hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(1024), 0, r.s, total, totals);
