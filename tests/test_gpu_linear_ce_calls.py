@@ -306,3 +306,40 @@ def test_classes_at_the_lowest_value_fill_tiles(n, d, v, dtype):
     rows = _loss((x / 64, w, one), t, reduction="none")
     want = torch.where((t == -100) | (t == lo), 0.0, torch.finfo(dtype).max)
     assert bool(((rows.double() - want).abs() <= 2.0 ** -23 * want).all())
+
+
+_FIRST = """
+import torch
+from yolov6_amd import clip_grad_norm_, linear_cross_entropy
+x, w, b, t = (torch.randn(4100, 256, device="cuda").{t}(), torch.randn(4200, 256, device="cuda").mul(0.1).{t}(), torch.randn(4200, device="cuda").{t}(),
+              torch.randint(0, 4200, (4100,), device="cuda"))
+leaves = [o.requires_grad_() for o in (x, w, b)]
+p = torch.nn.Parameter(torch.zeros(1000, device="cuda"))
+first = torch.randn(1000, device="cuda")
+p.grad = first.clone()
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    held = torch.autograd.grad(linear_cross_entropy(x, w, t, b), leaves)
+    norm = clip_grad_norm_([p], 1.0)
+for _ in range(3):
+    p.grad.copy_(first)
+    g.replay()
+    torch.cuda.synchronize()
+    want = torch.autograd.grad(linear_cross_entropy(x, w, t, b), leaves)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(held, want))
+    assert abs(float(norm) - float(first.double().norm())) <= 2.0 ** -23 * float(norm)
+print("as the first call")
+"""
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float"])
+def test_captured_as_the_first_call_of_a_process(dtype):
+    """No warm-up: the library, its kernels' limits and the extension come up inside the capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FIRST.replace("{t}", dtype)], cwd=root, capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "as the first call" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]

@@ -22,3 +22,17 @@ def test_under_guard_allocator(mode, tmp_path):
     assert r.returncode == 0, f"rc {r.returncode}\n--- stdout tail ---\n{r.stdout[-3000:]}\n--- stderr tail ---\n{r.stderr[-3000:]}"
     got_mode, blocks = open(mark).read().split()
     assert got_mode == mode and int(blocks) > 1000, (got_mode, blocks)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", ["end", "start"])
+def test_calls_under_guard_allocator(mode, tmp_path):
+    """The same of test_gpu_linear_ce_calls.py: the counts of many rows, operands at other addresses, tiles that are switched off."""
+    mark = str(tmp_path / "guard_mark.txt")
+    env = dict(os.environ, Y6_GUARD_ALLOC=mode, Y6_GUARD_ALLOC_MARK=mark)
+    r = subprocess.run([sys.executable, "-m", "pytest", "-q", "-x", "-m", "gpu", "-p", "no:cacheprovider", "--timeout", "80", "tests/test_gpu_linear_ce_calls.py",
+                        "-k", "many_rows or elsewhere or lowest or upstream or bias_gradient"],
+                       capture_output=True, text=True, timeout=110, cwd=ROOT, env=env)
+    assert r.returncode == 0, f"rc {r.returncode}\n--- stdout tail ---\n{r.stdout[-3000:]}\n--- stderr tail ---\n{r.stderr[-3000:]}"
+    got_mode, blocks = open(mark).read().split()
+    assert got_mode == mode and int(blocks) > 1000, (got_mode, blocks)
