@@ -133,3 +133,11 @@ def test_sizes_whose_launches_would_leave_32_bits_are_refused(hip_lib):
             assert (size > 0) == good, (rows, classes)
         if not good:
             assert b"rows" in hip_lib.y6_last_error()
+
+
+def test_sparse_gradients_are_refused(hip_lib):
+    p = torch.nn.Parameter(torch.zeros(4, 3))
+    p.grad = torch.sparse_coo_tensor([[1]], [[1.0, 2.0, 3.0]], (4, 3))
+    for call in (lambda: clip_grad_norm_([p], 1.0), lambda: grad_norm([p.grad])):
+        with pytest.raises(RuntimeError, match="dense"):
+            call()

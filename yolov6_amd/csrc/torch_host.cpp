@@ -7,6 +7,7 @@
 // the kernels were 60.
 #include <Python.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
@@ -51,8 +52,10 @@ int type_code(at::ScalarType t) {
 void require_gpu(const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda(), "yolov6_amd: ", name, " must live on a ROCm device (got ", t.device(), "); the hot path has no CPU fallback");
 }
-// a dual tensor does not require a gradient, and its tangent would be lost without a word
-void refuse_forward_mode(const Tensor& t, const char* what) {
+// A dual tensor does not require a gradient, and its tangent would be lost without a word.  (Outside a dual level there is none, and
+// asking each of 489 gradients took 7 us.)
+bool dual_level() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
+void refuse_dual(const Tensor& t, const char* what) {
     TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "yolov6_amd: ", what, " has no forward mode derivative (a dual tensor was given)");
 }
 Tensor bytes_on(const Tensor& like, size_t n) { return at::empty({(int64_t)n}, like.options().dtype(at::kByte).requires_grad(false)); }
@@ -211,7 +214,8 @@ struct Operands {
 Operands operands(const Tensor& features, const Tensor& weight, const Tensor& target, const std::optional<Tensor>& bias_in, int64_t ignore, double smoothing,
                   const std::string& reduction, bool recompute) {
     const Tensor bias = bias_in.has_value() ? *bias_in : Tensor();
-    for (const Tensor& t : {features, weight, bias}) refuse_forward_mode(t, "linear_cross_entropy");
+    if (dual_level())
+        for (const Tensor* t : {&features, &weight, &bias}) refuse_dual(*t, "linear_cross_entropy");
     const int64_t code = reduction == "none" ? Y6_REDUCE_NONE : reduction == "sum" ? Y6_REDUCE_SUM : reduction == "mean" ? Y6_REDUCE_MEAN : -1;
     TORCH_CHECK(code >= 0, "yolov6_amd: linear_cross_entropy reduction '", reduction, "' ('mean', 'sum' or 'none')");
     TORCH_CHECK(smoothing >= 0.0 && smoothing <= 1.0, "yolov6_amd: linear_cross_entropy label_smoothing ", smoothing, " is not in [0, 1]");
@@ -290,8 +294,9 @@ struct List {
     int64_t elements = 0;
     List(const std::vector<Tensor>& grads, int norm) {
         const auto device = grads[0].device();
+        const bool dual = dual_level();
         for (const Tensor& g : grads) {
-            refuse_forward_mode(g, "the gradients' norm");
+            if (dual) refuse_dual(g, "the gradients' norm");
             const int code = g.layout() == at::kStrided ? type_code(g.scalar_type()) : -1;
             TORCH_CHECK(code >= 0, "yolov6_amd: gradients must be dense fp16, bf16 or fp32 tensors (got ", g.scalar_type(), ", ", g.layout(), ")");
             TORCH_CHECK(g.device() == device, "yolov6_amd: gradients on ", device, " and ", g.device(), ": one norm is taken on one device");
@@ -325,12 +330,14 @@ Tensor clip_grad_norm(const py::object& parameters, double max_norm, int norm, b
     const at::NoGradGuard off;
     const auto grads = tensors_of(parameters.ptr(), true);
     if (grads.empty()) return at::zeros({});
-    for (const Tensor& g : grads) TORCH_CHECK(!g.requires_grad(), "yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place");
-    for (const Tensor& g : grads)
-        TORCH_CHECK(at::has_internal_overlap(g) != at::MemOverlap::Yes, "yolov6_amd: a gradient whose elements share memory is not scaled in place");
     // (y6_grad_clip refuses dense ones that overlap; those with gaps are scaled as copies, and it does not see them)
     bool gaps = false;
-    for (const Tensor& g : grads) gaps |= !g.is_non_overlapping_and_dense();
+    for (const Tensor& g : grads) {
+        TORCH_CHECK(!g.requires_grad(), "yolov6_amd: gradients that carry a graph (create_graph=True) are not scaled in place");
+        if (g.layout() != at::kStrided || g.is_non_overlapping_and_dense()) continue;            // (List refuses the former)
+        gaps = true;
+        TORCH_CHECK(at::has_internal_overlap(g) != at::MemOverlap::Yes, "yolov6_amd: a gradient whose elements share memory is not scaled in place");
+    }
     std::unordered_set<const void*> starts;
     if (gaps)
         for (const Tensor& g : grads)
