@@ -8,9 +8,11 @@
 // sums, then the scaling, whose blocks each add the partial sums again in the same fixed order (at most kJoin of them, out of L2: a
 // third launch to add them once costs more).  No atomics: the same gradients give the same bits.
 //
-// Measured: 489 fp32 tensors of 60 M elements (236 MB), the norm alone 2 x 18 us (6.5 TB/s, half of it from the cache), with the scaling's
-// launches 59-65 us where the norm is below the bound (nothing is written then); 112 M parameters stepped with a clipped gradient 549 us,
-// 2.8 GB at 5.1 TB/s, what a copy of 1 GB reaches; 40 tensors of at most 5000 elements 14 us, two launches and their host side.
+// Measured: 489 fp32 tensors of 29.5 M elements (118 MB).  The norm's two launches (330 and 159 tensors) 19 and 10 us, 4.1 TB/s although the data
+// lies in the last-level cache: a thread asks for 64 bytes, converts and adds them, and only then asks for more.  The scaling's two 34 and 19 us
+// where they write (236 MB read and written, 4.4 TB/s), 4-5 each where the factor is 1 and they read no gradient.  The call: the norm alone
+// 33 us, clipped 103, not clipped 57-67.  112 M parameters stepped with a clipped gradient 549 us, 2.8 GB at 5.1 TB/s, what a copy of 1 GB
+// reaches (the norm's part 449 MB in 120 us, 3.7 TB/s); 40 tensors of at most 5000 elements 14 us, two launches and their host side.
 //
 // Squares and sums are doubles: the square of an fp32 / bf16 gradient leaves the range of a float (1e20, 1e-23), the sum of 1e8
 // of them its precision, and the conversions hide behind the loads.  No sum of fp32 squares reaches infinity in double: the

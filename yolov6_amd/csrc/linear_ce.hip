@@ -1,4 +1,4 @@
-// linear_ce.hip - softmax cross entropy of a linear classifier, value and gradient, without keeping the logits.
+// linear_ce.hip - softmax cross entropy of a linear classifier, value and gradient, tile by tile: the logits are never stored.
 //
 //   z_nv = x_n . W_v + b_v          lse_n = log sum_v exp z_nv
 //   loss_n = lse_n - (1-e) z_n,t(n) - (e/V) sum_v z_nv               (label smoothing e; rows with ignore_index: 0)
@@ -13,8 +13,8 @@
 //               dx += dz W[piece] and dW[piece] = dz^T x in one launch (gemm_tile)
 // so a call holds one piece of dz (kPieceBytes) and what is kept, which is as large as logits of the operands' type up to kKeepBytes; a
 // caller who would rather have the memory, or the one rounding less, says so (Y6_CE_RECOMPUTE).  A kept exponential is rounded and dz once more
-// (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9 ms, 0.95
-// PFLOP/s over the three products; without the kept ones 8.1.  torch's product of such operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on
+// (twice u of a probability; the label's own entry has one rounding, from RowStat).  8192 rows x 131072 classes x 1024, bf16: 6.9-7.1 ms, 0.91 to
+// 0.94 PFLOP/s over the three products; without the kept ones 8.2.  torch's product of such operands reaches 1.01 (K = 1024) to 1.29 (8192^3) on
 // the same card, which lowers its clock under either.
 // Labelled rows are gathered first (gather_kernel): rows with ignore_index cost nothing, and an infinity or a NaN in one of them reaches no
 // gradient.  What the forward gathered, and its statistics, are kept for the backward.
@@ -1108,9 +1108,9 @@ __global__ __launch_bounds__(256) void bias_part_kernel(const char* __restrict__
     }
 }
 // dz of a piece from the exponentials that the forward kept: dz = c (e 2^((tile's largest - top) log2 e - log2s) - share), the label's from
-// its RowStat.  A wave takes 512 classes, 16 bytes a lane, and 16 rows, four at a time, so that it also has their sum, which becomes db: the
-// block adds its four waves', in order.  Memory bounds it: 128 MB to 128 MB in 53 us, 4.9 TB/s, where forming the scores of 1024 features again
-// took 150.  (32 rows a wave: 37 instead of 31 us at 1383 x 25088.)
+// its RowStat.  A wave takes 512 classes, 16 bytes a lane, and 4, 8 or 16 rows (layout), four at a time, so that it also has their sum, which
+// becomes db: the block adds its four waves', in order.  Memory bounds it: 128 MB to 128 MB in 48-53 us, 5-5.3 TB/s, where forming the scores of
+// 1024 features again took 150.  (32 rows a wave: 37 instead of 31 us at 1383 x 25088.)
 constexpr int kKeptCols = 512;
 struct KeptArgs {
     const char* e;                 // the piece's first class
