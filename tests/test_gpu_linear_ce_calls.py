@@ -343,3 +343,35 @@ def test_captured_as_the_first_call_of_a_process(dtype):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     r = subprocess.run([sys.executable, "-c", _FIRST.replace("{t}", dtype)], cwd=root, capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "as the first call" in r.stdout, r.stdout[-2000:] + r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("which", ["weight", "saved", "bias"])
+@pytest.mark.parametrize("change", ["host", "shape", "type"])
+def test_what_a_hook_must_not_hand_back(which, change):
+    """Another device, shape or type than it was given: refused before anything is launched."""
+    ops = _inputs(64, 40, 50, torch.bfloat16, True, seed=3)
+    leaves = _leaves(ops, torch.bfloat16)
+
+    def unpack(t):
+        mine = {"weight": t.dim() == 2, "saved": t.dtype == torch.uint8, "bias": t.dim() == 1 and t.dtype == torch.bfloat16}[which]
+        return t if not mine else t.cpu() if change == "host" else t[:-1] if change == "shape" else t.half() if t.dtype != torch.uint8 else t.to(torch.int8)
+
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        loss = _loss(leaves, ops[3])
+    with pytest.raises(RuntimeError, match="yolov6_amd"):
+        torch.autograd.grad(loss, leaves)
+    torch.cuda.synchronize()
+
+
+def test_what_the_backward_op_refuses():
+    import yolov6_amd.torch_ops  # noqa: F401
+    x, w, b, t = _inputs(64, 40, 50, torch.bfloat16, True, seed=3)
+    loss, saved = torch.ops.yolov6_hip.linear_cross_entropy(x, w, t, b, -100, 0.0, "none")
+    back = torch.ops.yolov6_hip.linear_cross_entropy_backward
+    good = torch.ones_like(loss)
+    back(good, x, w, t, b, saved, -100, 0.0, "none", False)
+    for grad, kept in ((good[:-1], saved), (good.cpu(), saved), (good, saved.cpu()), (good, saved[:-256]), (good, saved[::2]), (good, saved.to(torch.int8)),
+                       (torch.ones((), device=DEV), saved)):
+        with pytest.raises(RuntimeError, match="yolov6_amd"):
+            back(grad, x, w, t, b, kept, -100, 0.0, "none", False)
+    torch.cuda.synchronize()

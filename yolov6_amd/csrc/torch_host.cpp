@@ -52,6 +52,11 @@ int type_code(at::ScalarType t) {
 void require_gpu(const Tensor& t, const char* name) {
     TORCH_CHECK(t.is_cuda(), "yolov6_amd: ", name, " must live on a ROCm device (got ", t.device(), "); the hot path has no CPU fallback");
 }
+std::string shape(const Tensor& t) {
+    std::ostringstream s;
+    s << t.sizes();
+    return s.str();
+}
 // A dual tensor does not require a gradient, and its tangent would be lost without a word.  (Outside a dual level there is none, and
 // asking each of 489 gradients took 7 us.)
 bool dual_level() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
@@ -112,9 +117,19 @@ std::tuple<Tensor, Tensor> ce_forward(const Tensor& x, const Tensor& w, const Te
 
 std::tuple<Tensor, Tensor, Tensor> ce_backward(const Tensor& grad, int64_t n, const Tensor& w, const Tensor& b, const Tensor& saved, const Options& o, bool want_x,
                                                bool want_w, bool want_b) {
+    // (saved-tensor hooks, or a caller of the op, may hand over anything: what the kernels would read by its address is looked at here)
+    require_gpu(w, "weight");
+    TORCH_CHECK(w.dim() == 2 && type_code(w.scalar_type()) >= 0 && w.layout() == at::kStrided, "yolov6_amd: linear_cross_entropy's backward is given a weight ", shape(w));
+    const int64_t width = w.size(1), classes = w.size(0);
+    for (const auto& [name, t] : {std::pair<const char*, const Tensor&>{"gradient", grad}, {"saved bytes", saved}, {"bias", b}})
+        TORCH_CHECK(!t.defined() || (t.device() == w.device() && t.layout() == at::kStrided), "yolov6_amd: linear_cross_entropy's backward is given ", name, " on ",
+                    t.device(), ", the weight on ", w.device());
+    TORCH_CHECK(grad.numel() == (o.reduction == Y6_REDUCE_NONE ? n : 1) && saved.scalar_type() == at::kByte && saved.is_contiguous() &&
+                    (!b.defined() || (b.dim() == 1 && b.size(0) == classes && b.scalar_type() == w.scalar_type())),
+                "yolov6_amd: linear_cross_entropy's backward of ", n, " rows is given a gradient ", shape(grad), ", saved bytes ", shape(saved), " of ",
+                saved.scalar_type(), b.defined() ? ", a bias " + shape(b) : std::string());
     want_b = want_b && b.defined();
     const auto like = w.options().requires_grad(false);
-    const int64_t width = w.size(1), classes = w.size(0);
     const c10::DeviceGuard guard(w.device());
     if (n == 0) {
         return {want_x ? at::zeros({0, width}, like) : Tensor(), want_w ? at::zeros({classes, width}, like) : Tensor(),
@@ -156,6 +171,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         // (neither features nor labels: the backward reads what the forward gathered of them, and they may go)
         ctx->save_for_backward({w, b, saved});
         ctx->saved_data["rows"] = x.size(0);
+        ctx->saved_data["width"] = w.size(1);
+        ctx->saved_data["classes"] = w.size(0);
+        ctx->saved_data["type"] = (int64_t)w.scalar_type();
         ctx->saved_data["ignore"] = ignore;
         ctx->saved_data["smoothing"] = smoothing;
         ctx->saved_data["reduction"] = reduction;
@@ -169,6 +187,9 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         variable_list out;
         {
             const at::AutoGradMode off(false);
+            TORCH_CHECK(s[0].dim() == 2 && s[0].size(0) == ctx->saved_data["classes"].toInt() && s[0].size(1) == ctx->saved_data["width"].toInt() &&
+                            (int64_t)s[0].scalar_type() == ctx->saved_data["type"].toInt(),
+                        "yolov6_amd: linear_cross_entropy's weight comes back from a saved-tensor hook as ", shape(s[0]), " of ", s[0].scalar_type());
             auto [dx, dw, db] = ce_backward(grads[0], ctx->saved_data["rows"].toInt(), s[0], s[1], s[2], o, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                             s[1].defined() && ctx->needs_input_grad(2));
             out = {dx, dw, db};
@@ -182,12 +203,6 @@ struct LinearCrossEntropy : torch::autograd::Function<LinearCrossEntropy> {
         return {out[0], out[1], out[2], Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
-
-std::string shape(const Tensor& t) {
-    std::ostringstream s;
-    s << t.sizes();
-    return s.str();
-}
 
 // While a stream is captured, a leaf's gradient accumulator must not be one that a living eager graph made on the default stream: the
 // engine would make that stream wait for the captured one, which it cannot join, and the capture's end brings the process down.  (Another
